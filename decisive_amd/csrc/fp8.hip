@@ -1,0 +1,392 @@
+// fp8.hip -- products on 8-bit floating point weights with a scale for each
+// 128 x 128 block (fp8.hpp has the form and the layout).
+//
+//   y[i, j] = sum over 128-blocks b of sx[i, b] sw[j / 128, b] dot_b(i, j)
+//
+// dot_b is the dot of 128 codes. The blocks are folded in f32, in order of b:
+// acc = fma(dot_b, sx * sw, acc).
+#include <algorithm>
+
+#include "../../include/decisive_rocm.h"
+#include "fp8.hpp"
+#include "tiles.hpp"
+
+struct dz_fp8_weight {
+    dz::Fp8Weight w;
+    int device = 0;
+};
+
+namespace dz {
+
+int32_t ctx_fail(dz_ctx *ctx, int32_t code, const std::string &msg);
+int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what);
+hipStream_t ctx_stream(dz_ctx *ctx);
+int *ctx_flag(dz_ctx *ctx);
+int ctx_device(dz_ctx *ctx);
+int ctx_variant(dz_ctx *ctx, const char *family);
+int32_t ctx_workspace(dz_ctx *ctx, size_t bytes, void **out);
+int32_t ctx_launched(dz_ctx *ctx, const char *what);
+int32_t ctx_flag_value(dz_ctx *ctx, int *value);
+
+namespace {
+
+// ---- weights -------------------------------------------------------------------
+
+// One thread per 16-byte piece of the native layout.
+__global__ __launch_bounds__(256) void fp8_retile_kernel(const uint8_t *__restrict__ codes, int rows, int cols,
+                                                         int np, int kbs, uint8_t *__restrict__ dst,
+                                                         size_t tile_bytes, size_t kb_bytes, int *bad) {
+    // consecutive threads take consecutive pieces of a row: whole lines are read
+    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < (size_t)np * kbs * 8; id += gridDim.x * (size_t)256) {
+        const int piece = (int)(id % 8), kb = (int)(id / 8 % kbs), n = (int)(id / 8 / kbs);
+        const int h = piece / 4, g = piece % 4, k0 = kb * 128 + 16 * piece;
+        const uint8_t *src = codes + (size_t)n * cols + k0;
+        uint32_t w[4] = {0, 0, 0, 0};
+        bool nan = false;
+        for (int e = 0; e < 16; e++) {
+            const uint32_t c = n < rows && k0 + e < cols ? src[e] : 0u;
+            nan |= (c & 127u) == 127u;
+            w[e / 4] |= c << (8 * (e % 4));
+        }
+        if (nan) atomicOr(bad, 1);
+        *(uint4_t *)(dst + (size_t)(n / 16) * tile_bytes + (size_t)kb * kb_bytes + h * 1024 + (g * 16 + n % 16) * 16) =
+            uint4_t{w[0], w[1], w[2], w[3]};
+    }
+}
+
+__global__ __launch_bounds__(256) void fp8_scales_kernel(const float *__restrict__ src, float *__restrict__ dst,
+                                                         size_t n, int *bad) {
+    const size_t id = blockIdx.x * (size_t)256 + threadIdx.x;
+    if (id >= n) return;
+    const float v = src[id];
+    if (!(v >= 0.0f && v <= 3.4028235e38f)) atomicOr(bad, 1);
+    dst[id] = v;
+}
+
+// One block of threads per 128 x 128 block of values: its scale
+// max(max|v| / 448, 2^-126) and its codes, as fp8_quantize8 makes them.
+template <class T>
+__global__ __launch_bounds__(256) void fp8_quantize_weight_kernel(const T *__restrict__ values, int rows, int cols,
+                                                                  int np, int kbs, uint8_t *__restrict__ codes,
+                                                                  float *__restrict__ scales, int *bad) {
+    const int kb = blockIdx.x % kbs, nb = blockIdx.x / kbs;
+    __shared__ uint32_t part[4];
+    uint32_t most = 0;
+    for (int i = threadIdx.x; i < 128 * 128; i += 256) {
+        const int n = nb * 128 + i / 128, k = kb * 128 + i % 128;
+        if (n >= rows || k >= cols) continue;
+        const uint32_t b = __builtin_bit_cast(uint32_t, (float)values[(size_t)n * cols + k]) & 0x7fffffffu;
+        most = most > b ? most : b;
+    }
+    for (int o = 32; o; o >>= 1) {
+        const uint32_t other = (uint32_t)__shfl_xor((int)most, o);
+        most = most > other ? most : other;
+    }
+    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = most;
+    __syncthreads();
+    for (int i = 0; i < 4; i++) most = most > part[i] ? most : part[i];
+    if (most >= 0x7f800000u) {
+        if (threadIdx.x == 0) atomicOr(bad, 1);
+        return;
+    }
+    const float s = fmaxf(__fdiv_rn(word_as_float(most), 448.0f), 1.17549435e-38f);
+    if (threadIdx.x == 0) scales[(size_t)nb * kbs + kb] = s;
+    for (int i = threadIdx.x; i < 128 * 8; i += 256) {
+        const int n = nb * 128 + i / 8, piece = i % 8, k0 = kb * 128 + 16 * piece;
+        if (n >= np) continue;
+        uint32_t w[4];
+        for (int e = 0; e < 16; e += 4) {
+            float q[4];
+            for (int f = 0; f < 4; f++)
+                q[f] = n < rows && k0 + e + f < cols ? __fdiv_rn((float)values[(size_t)n * cols + k0 + e + f], s) : 0.0f;
+            int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+            w[e / 4] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], p, true);
+        }
+        *(uint4_t *)(codes + ((size_t)(n / 16) * kbs + kb) * 2048 + piece / 4 * 1024 + (piece % 4 * 16 + n % 16) * 16) =
+            uint4_t{w[0], w[1], w[2], w[3]};
+    }
+}
+
+__global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t *__restrict__ codes,
+                                                          const float *__restrict__ scales, int rows, int cols,
+                                                          int kbs, float *__restrict__ y) {
+    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < (size_t)rows * cols; id += gridDim.x * (size_t)256) {
+        const int n = (int)(id / cols), k = (int)(id % cols), kb = k / 128, kk = k % 128;
+        const uint8_t c = codes[((size_t)(n / 16) * kbs + kb) * 2048 + kk / 64 * 1024 + (kk / 16 % 4 * 16 + n % 16) * 16 +
+                                kk % 16];
+        const half2_t v = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((uint32_t)c, 1.0f, false);
+        y[id] = __fmul_rn((float)v[0], scales[(size_t)(n / 128) * kbs + kb]);
+    }
+}
+
+// ---- activations ---------------------------------------------------------------
+
+// Codes [m x 128 kbs] and scales [kbs x m] of the rows of x. 16 lanes take a
+// block of 128 values; a workgroup takes the same block of 16 rows, so that it
+// writes their scales side by side. Bound by memory: (sizeof(T) + 1) bytes per value.
+template <class T>
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs, int vec,
+                                                           uint8_t *__restrict__ q, float *__restrict__ sx) {
+    const int row = blockIdx.x * 16 + threadIdx.x / 16, kb = blockIdx.y, k0 = kb * 128 + threadIdx.x % 16 * 8;
+    float v[8];
+    const bool live = row < m;  // whole DPP rows of lanes
+    fp8_load8(x + (size_t)(live ? row : 0) * k, k0, k, vec, v);
+    uint2_t codes;
+    const float s = fp8_quantize8(v, codes);
+    if (!live) return;
+    *(uint2_t *)(q + ((size_t)row * kbs + kb) * 128 + threadIdx.x % 16 * 8) = codes;
+    if (threadIdx.x % 16 == 0) sx[(size_t)kb * m + row] = s;
+}
+
+// ---- products: the weight streamed over a few rows -----------------------------
+
+// A workgroup owns 16 weight rows and 16 MB activation rows. Its 8 waves take
+// the k-blocks in turn (block b on wave b % 8), operands straight from memory,
+// and their f32 partials are added in wave order, from LDS. The matrix unit's
+// operands are swapped (weight first), so a lane holds one activation row and
+// four output columns.
+constexpr int kRowsWaves = 8;
+
+template <int MB, bool WIDE>
+__global__ __launch_bounds__(kRowsWaves * 64) void fp8_rows_kernel(const uint8_t *__restrict__ codes,
+                                                                   const float *__restrict__ scales, int n, int kbs,
+                                                                   const uint8_t *__restrict__ q,
+                                                                   const float *__restrict__ sx, int m,
+                                                                   void *__restrict__ y, int dtype) {
+    __shared__ __align__(16) float part[kRowsWaves][MB * 256];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int g = lane / 16, j = lane % 16;
+    const int tiles = (n + 15) / 16, t = blockIdx.x % tiles, row0 = blockIdx.x / tiles * 16 * MB;
+    const uint8_t *wbase = codes + (size_t)t * kbs * 2048 + lane * 16;
+    const float *swrow = scales + (size_t)(t / 8) * kbs;
+    float4_t acc[MB];
+#pragma unroll
+    for (int b = 0; b < MB; b++) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int kb = wave; kb < kbs; kb += kRowsWaves) {
+        const uint4_t w0 = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048));
+        const uint4_t w1 = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048 + 1024));
+        const float sw = swrow[kb];
+#pragma unroll
+        for (int b = 0; b < MB; b++) {
+            const int row = row0 + 16 * b + j;
+            uint4_t x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+            float s = 0.0f;
+            if (row < m) {
+                const uint8_t *xr = q + ((size_t)row * kbs + kb) * 128 + 16 * g;
+                x0 = *(const uint4_t *)xr;
+                x1 = *(const uint4_t *)(xr + 64);
+                s = sx[(size_t)kb * m + row] * sw;
+            }
+            const float4_t d = WIDE ? fp8_mfma_wide(fp8_widen(w0, w1), fp8_widen(x0, x1)) : fp8_mfma(w0, w1, x0, x1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[b][e] = __builtin_fmaf(d[e], s, acc[b][e]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++) *(float4_t *)&part[wave][(b * 16 + j) * 16 + 4 * g] = acc[b];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MB * 256; i += kRowsWaves * 64) {
+        const int row = row0 + i / 16, col = t * 16 + i % 16;
+        if (row >= m || col >= n) continue;
+        float v = part[0][i];
+#pragma unroll
+        for (int w = 1; w < kRowsWaves; w++) v += part[w][i];
+        fp8_store(y, dtype, (size_t)row * n + col, v);
+    }
+}
+
+template <int MB>
+void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
+    const dim3 grid(cdiv(w.rows, 16) * cdiv(m, 16 * MB));
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL((fp8_rows_kernel<MB, true>), grid, dim3(kRowsWaves * 64), 0, s, w.codes, w.scales, w.rows,
+                           w.kbs, q, sx, m, y, dtype);
+    else
+        hipLaunchKernelGGL((fp8_rows_kernel<MB, false>), grid, dim3(kRowsWaves * 64), 0, s, w.codes, w.scales, w.rows,
+                           w.kbs, q, sx, m, y, dtype);
+}
+
+void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, float *sx, hipStream_t s) {
+    const int kbs = (int)cdiv(k, 128);
+    const int vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    const dim3 grid(cdiv(m, 16), kbs);
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL(fp8_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, vec, q, sx);
+    else if (dtype == DZ_F16)
+        hipLaunchKernelGGL(fp8_quantize_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)x, m, k, kbs, vec, q, sx);
+    else
+        hipLaunchKernelGGL(fp8_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, vec, q, sx);
+}
+
+// The product of m > 0 rows of codes.
+void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype,
+                        hipStream_t s) {
+    if (m <= 16) fp8_rows_launch<1>(w, q, sx, m, y, dtype, s);
+    else fp8_rows_launch<4>(w, q, sx, m, y, dtype, s);
+}
+
+bool fp8_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }
+
+int32_t fp8_alloc(dz_ctx *ctx, size_t rows, size_t cols, dz_fp8_weight **out) {
+    if (rows == 0 || cols == 0 || rows > kFp8MostRows || cols > kFp8MostCols)
+        return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "invalid weight shape");
+    dz_fp8_weight *h = new (std::nothrow) dz_fp8_weight();
+    if (!h) return ctx_fail(ctx, DZ_RESOURCE_LIMIT, "weight allocation");
+    h->device = ctx_device(ctx);
+    Fp8Weight &w = h->w;
+    w.rows = (int)rows;
+    w.cols = (int)cols;
+    w.np = (int)((rows + 15) / 16 * 16);
+    w.kbs = (int)((cols + 127) / 128);
+    hipError_t e = hipMalloc(&w.codes, w.code_bytes());
+    if (e == hipSuccess) e = hipMalloc(&w.scales, w.scale_bytes());
+    if (e != hipSuccess) {
+        if (w.codes) hipFree(w.codes);
+        delete h;
+        return ctx_hip_fail(ctx, e, "weight allocation");
+    }
+    *out = h;
+    return DZ_OK;
+}
+
+void fp8_release(dz_fp8_weight *h) {
+    if (!h) return;
+    hipFree(h->w.codes);
+    hipFree(h->w.scales);
+    delete h;
+}
+
+int32_t fp8_weight_ok(dz_ctx *ctx, const dz_fp8_weight *w) {
+    if (!w) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (w->device != ctx_device(ctx)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "the weight lives on another device");
+    return DZ_OK;
+}
+
+}  // namespace
+
+void launch_fp8_retile(const uint8_t *codes, int rows, int cols, uint8_t *dst, size_t tile_bytes, size_t kb_bytes,
+                       int *bad, hipStream_t s) {
+    const int np = (rows + 15) / 16 * 16, kbs = (cols + 127) / 128;
+    hipLaunchKernelGGL(fp8_retile_kernel, dim3(std::min(cdiv((size_t)np * kbs * 8, 256), 1u << 20)), dim3(256), 0, s, codes, rows, cols, np,
+                       kbs, dst, tile_bytes, kb_bytes, bad);
+}
+
+void launch_fp8_scales(const float *src, float *dst, size_t n, int *bad, hipStream_t s) {
+    hipLaunchKernelGGL(fp8_scales_kernel, dim3(cdiv(n, 256)), dim3(256), 0, s, src, dst, n, bad);
+}
+
+int32_t fp8_weight_create(dz_ctx *ctx, const uint8_t *codes, const float *scales, size_t rows, size_t cols,
+                          dz_fp8_weight **out) {
+    if (!out) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    *out = nullptr;
+    if (!codes || !scales) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    dz_fp8_weight *h = nullptr;
+    int32_t rc = fp8_alloc(ctx, rows, cols, &h);
+    if (rc) return rc;
+    int *bad = ctx_flag(ctx), value = 0;
+    hipStream_t s = ctx_stream(ctx);
+    launch_fill_i32(bad, 0, 1, s);
+    launch_fp8_retile(codes, h->w.rows, h->w.cols, h->w.codes, (size_t)h->w.kbs * 2048, 2048, bad, s);
+    launch_fp8_scales(scales, h->w.scales, h->w.scale_bytes() / sizeof(float), bad, s);
+    rc = ctx_flag_value(ctx, &value);
+    if (!rc && value) rc = ctx_fail(ctx, DZ_INVALID_CHECKPOINT, "invalid 8-bit floating point weight");
+    if (rc) {
+        fp8_release(h);
+        return rc;
+    }
+    *out = h;
+    return DZ_OK;
+}
+
+int32_t fp8_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                            dz_fp8_weight **out) {
+    if (!out) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    *out = nullptr;
+    if (!values) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!fp8_dtype(dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    dz_fp8_weight *h = nullptr;
+    int32_t rc = fp8_alloc(ctx, rows, cols, &h);
+    if (rc) return rc;
+    int *bad = ctx_flag(ctx), value = 0;
+    hipStream_t s = ctx_stream(ctx);
+    launch_fill_i32(bad, 0, 1, s);
+    const Fp8Weight &w = h->w;
+    const dim3 grid((unsigned)w.kbs * cdiv(w.rows, 128));
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL(fp8_quantize_weight_kernel<float>, grid, dim3(256), 0, s, (const float *)values, w.rows,
+                           w.cols, w.np, w.kbs, w.codes, w.scales, bad);
+    else if (dtype == DZ_F16)
+        hipLaunchKernelGGL(fp8_quantize_weight_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)values, w.rows,
+                           w.cols, w.np, w.kbs, w.codes, w.scales, bad);
+    else
+        hipLaunchKernelGGL(fp8_quantize_weight_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)values, w.rows,
+                           w.cols, w.np, w.kbs, w.codes, w.scales, bad);
+    rc = ctx_flag_value(ctx, &value);
+    if (!rc && value) rc = ctx_fail(ctx, DZ_INVALID_CHECKPOINT, "non-finite weight");
+    if (rc) {
+        fp8_release(h);
+        return rc;
+    }
+    *out = h;
+    return DZ_OK;
+}
+
+void fp8_weight_free(dz_fp8_weight *w) { fp8_release(w); }
+
+int32_t fp8_weight_info(const dz_fp8_weight *w, size_t *rows, size_t *cols, size_t *device_bytes) {
+    if (!w) return DZ_INVALID_REQUEST;
+    if (rows) *rows = (size_t)w->w.rows;
+    if (cols) *cols = (size_t)w->w.cols;
+    if (device_bytes) *device_bytes = w->w.code_bytes() + w->w.scale_bytes();
+    return DZ_OK;
+}
+
+int32_t fp8_dequant(dz_ctx *ctx, const dz_fp8_weight *w, float *y) {
+    if (int32_t rc = fp8_weight_ok(ctx, w)) return rc;
+    if (!y) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    hipLaunchKernelGGL(fp8_dequant_kernel, dim3(std::min(cdiv((size_t)w->w.rows * w->w.cols, 256), 1u << 20)),
+                       dim3(256), 0, ctx_stream(ctx), w->w.codes, w->w.scales, w->w.rows, w->w.cols, w->w.kbs, y);
+    return ctx_launched(ctx, "fp8 dequant");
+}
+
+int32_t fp8_quantize(dz_ctx *ctx, const void *x, int32_t dtype, size_t m, size_t k, uint8_t *q, float *s) {
+    if (!fp8_dtype(dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (k == 0 || k > kFp8MostCols) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "invalid activation shape");
+    if (m && (!x || !q || !s)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (((uintptr_t)q & 15) != 0) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes must be 16-byte aligned");
+    if (m == 0) return DZ_OK;
+    launch_fp8_quantize(x, dtype, (int)m, (int)k, q, s, ctx_stream(ctx));
+    return ctx_launched(ctx, "fp8 quantize");
+}
+
+int32_t fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q, const float *s, size_t m, void *y,
+                      int32_t y_dtype) {
+    if (int32_t rc = fp8_weight_ok(ctx, w)) return rc;
+    if (m && (!q || !s || !y)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!fp8_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (((uintptr_t)q & 15) != 0) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes must be 16-byte aligned");
+    if (m == 0) return DZ_OK;
+    launch_fp8_product(w->w, q, s, (int)m, y, y_dtype, ctx_stream(ctx));
+    return ctx_launched(ctx, "fp8 linear");
+}
+
+int32_t fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                   int32_t y_dtype) {
+    if (int32_t rc = fp8_weight_ok(ctx, w)) return rc;
+    if (m && (!x || !y)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!fp8_dtype(x_dtype) || !fp8_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (m == 0) return DZ_OK;
+    const size_t qbytes = m * (size_t)w->w.kbs * 128, at = (qbytes + 255) / 256 * 256;
+    void *work = nullptr;
+    if (int32_t rc = ctx_workspace(ctx, at + m * (size_t)w->w.kbs * sizeof(float), &work)) return rc;
+    uint8_t *q = (uint8_t *)work;
+    float *sx = (float *)(q + at);
+    launch_fp8_quantize(x, x_dtype, (int)m, w->w.cols, q, sx, ctx_stream(ctx));
+    launch_fp8_product(w->w, q, sx, (int)m, y, y_dtype, ctx_stream(ctx));
+    return ctx_launched(ctx, "fp8 linear");
+}
+
+}  // namespace dz

@@ -33,7 +33,8 @@ struct dz_ctx {
     int cus = 0;
     int clock_khz = 0;
     // device ints: [0] validation / non-finite flag, [1..62] the product flag
-    // ring, [kCaptureSlot0 ..] one flag per product recorded under stream capture
+    // ring, [kTicketSlot] the ticket of the mixture-of-experts router (0 between
+    // calls), [kCaptureSlot0 ..] one flag per product recorded under stream capture
     int *flag = nullptr;
     uint64_t product_calls = 0;  // ring products since the last stream change (picks the slot)
     int captured_flags = 0;      // capture slots ever handed out (the high-water mark)
@@ -90,6 +91,26 @@ int32_t pplx_forward_rows(dz_ctx *ctx, dz_pplx *p, const void *rows_host, size_t
 int32_t encoder_forward(dz_ctx *ctx, dz_encoder *enc, const int32_t *ids_dev, const void *rows_host,
                         size_t batch, size_t seq, float *out);
 int32_t tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cache_out, size_t cap);
+int32_t fp8_weight_create(dz_ctx *ctx, const uint8_t *codes, const float *scales, size_t rows, size_t cols,
+                          dz_fp8_weight **out);
+int32_t fp8_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                            dz_fp8_weight **out);
+void fp8_weight_free(dz_fp8_weight *w);
+int32_t fp8_weight_info(const dz_fp8_weight *w, size_t *rows, size_t *cols, size_t *device_bytes);
+int32_t fp8_dequant(dz_ctx *ctx, const dz_fp8_weight *w, float *y);
+int32_t fp8_quantize(dz_ctx *ctx, const void *x, int32_t dtype, size_t m, size_t k, uint8_t *q, float *s);
+int32_t fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                   int32_t y_dtype);
+int32_t fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q, const float *s, size_t m, void *y,
+                      int32_t y_dtype);
+int32_t moe_create(dz_ctx *ctx, const dz_moe_config *cfg, const void *router, int32_t router_dtype,
+                   const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
+                   const uint8_t *down, const float *down_scales, dz_moe **out);
+void moe_free(dz_moe *e);
+int32_t moe_info(const dz_moe *e, dz_moe_config *cfg, size_t *device_bytes);
+int32_t moe_route(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, int32_t *ids,
+                  float *shares);
+int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, void *y);
 }  // namespace dz
 
 namespace {
@@ -143,6 +164,7 @@ int variant(dz_ctx *ctx, const char *family) {
 }
 
 constexpr int kRingSlots = 62;
+constexpr int kTicketSlot = 63;
 constexpr int kCaptureSlot0 = 64;
 constexpr int kCaptureSlots = 4032;  // 16 KiB flag buffer
 constexpr size_t kFlagBytes = (size_t)(kCaptureSlot0 + kCaptureSlots) * sizeof(int);
@@ -1034,6 +1056,87 @@ int32_t dz_q4_rows_gemm(dz_ctx *ctx, const int8_t *a, const float *sa, size_t m,
     return launched(ctx, "q4 rows gemm");
 }
 
+// ---- 8-bit floating point weights ------------------------------------------------------
+
+int32_t dz_fp8_weight_create(dz_ctx *ctx, const uint8_t *codes, const float *scales, size_t rows, size_t cols,
+                             dz_fp8_weight **out) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    return dz::fp8_weight_create(ctx, codes, scales, rows, cols, out);
+}
+
+int32_t dz_fp8_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                               dz_fp8_weight **out) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    return dz::fp8_weight_quantize(ctx, values, dtype, rows, cols, out);
+}
+
+int32_t dz_fp8_weight_free(dz_ctx *ctx, dz_fp8_weight *w) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    DZ_HIP(ctx, hipStreamSynchronize(ctx->stream), "stream synchronize");
+    dz::fp8_weight_free(w);
+    return DZ_OK;
+}
+
+int32_t dz_fp8_weight_info(const dz_fp8_weight *w, size_t *rows, size_t *cols, size_t *device_bytes) {
+    return dz::fp8_weight_info(w, rows, cols, device_bytes);
+}
+
+int32_t dz_fp8_dequant(dz_ctx *ctx, const dz_fp8_weight *w, float *y) {
+    DZ_BEGIN(ctx);
+    return dz::fp8_dequant(ctx, w, y);
+}
+
+int32_t dz_fp8_quantize(dz_ctx *ctx, const void *x, int32_t x_dtype, size_t m, size_t k, uint8_t *q, float *s) {
+    DZ_BEGIN(ctx);
+    return dz::fp8_quantize(ctx, x, x_dtype, m, k, q, s);
+}
+
+int32_t dz_fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                      int32_t y_dtype) {
+    DZ_BEGIN(ctx);
+    return dz::fp8_linear(ctx, w, x, x_dtype, m, y, y_dtype);
+}
+
+int32_t dz_fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q, const float *s, size_t m, void *y,
+                         int32_t y_dtype) {
+    DZ_BEGIN(ctx);
+    return dz::fp8_linear_q8(ctx, w, q, s, m, y, y_dtype);
+}
+
+int32_t dz_moe_create(dz_ctx *ctx, const dz_moe_config *cfg, const void *router, int32_t router_dtype,
+                      const uint8_t *gate, const float *gate_scales, const uint8_t *up, const float *up_scales,
+                      const uint8_t *down, const float *down_scales, dz_moe **out) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    return dz::moe_create(ctx, cfg, router, router_dtype, gate, gate_scales, up, up_scales, down, down_scales, out);
+}
+
+int32_t dz_moe_free(dz_ctx *ctx, dz_moe *moe) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    DZ_HIP(ctx, hipStreamSynchronize(ctx->stream), "stream synchronize");
+    dz::moe_free(moe);
+    return DZ_OK;
+}
+
+int32_t dz_moe_info(const dz_moe *moe, dz_moe_config *cfg, size_t *device_bytes) {
+    return dz::moe_info(moe, cfg, device_bytes);
+}
+
+int32_t dz_moe_route(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtype, size_t tokens, int32_t *ids,
+                     float *shares) {
+    DZ_BEGIN(ctx);
+    return dz::moe_route(ctx, moe, x, dtype, tokens, ids, shares);
+}
+
+int32_t dz_moe_forward(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtype, size_t tokens, void *y) {
+    DZ_BEGIN(ctx);
+    return dz::moe_forward(ctx, moe, x, dtype, tokens, y);
+}
+
 // ---- epilogues --------------------------------------------------------------------------
 
 int32_t dz_layernorm(dz_ctx *ctx, const void *x, void *y, int32_t dtype, size_t rows, size_t d,
@@ -1275,6 +1378,17 @@ int32_t ctx_fail(dz_ctx *ctx, int32_t code, const std::string &msg) { return fai
 int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what) { return hip_fail(ctx, e, what); }
 hipStream_t ctx_stream(dz_ctx *ctx) { return ctx->stream; }
 int *ctx_flag(dz_ctx *ctx) { return ctx->flag; }
+int *ctx_ticket(dz_ctx *ctx) { return ctx->flag + kTicketSlot; }
+int ctx_device(dz_ctx *ctx) { return ctx->device; }
+int32_t ctx_launched(dz_ctx *ctx, const char *what) { return launched(ctx, what); }
+// Waits for the work just enqueued, whose kernels report in the context's flag, and reads it.
+int32_t ctx_flag_value(dz_ctx *ctx, int *value) {
+    int32_t rc = launched(ctx, "kernel launch");
+    if (rc) return rc;
+    DZ_HIP(ctx, hipMemcpyAsync(value, ctx->flag, sizeof(int), hipMemcpyDeviceToHost, ctx->stream), "flag readback");
+    DZ_HIP(ctx, hipStreamSynchronize(ctx->stream), "stream synchronize");
+    return DZ_OK;
+}
 int ctx_variant(dz_ctx *ctx, const char *family) { return variant(ctx, family); }
 
 // h += the W4A8 product of x (f32 rows, quantized here to A8 codes) or of the

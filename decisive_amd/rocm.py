@@ -79,6 +79,14 @@ class PplxConfig(ctypes.Structure):
                 ("attn_kv_heads", ctypes.c_int32), ("attn_head_dim", ctypes.c_int32)]
 
 
+class MoeConfig(ctypes.Structure):
+    _fields_ = [("experts", ctypes.c_int32), ("top_k", ctypes.c_int32), ("hidden", ctypes.c_int32),
+                ("ff", ctypes.c_int32), ("renormalize", ctypes.c_int32)]
+
+
+MOE_MAX_TOKENS = 128  # dz_moe_forward's tokens per call
+
+
 _lib = None
 
 P, SZ, I32, U32, U64, F = (ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_uint32,
@@ -155,6 +163,19 @@ _SIGNATURES = {
     "dz_pplx_forward_rows": (I32, [P, P, P, SZ, P, SZ, P]),
     "dz_pplx_set_residency": (I32, [P, P, I32]),
     "dz_pplx_residency_info": (I32, [P, P, ctypes.c_char_p, SZ]),
+    "dz_fp8_weight_create": (I32, [P, P, P, SZ, SZ, PP]),
+    "dz_fp8_weight_quantize": (I32, [P, P, I32, SZ, SZ, PP]),
+    "dz_fp8_weight_free": (I32, [P, P]),
+    "dz_fp8_weight_info": (I32, [P, ctypes.POINTER(SZ), ctypes.POINTER(SZ), ctypes.POINTER(SZ)]),
+    "dz_fp8_dequant": (I32, [P, P, P]),
+    "dz_fp8_quantize": (I32, [P, P, I32, SZ, SZ, P, P]),
+    "dz_fp8_linear": (I32, [P, P, P, I32, SZ, P, I32]),
+    "dz_fp8_linear_q8": (I32, [P, P, P, P, SZ, P, I32]),
+    "dz_moe_create": (I32, [P, ctypes.POINTER(MoeConfig), P, I32, P, P, P, P, P, P, PP]),
+    "dz_moe_free": (I32, [P, P]),
+    "dz_moe_info": (I32, [P, ctypes.POINTER(MoeConfig), ctypes.POINTER(SZ)]),
+    "dz_moe_route": (I32, [P, P, P, I32, SZ, P, P]),
+    "dz_moe_forward": (I32, [P, P, P, I32, SZ, P]),
     "dz_tune": (I32, [P, U32, ctypes.c_char_p, ctypes.c_char_p, SZ]),
     "dz_select_variant": (I32, [P, ctypes.c_char_p, ctypes.c_char_p]),
 }
@@ -223,6 +244,59 @@ class Weight:
         try:
             if self.handle and self.owned and self.ctx.handle:
                 load().dz_weight_free(self.ctx.handle, self.handle)
+                self.handle = 0
+        except Exception:
+            pass
+
+
+class Fp8Weight:
+    """A device-resident weight in e4m3 with a scale for each 128 x 128 block (dz_fp8_weight)."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self.handle = ctx, handle
+        rows, cols, dbytes = SZ(), SZ(), SZ()
+        load().dz_fp8_weight_info(handle, ctypes.byref(rows), ctypes.byref(cols), ctypes.byref(dbytes))
+        self.rows, self.cols, self.device_bytes = rows.value, cols.value, dbytes.value
+
+    def free(self):
+        if self.handle:
+            self.ctx._check(load().dz_fp8_weight_free(self.ctx.handle, self.handle))
+        self.handle = 0
+
+    def __del__(self):
+        try:
+            if self.handle and self.ctx.handle:
+                load().dz_fp8_weight_free(self.ctx.handle, self.handle)
+                self.handle = 0
+        except Exception:
+            pass
+
+
+class Moe:
+    """A mixture-of-experts layer for a few tokens (dz_moe)."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self.handle = ctx, handle
+        self.cfg, dbytes = MoeConfig(), SZ()
+        load().dz_moe_info(handle, ctypes.byref(self.cfg), ctypes.byref(dbytes))
+        self.device_bytes = dbytes.value
+
+    def route(self, x, dtype: int, tokens: int, ids, shares):
+        self.ctx._check(load().dz_moe_route(self.ctx.handle, self.handle, _addr(x), dtype, tokens, _addr(ids),
+                                            _addr(shares)))
+
+    def forward(self, x, dtype: int, tokens: int, y):
+        self.ctx._check(load().dz_moe_forward(self.ctx.handle, self.handle, _addr(x), dtype, tokens, _addr(y)))
+
+    def free(self):
+        if self.handle:
+            self.ctx._check(load().dz_moe_free(self.ctx.handle, self.handle))
+        self.handle = 0
+
+    def __del__(self):
+        try:
+            if self.handle and self.ctx.handle:
+                load().dz_moe_free(self.ctx.handle, self.handle)
                 self.handle = 0
         except Exception:
             pass
@@ -395,6 +469,39 @@ class Context:
 
     def attention(self, qkv, out, batch: int, seq: int, heads: int, dh: int, scale: float):
         self._check(load().dz_attention(self.handle, _addr(qkv), _addr(out), batch, seq, heads, dh, scale))
+
+    # ---- 8-bit floating point weights ----
+    def fp8_weight(self, codes, scales, rows: int, cols: int) -> "Fp8Weight":
+        """dz_fp8_weight_create: e4m3 codes [rows x cols] and f32 scales of 128 x 128 blocks, both on the device."""
+        h = ctypes.c_void_p()
+        self._check(load().dz_fp8_weight_create(self.handle, _addr(codes), _addr(scales), rows, cols,
+                                                ctypes.byref(h)))
+        return Fp8Weight(self, h.value)
+
+    def fp8_weight_quantize(self, values, dtype: int, rows: int, cols: int) -> "Fp8Weight":
+        h = ctypes.c_void_p()
+        self._check(load().dz_fp8_weight_quantize(self.handle, _addr(values), dtype, rows, cols, ctypes.byref(h)))
+        return Fp8Weight(self, h.value)
+
+    def fp8_dequant(self, w: "Fp8Weight", y):
+        self._check(load().dz_fp8_dequant(self.handle, w.handle, _addr(y)))
+
+    def fp8_quantize(self, x, x_dtype: int, m: int, k: int, q, s):
+        self._check(load().dz_fp8_quantize(self.handle, _addr(x), x_dtype, m, k, _addr(q), _addr(s)))
+
+    def fp8_linear(self, w: "Fp8Weight", x, x_dtype: int, m: int, y, y_dtype: int):
+        self._check(load().dz_fp8_linear(self.handle, w.handle, _addr(x), x_dtype, m, _addr(y), y_dtype))
+
+    def fp8_linear_q8(self, w: "Fp8Weight", q, s, m: int, y, y_dtype: int):
+        self._check(load().dz_fp8_linear_q8(self.handle, w.handle, _addr(q), _addr(s), m, _addr(y), y_dtype))
+
+    def moe(self, cfg: MoeConfig, router, router_dtype: int, gate, up, down) -> "Moe":
+        """dz_moe_create: gate, up and down are pairs (codes, scales) over all experts."""
+        h = ctypes.c_void_p()
+        self._check(load().dz_moe_create(self.handle, ctypes.byref(cfg), _addr(router), router_dtype,
+                                         _addr(gate[0]), _addr(gate[1]), _addr(up[0]), _addr(up[1]),
+                                         _addr(down[0]), _addr(down[1]), ctypes.byref(h)))
+        return Moe(self, h.value)
 
     # ---- encoder ----
     def encoder_random(self, cfg: EncoderConfig, seed: int) -> "Encoder":
