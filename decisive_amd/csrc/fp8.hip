@@ -6,6 +6,7 @@
 // dot_b is the dot of 128 codes. The blocks are folded in f32, in order of b:
 // acc = fma(dot_b, sx * sw, acc).
 #include <algorithm>
+#include <type_traits>
 
 #include "../../include/decisive_rocm.h"
 #include "fp8.hpp"
@@ -206,6 +207,190 @@ void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
                            w.kbs, q, sx, m, y, dtype);
 }
 
+// ---- products: tiles over many rows ----------------------------------------------
+
+// Block tile BM x BN (activation rows x weight rows). KS groups of WGM x WGN
+// waves each take every KS-th 128-block of k; a step is KS blocks, one a group,
+// in one of NS LDS stages that buffer_load ... lds fills. The weight's chunks
+// land as they are, in operand order; activation rows of 128 bytes are
+// swizzled, chunk c of row r in slot c ^ (r / 2 % 8), so that 16 lanes reading 16
+// rows meet distinct banks. NS - 1 steps' loads are in flight or in use. Each
+// block's dots come from a zero accumulator and are folded by sx * sw with one fma
+// per output, in the shadow of the next MFMAs. The groups' sums are added in group
+// order, through LDS.
+template <int BM, int BN, int WGM, int WGN, int KS, int NS, bool WIDE>
+__global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8_t *__restrict__ codes,
+                                                                     const float *__restrict__ scales, int n, int kbs,
+                                                                     const uint8_t *__restrict__ q,
+                                                                     const float *__restrict__ sx, int m,
+                                                                     void *__restrict__ y, int dtype) {
+    constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
+    constexpr int XPW = BM / 8 / WAVES, WPW = BN / 8 / WAVES;  // 1 KiB loads per wave and stage
+    constexpr int PB = XPW + WPW + 1;                          // and the row scales
+    constexpr int XB = BM * 128, PART = XB + BN * 128 + (BM < 64 ? 64 : BM) * 4, STAGE = KS * PART;
+    static_assert(XPW * 8 * WAVES == BM && WPW * 8 * WAVES == BN, "whole loads for each wave");
+    static_assert(WPW == 1 || WPW % 2 == 0, "column tiles and halves known at compile time");
+    static_assert(TN <= 128 && 128 % TN == 0, "one column block a wave");
+    static_assert((NS - 2) * PB <= 63, "vmcnt range");
+    static_assert((KS - 1) * BM * BN * 4 <= NS * STAGE, "the groups' sums fit the stages");
+    __shared__ __align__(16) uint8_t lds[NS * STAGE];
+
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int group = wave_all / WAVES, wave = wave_all % WAVES;
+    const int wm = wave / WGN, wn = wave % WGN, g = lane / 16, j = lane % 16;
+    const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
+    int tm, tn;
+    xcd_tile(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+    const int row0 = tm * BM, col0 = tn * BN, rows = min(BM, m - row0);
+    const int kp = kbs * 128, tile0 = col0 / 16, tvalid = min(BN / 16, (n + 15) / 16 - tile0);
+    const int32x4_t rx = buffer_rsrc(q + (size_t)row0 * kp, (uint32_t)(rows * kp));
+    const int32x4_t rw = buffer_rsrc(codes + (size_t)tile0 * kbs * 2048, (uint32_t)(tvalid * kbs) * 2048u);
+    // load p of this wave fills rows 8 (wave XPW + p) + lane / 8, slot lane % 8
+    uint32_t xoff[XPW], woff[WPW];
+#pragma unroll
+    for (int p = 0; p < XPW; p++) {
+        const int r = (wave * XPW + p) * 8 + lane / 8;
+        xoff[p] = (uint32_t)r * kp + (lane % 8 ^ (r / 2 % 8)) * 16;
+    }
+#pragma unroll
+    for (int p = 0; p < WPW; p++) {
+        const int u = wave * WPW + p;
+        woff[p] = (uint32_t)(u / 2) * kbs * 2048 + u % 2 * 1024 + lane * 16;
+    }
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + group * PART;
+    // a wave's columns lie in one block of 128
+    const float *sw = scales + (size_t)min((col0 + wn * TN) / 128, (n - 1) / 128) * kbs;
+
+    // Blocks past the last one load nothing (every offset out of range, zeros in LDS), so that all waits go by count.
+    auto load_stage = [&](int stage, int step) {
+        const int kb = step * KS + group;
+        const bool live = kb < kbs;
+        const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u;
+#pragma unroll
+        for (int p = 0; p < XPW; p++)
+            dma16_at(at + (wave * XPW + p) * 1024, xoff[p] | past, rx, live ? (uint32_t)kb * 128 : 0u);
+#pragma unroll
+        for (int p = 0; p < WPW; p++)
+            dma16_at(at + XB + (wave * WPW + p) * 1024, woff[p] | past, rw, live ? (uint32_t)kb * 2048 : 0u);
+        // every wave loads 64 of the row scales
+        const int part = wave % (BM < 64 ? 1 : BM / 64);
+        const int32x4_t rs = buffer_rsrc(sx + (live ? (size_t)kb * m + row0 : 0), live ? (uint32_t)rows * 4 : 0u);
+        dma4(__builtin_amdgcn_readfirstlane(at + XB + BN * 128 + part * 256), (uint32_t)(part * 64 + lane) * 4,
+             int32x4_t{__builtin_amdgcn_readfirstlane(rs[0]), __builtin_amdgcn_readfirstlane(rs[1]),
+                       __builtin_amdgcn_readfirstlane(rs[2]), 0x00020000});
+    };
+
+    float4_t acc[NT][MT];
+#pragma unroll
+    for (int a = 0; a < NT; a++)
+#pragma unroll
+        for (int b = 0; b < MT; b++) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t sl = (j >> 1) & 7, own = group * PART;
+    const uint32_t x0 = own + (wm * TM + j) * 128 + (g ^ sl) * 16, x1 = own + (wm * TM + j) * 128 + ((4 + g) ^ sl) * 16;
+    const uint32_t w0 = own + XB + wn * TN * 128 + lane * 16, s0 = own + XB + BN * 128 + (wm * TM + j) * 4;
+    auto compute = [&](int stage, float scale) {
+        const uint8_t *st = lds + stage * STAGE;
+        uint4_t w[NT][2], x[2][2];
+        float s[MT];
+#pragma unroll
+        for (int a = 0; a < NT; a++) {
+            w[a][0] = *(const uint4_t *)(st + w0 + a * 2048);
+            w[a][1] = *(const uint4_t *)(st + w0 + a * 2048 + 1024);
+        }
+        x[0][0] = *(const uint4_t *)(st + x0);
+        x[0][1] = *(const uint4_t *)(st + x1);
+#pragma unroll
+        for (int b = 0; b < MT; b++) s[b] = *(const float *)(st + s0 + b * 64);
+#pragma unroll
+        for (int b = 0; b < MT; b++) s[b] *= scale;
+        Fp8Wide ww[WIDE ? NT : 1];
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int a = 0; a < NT; a++) ww[a] = fp8_widen(w[a][0], w[a][1]);
+        }
+        float4_t d[2][NT];
+#pragma unroll
+        for (int b = 0; b <= MT; b++) {
+            if (b + 1 < MT) {
+                x[(b + 1) & 1][0] = *(const uint4_t *)(st + x0 + (b + 1) * 2048);
+                x[(b + 1) & 1][1] = *(const uint4_t *)(st + x1 + (b + 1) * 2048);
+            }
+            Fp8Wide xw;
+            if constexpr (WIDE) xw = fp8_widen(x[b & 1][0], x[b & 1][1]);
+#pragma unroll
+            for (int a = 0; a < NT; a++) {
+                if (b < MT)
+                    d[b & 1][a] = WIDE ? fp8_mfma_wide(ww[WIDE ? a : 0], xw)
+                                       : fp8_mfma(w[a][0], w[a][1], x[b & 1][0], x[b & 1][1]);
+                if (b > 0) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        acc[a][b - 1][e] = __builtin_fmaf(d[(b - 1) & 1][a][e], s[b - 1], acc[a][b - 1][e]);
+                }
+            }
+        }
+    };
+
+    const int steps = (kbs + KS - 1) / KS;
+#pragma unroll
+    for (int p = 0; p < NS - 1; p++) load_stage(p, p);
+    float scale = sw[min(group, kbs - 1)];
+    int stage = 0;
+    for (int i = 0; i < steps; i++) {
+        // this wave's loads of step i are done once only the later steps' are left; then the barrier covers every wave
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
+        load_stage(stage == 0 ? NS - 1 : stage - 1, i + NS - 1);  // the stage that the step before read
+        const float next = sw[min((i + 1) * KS + group, kbs - 1)];
+        compute(stage, scale);
+        scale = next;
+        stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight once the block goes on
+
+    if constexpr (KS > 1) {
+        float4_t *sums = (float4_t *)lds;  // [groups - 1][waves][tiles][64 lanes]
+        __syncthreads();
+        if (group > 0) {
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+#pragma unroll
+                for (int b = 0; b < MT; b++)
+                    sums[(((group - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane] = acc[a][b];
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int h = 1; h < KS; h++)
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+#pragma unroll
+                for (int b = 0; b < MT; b++) acc[a][b] += sums[(((h - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane];
+    }
+    const bool vec = (n & 3) == 0 && ((uintptr_t)y & 15) == 0;
+#pragma unroll
+    for (int b = 0; b < MT; b++) {
+        const int row = row0 + wm * TM + b * 16 + j;
+        if (row >= m) continue;
+#pragma unroll
+        for (int a = 0; a < NT; a++) {
+            const int col = col0 + wn * TN + a * 16 + 4 * g;
+            if (col < n) fp8_store4(y, dtype, (size_t)row * n + col, acc[a][b], n - col, vec);
+        }
+    }
+}
+
+template <int BM, int BN, int WGM, int WGN, int KS, int NS>
+void fp8_tile_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
+    const dim3 grid(cdiv(m, BM) * cdiv(w.rows, BN)), block(WGM * WGN * KS * 64);
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WGM, WGN, KS, NS, true>), grid, block, 0, s, w.codes, w.scales,
+                           w.rows, w.kbs, q, sx, m, y, dtype);
+    else
+        hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WGM, WGN, KS, NS, false>), grid, block, 0, s, w.codes, w.scales,
+                           w.rows, w.kbs, q, sx, m, y, dtype);
+}
+
+
 void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, float *sx, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
     const int vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0;
@@ -218,11 +403,67 @@ void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, flo
         hipLaunchKernelGGL(fp8_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, vec, q, sx);
 }
 
-// The product of m > 0 rows of codes.
+// The tiles, in the order of the "fp8" family's variants from kTile0 on. Where a
+// grid takes r rounds of the chip (`resident` blocks a compute unit), a product
+// takes about r (f + blocks-of-k c) us; the least is taken. f covers a block's
+// first loads and its stores; c, the time of one 128-block, is measured with 8-bit
+// and with f32-accurate dots (two blocks a unit: 64x64 takes c 1.45 times). A
+// smaller tile walks k faster and loads more for it: a unit loads about 60 bytes
+// a nanosecond into LDS whatever the tile, which bounds all but the largest.
+// Measured (us, f16 or bf16 out; 32x32k4 / 64x32k2 / 64x64k4 / 64x64 / 128x128 /
+// 256x128 / 256x256): 64 rows, K=N=4096 8.0 / 9.8 / 14.1 / 14.1 / 23.3 / - / -;
+// 128 rows, K=N=2560 9.0 / 6.9 / 7.5 / 9.4 / 16.4; 229 rows, K=9216, N=2560
+// 28.9 / 32.5 / 20.6 / 27.4 / 48.5; 308 rows, K=1024, N=4096 14.9 / 11.4 / 10.3 /
+// 7.0 / 9.1 / 13.7; 600 rows, K=N=4096 - / - / 30.4 / 27.9 / 24.4 / 37.8 / 57.7;
+// 1024 rows, K=2560, N=8192 - / - / 59.7 / 44.5 / 33.9 / 29.3 / 42.6; 4096 rows,
+// K=1024, N=4096 - / - / - / 45.3 / 35.0 / 30.3 / 25.4; 8192 rows, K=N=4096 194 /
+// 160 / 133 on the last three. f32 out: 229 rows 37.3 / 42.8 / 25.7 / 39.3 / 79;
+// 1024 rows - / - / 73 / 64 / 53 / 44.
+struct Fp8Tile {
+    int bm, bn, resident;
+    float f, c, wide_c;
+};
+constexpr Fp8Tile kFp8Tiles[] = {{32, 32, 1, 3.0f, 0.13f, 0.165f}, {64, 32, 1, 2.5f, 0.215f, 0.28f},
+                                 {64, 64, 1, 3.0f, 0.265f, 0.345f}, {64, 64, 2, 3.0f, 0.36f, 0.53f},
+                                 {128, 128, 1, 3.5f, 0.66f, 1.07f}, {256, 128, 1, 7.5f, 1.05f, 1.75f},
+                                 {256, 256, 1, 8.0f, 1.95f, 1e9f}};
+constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 7;
+
+int fp8_pick(int m, int n, int kbs, bool wide) {
+    if (m <= 32) return m <= 16 ? 1 : 2;
+    const size_t cus = (size_t)device_cus();
+    int best = 0;
+    float least = 1e30f;
+    for (int i = 0; i < kTiles; i++) {
+        const Fp8Tile &t = kFp8Tiles[i];
+        const size_t blocks = (size_t)cdiv(m, t.bm) * cdiv(n, t.bn), round = cus * t.resident;
+        float c = wide ? t.wide_c : t.c;
+        if (t.resident > 1 && blocks > cus) c *= 1.45f;
+        const float us = (float)((blocks + round - 1) / round) * (t.f + (float)kbs * c);
+        if (us < least) least = us, best = i;
+    }
+    return kTile0 + best;
+}
+
+// The product of m > 0 rows of codes. Few rows stream the weight (up to 32 rows:
+// K=N=4096 7.6 us against 8.0 on 32x32 tiles, and N many times K far less).
 void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype,
-                        hipStream_t s) {
-    if (m <= 16) fp8_rows_launch<1>(w, q, sx, m, y, dtype, s);
-    else fp8_rows_launch<4>(w, q, sx, m, y, dtype, s);
+                        int variant, hipStream_t s) {
+    switch (variant ? variant : fp8_pick(m, w.rows, w.kbs, dtype == DZ_F32)) {
+        case 1: return fp8_rows_launch<1>(w, q, sx, m, y, dtype, s);
+        case 2: return fp8_rows_launch<2>(w, q, sx, m, y, dtype, s);
+        case 3: return fp8_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, s);
+        case 4: return fp8_tile_launch<64, 32, 2, 2, 2, 4>(w, q, sx, m, y, dtype, s);
+        case 5: return fp8_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, s);
+        case 6: return fp8_tile_launch<64, 64, 2, 2, 1, 4>(w, q, sx, m, y, dtype, s);
+        case 7: return fp8_tile_launch<128, 128, 2, 4, 1, 3>(w, q, sx, m, y, dtype, s);
+        case 8: return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, s);
+        default: break;
+    }
+    // 256x256: its f32-accurate form would not fit the registers
+    if (dtype == DZ_F32) return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, s);
+    hipLaunchKernelGGL((fp8_tile_kernel<256, 256, 2, 4, 1, 2, false>), dim3(cdiv(m, 256) * cdiv(w.rows, 256)),
+                       dim3(512), 0, s, w.codes, w.scales, w.rows, w.kbs, q, sx, m, y, dtype);
 }
 
 bool fp8_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }
@@ -368,7 +609,7 @@ int32_t fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q, con
     if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (((uintptr_t)q & 15) != 0) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes must be 16-byte aligned");
     if (m == 0) return DZ_OK;
-    launch_fp8_product(w->w, q, s, (int)m, y, y_dtype, ctx_stream(ctx));
+    launch_fp8_product(w->w, q, s, (int)m, y, y_dtype, ctx_variant(ctx, "fp8"), ctx_stream(ctx));
     return ctx_launched(ctx, "fp8 linear");
 }
 
@@ -385,7 +626,7 @@ int32_t fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x
     uint8_t *q = (uint8_t *)work;
     float *sx = (float *)(q + at);
     launch_fp8_quantize(x, x_dtype, (int)m, w->w.cols, q, sx, ctx_stream(ctx));
-    launch_fp8_product(w->w, q, sx, (int)m, y, y_dtype, ctx_stream(ctx));
+    launch_fp8_product(w->w, q, sx, (int)m, y, y_dtype, ctx_variant(ctx, "fp8"), ctx_stream(ctx));
     return ctx_launched(ctx, "fp8 linear");
 }
 

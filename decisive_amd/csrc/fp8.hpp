@@ -144,6 +144,23 @@ __device__ __forceinline__ void fp8_store(void *__restrict__ y, int dtype, size_
     else ((bf16_t *)y)[at] = (bf16_t)v;
 }
 
+// Four consecutive outputs at element `at`, `left` of them inside the row.
+__device__ __forceinline__ void fp8_store4(void *__restrict__ y, int dtype, size_t at, float4_t v, int left, bool vec) {
+    if (!vec) {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (e < left) fp8_store(y, dtype, at + e, v[e]);
+    } else if (dtype == 0) {
+        *(float4_t *)((float *)y + at) = v;
+    } else if (dtype == 1) {
+        const half2_t a = {(half_t)v[0], (half_t)v[1]}, b = {(half_t)v[2], (half_t)v[3]};
+        *(uint2_t *)((half_t *)y + at) = uint2_t{half2_as_word(a), half2_as_word(b)};
+    } else {
+        const bf16x2_t a = {(bf16_t)v[0], (bf16_t)v[1]}, b = {(bf16_t)v[2], (bf16_t)v[3]};
+        *(uint2_t *)((bf16_t *)y + at) = uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+    }
+}
+
 }  // namespace
 
 // ---- launchers (fp8.hip) -----------------------------------------------------

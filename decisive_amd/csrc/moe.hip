@@ -389,7 +389,7 @@ __global__ __launch_bounds__(kDownWaves * 64) void moe_down_kernel(const uint8_t
                                                                    const float *__restrict__ ds, int tokens, int d,
                                                                    int kbf, int all_rows, MoePlan plan,
                                                                    void *__restrict__ y, int dtype) {
-    extern __shared__ __align__(16) float sums[];  // [waves][tokens][16]
+    __shared__ __align__(16) float sums[kDownWaves * MC * 256];  // [waves][tokens][16]
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int g = lane / 16, j = lane % 16, t = blockIdx.x, tiles = (d + 15) / 16;
     const size_t hp = (size_t)kbf * 128;
@@ -500,25 +500,18 @@ void launch_route(const dz_moe *e, const void *x, int dtype, int tokens, const M
 }
 
 template <int MC, int XT, int HT>
-hipError_t launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
     const int rows = tokens * c.top_k;
     hipLaunchKernelGGL((moe_gate_up_kernel<MC, XT, HT>), dim3(e->kbf * 8, std::min(rows, c.experts)),
                        dim3(kGateWaves * 64), 0, s, e->gate_up, e->gate_scales, e->up_scales, tokens, c.ff, e->kbd,
                        e->kbf, rows, plan);
-    const size_t lds = (size_t)kDownWaves * tokens * 64;
-    if (lds > 65536) {
-        const hipError_t err = hipFuncSetAttribute((const void *)moe_down_kernel<MC, HT>,
-                                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (err != hipSuccess) return err;
-    }
-    hipLaunchKernelGGL((moe_down_kernel<MC, HT>), dim3(cdiv(c.hidden, 16)), dim3(kDownWaves * 64), lds, s, e->down,
+    hipLaunchKernelGGL((moe_down_kernel<MC, HT>), dim3(cdiv(c.hidden, 16)), dim3(kDownWaves * 64), 0, s, e->down,
                        e->down_scales, tokens, c.hidden, e->kbf, rows, plan, y, dtype);
-    return hipSuccess;
 }
 
 template <int MC>
-hipError_t launch_experts_dtype(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+void launch_experts_dtype(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
     if (dtype == DZ_F32) return launch_experts<MC, 3, 3>(e, dtype, tokens, plan, y, s);
     if (dtype == DZ_F16) return launch_experts<MC, 2, 2>(e, dtype, tokens, plan, y, s);
     return launch_experts<MC, 1, 2>(e, dtype, tokens, plan, y, s);
@@ -646,11 +639,10 @@ int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, 
     hipStream_t s = ctx_stream(ctx);
     launch_route(e, x, dtype, (int)tokens, plan, ctx_ticket(ctx), nullptr, nullptr, s);
     const int t = (int)tokens;
-    const hipError_t err = t <= 16   ? launch_experts_dtype<1>(e, dtype, t, plan, y, s)
-                           : t <= 32 ? launch_experts_dtype<2>(e, dtype, t, plan, y, s)
-                           : t <= 64 ? launch_experts_dtype<4>(e, dtype, t, plan, y, s)
-                                     : launch_experts_dtype<8>(e, dtype, t, plan, y, s);
-    if (err != hipSuccess) return ctx_hip_fail(ctx, err, "mixture of experts");
+    if (t <= 16) launch_experts_dtype<1>(e, dtype, t, plan, y, s);
+    else if (t <= 32) launch_experts_dtype<2>(e, dtype, t, plan, y, s);
+    else if (t <= 64) launch_experts_dtype<4>(e, dtype, t, plan, y, s);
+    else launch_experts_dtype<8>(e, dtype, t, plan, y, s);
     return ctx_launched(ctx, "mixture of experts");
 }
 

@@ -2524,6 +2524,8 @@ const char *const kMlpNames[] = {"pipe-auto", "pipe256x64w8", "pipe128x64w4", "w
                                   "pipe64x64n4"};
 const char *const kDeltaNames[] = {"chunked64", "chunked64-c32", "recurrent", "recurrent-rolled", "auto"};
 const char *const kNormNames[] = {"fused", "separate"};
+const char *const kFp8Names[] = {"auto",  "rows16",  "rows32",  "32x32k4", "64x32k2",
+                                 "64x64k4", "64x64", "128x128", "256x128", "256x256"};
 
 template <int W, int MPAD, bool G32, int NP>
 void gemv_launch_np(const Weight &w, const half_t *x, int m, float *y, hipStream_t s) {
@@ -2827,6 +2829,7 @@ int variant_count(const char *family) {
     if (f == "mlp") return 7;
     if (f == "delta_scan") return 5;
     if (f == "norm") return 2;
+    if (f == "fp8") return (int)(sizeof(kFp8Names) / sizeof(kFp8Names[0]));
     return 0;
 }
 
@@ -2856,6 +2859,7 @@ const char *variant_name(const char *family, int index) {
     if (f == "mlp") return kMlpNames[index];
     if (f == "delta_scan") return kDeltaNames[index];
     if (f == "norm") return kNormNames[index];
+    if (f == "fp8") return kFp8Names[index];
     return nullptr;
 }
 

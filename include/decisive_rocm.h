@@ -670,7 +670,8 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
                 size_t cap);
 /* Forces a variant of a family by name (tests and benchmarks). Families and
  * variants (the first of each is the default; every variant of a family
- * gives the same bits, except the delta scan's two opt-ins below):
+ * gives the same bits, except the delta scan's two opt-ins and the "fp8" family
+ * below):
  *   "gemv"        auto, w16, w8, stream8, stream4, persist (w16/w8: 16 or 8 waves
  *                 share one 16-row tile, each wave a fixed chunk of K; stream8/
  *                 stream4: one wave per tile, 8 or 4 tiles per block, for K a
@@ -713,12 +714,18 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *                 below 384 tokens and the chunked one from there, so a
  *                 decider's bits then depend on its chunk length. The token
  *                 scans and auto are explicit opt-ins that the tuner never
- *                 selects, and the only variants anywhere that do not give
+ *                 selects, and the only variants of a tuned family that do not give
  *                 their family's reference bits)
  *   "norm"        fused, separate (the decider's layer norms above 16 rows:
  *                 one kernel for the RMSNorm and the A8 codes its products
  *                 share, or the norm then one quantization per product; the
- *                 same bits) */
+ *                 same bits)
+ *   "fp8"         auto, rows16, rows32 (the weight streamed over 16 or 32 rows at a
+ *                 time), 32x32k4, 64x32k2, 64x64k4, 64x64, 128x128, 256x128, 256x256
+ *                 (tiles; k2 and k4 share the 128-blocks of k among two or four
+ *                 groups of waves). For tests and benchmarks: "auto" picks by the
+ *                 grid, dz_tune leaves it alone, and the variants add a row's blocks
+ *                 in orders of their own, so their f32 sums agree to rounding */
 int32_t dz_select_variant(dz_ctx *ctx, const char *family, const char *variant);
 
 #ifdef __cplusplus

@@ -220,6 +220,31 @@ def test_products_of_whole_numbers_lose_nothing(ctx, m, n, k, y_dtype):
     w.free()
 
 
+VARIANTS = ["rows16", "rows32", "32x32k4", "64x32k2", "64x64k4", "64x64", "128x128", "256x128", "256x256"]
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (33, 70, 130), (64, 128, 512), (257, 300, 1111), (300, 513, 640)])
+def test_every_variant_against_64_bits(ctx, variant, m, n, k):
+    """Each kernel forced on sizes below, at and past its tile, from one block of k on."""
+    rng = np.random.default_rng(m + n + k)
+    codes, scales = make_weight(rng, n, k)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    q, s = quantize(x)
+    want, mags = product(q, s, codes, scales, n, k)
+    w = ctx.fp8_weight(dev(codes), dev(scales), n, k)
+    ctx.select_variant("fp8", variant)
+    try:
+        for y_dtype in DTYPES:
+            y = empty((m, n), _torch(y_dtype))
+            ctx.fp8_linear(w, dev(x), rocm.F32, m, y, y_dtype)
+            ctx.sync()
+            check(f64(y), want, mags, k, y_dtype)
+    finally:
+        ctx.select_variant("fp8", "auto")
+    w.free()
+
+
 @pytest.mark.parametrize("m", [1, 3, 20, 70, 300])
 @pytest.mark.parametrize("x_dtype", DTYPES)
 def test_a_row_that_is_not_finite_makes_its_own_outputs_nan(ctx, m, x_dtype):
