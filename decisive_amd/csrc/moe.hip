@@ -7,11 +7,19 @@
 // c_e is p_e, or p_e / (sum of the chosen p). A few tokens read far more
 // weight than they multiply (2 operations a byte and row), so the layer is
 // bound by the bytes of the experts that are chosen, each read once:
-//   1 moe_route_kernel    logits; its last workgroup picks the experts and lists
-//                         each expert's rows (token and share), ordered by expert then token
-//   2 moe_gate_up_kernel  per (chosen expert, 16 columns of ff): h = silu(gate) * up of its rows
+//   1 moe_logits_kernel   logits, and x as bf16 terms
+// up to 16 tokens, where launches and trips to memory count:
+//   2 moe_gate_up_kernel  finds each token's experts; per (chosen expert, 16
+//                         columns of ff): h = silu(gate) * up of its rows
 //   3 moe_down_kernel     per 16 columns of the output: every chosen expert's down
 //                         product, times the rows' shares, summed
+// and above:
+//   2 moe_top_kernel      the experts of each token
+//   3, 4 moe_wide_kernel  h, and then each slot's down product
+//   5 moe_combine_kernel  the shares' sum
+// A token's i-th expert is slot = token * top_k + i, and h has a row for each
+// slot. Each workgroup finds the rows of its experts from the slots' experts,
+// expert by expert and in order of tokens; no order depends on timing.
 // The products run on the bf16 matrix unit: e4m3 is exact in bf16, and an
 // activation is a sum of bf16 terms: x is one term (bf16), two (f16, exactly)
 // or three (f32, exactly); h, which never leaves the layer, is two terms (16
@@ -43,7 +51,6 @@ int32_t ctx_fail(dz_ctx *ctx, int32_t code, const std::string &msg);
 int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what);
 hipStream_t ctx_stream(dz_ctx *ctx);
 int *ctx_flag(dz_ctx *ctx);
-int *ctx_ticket(dz_ctx *ctx);
 int ctx_device(dz_ctx *ctx);
 int32_t ctx_workspace(dz_ctx *ctx, size_t bytes, void **out);
 int32_t ctx_launched(dz_ctx *ctx, const char *what);
@@ -52,16 +59,17 @@ int32_t ctx_flag_value(dz_ctx *ctx, int *value);
 namespace {
 
 constexpr int kMostExperts = 512, kMostTop = 16, kMostWidth = 65536;
-constexpr int kRouteThreads = 512, kRouteTokens = 4;
+constexpr int kRouteTokens = 4;  // tokens a workgroup of the logits kernel takes together
+constexpr int kFewTokens = 16;   // tokens up to which a call goes through the kernels for few
 
-// What the first kernel leaves for the other two, in the workspace.
+// What the kernels leave for the ones after, in the workspace.
 struct MoePlan {
-    float *logits;     // [tokens][experts]
-    int *active;       // [0] how many experts are chosen, then per chosen expert {expert, first row, rows}
-    int *token;        // [rows] the row's token
-    float *share;      // [rows] c of the row
-    bf16_t *x;         // [terms][tokens][128 kbd]
-    bf16_t *h;         // [terms][rows][128 kbf]
+    float *logits;  // [tokens][experts]
+    int *ids;       // [slots] experts
+    float *shares;  // [slots]
+    bf16_t *x;      // [terms][tokens][128 kbd]
+    bf16_t *h;      // [terms][slots][128 kbf]
+    float *p;       // [slots][128 kbd] the experts' outputs, past kFewTokens
 };
 
 // v as TERMS bf16 values that add up to it: each term the leading 8 bits of
@@ -77,16 +85,19 @@ __device__ __forceinline__ void moe_split(float v, bf16_t out[TERMS]) {
     out[TERMS - 1] = (bf16_t)v;
 }
 
+// Maximum over the wave, in every lane (wave_max_dpp's pattern).
 __device__ __forceinline__ uint32_t moe_wave_max(uint32_t v) {
     v = dpp_max_u32<0xB1>(v);
     v = dpp_max_u32<0x4E>(v);
     v = dpp_max_u32<0x124>(v);
     v = dpp_max_u32<0x128>(v);
-    for (int o = 16; o < 64; o *= 2) {
-        const uint32_t other = (uint32_t)__shfl_xor((int)v, o);
-        v = v > other ? v : other;
-    }
-    return v;
+    uint32_t a = v, b = v;
+    asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    v = a > b ? a : b;
+    a = v;
+    b = v;
+    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(a), "+v"(b));
+    return a > b ? a : b;
 }
 
 // A logit's order as an unsigned number above 0 (0 marks an expert that is taken or absent).
@@ -95,170 +106,129 @@ __device__ __forceinline__ uint32_t moe_key(float v) {
     return b & 0x80000000u ? (b == 0xffffffffu ? 1u : ~b) : b | 0x80000000u;
 }
 
-// A wave takes one expert and four tokens: its router row against theirs, f32
-// throughout. Workgroups also write their share of x's bf16 terms. The last
-// workgroup to finish (a ticket that it sets back to 0) picks the experts:
-// per token a wave finds the largest logit top_k times, equal ones by the lower
-// index; lists come from bit masks of tokens per expert, so their order never
-// depends on which wave came first.
+// The experts of one token by one wave: top times the largest logit, equal
+// ones by the lower index (lane l holds experts PER l .. + PER - 1, so the first
+// lane with the largest has the lowest). Lane i < top is left with the i-th.
+template <int PER>
+__device__ __forceinline__ void moe_top(const float *__restrict__ logits, int experts, int top, int renormalize,
+                                        int &expert, float &share) {
+    const int lane = threadIdx.x % 64;
+    constexpr float kLeast = -3.4028235e38f;
+    float l[PER], most = kLeast;
+    uint32_t key[PER];
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const bool here = lane * PER + i < experts;
+        l[i] = here ? logits[lane * PER + i] : kLeast;
+        key[i] = here ? moe_key(l[i]) : 0u;
+        if (!(fabsf(l[i]) <= 3.4028235e38f)) fine = false;
+        most = fmaxf(most, l[i]);
+    }
+    fine = __all(fine);
+    most = wave_max_dpp(most);
+    float p[PER], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        p[i] = lane * PER + i < experts ? expf(l[i] - most) : 0.0f;
+        sum += p[i];
+    }
+    float picked = 0.0f;
+    expert = 0;
+    share = 0.0f;
+    for (int s = 0; s < top; s++) {
+        uint32_t best = 0;
+        int at = 0;
+        float mine = 0.0f;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (key[i] > best) best = key[i], at = i, mine = p[i];
+        const uint32_t largest = moe_wave_max(best);
+        const int owner = __ffsll((unsigned long long)__ballot(best == largest)) - 1;
+        const float c = word_as_float((uint32_t)__builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), owner));
+        const int e = owner * PER + __builtin_amdgcn_readlane(at, owner);
+        picked += c;
+        if (lane == s) expert = e, share = c;
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            if (lane == owner && i == at) key[i] = 0;
+    }
+    const float whole = renormalize ? picked : wave_sum_dpp(sum);
+    share = fine ? share / whole : __builtin_nanf("");
+}
+
+__device__ __forceinline__ void moe_top_any(const float *__restrict__ logits, int experts, int top, int renormalize,
+                                            int &expert, float &share) {
+    if (experts <= 64) moe_top<1>(logits, experts, top, renormalize, expert, share);
+    else if (experts <= 128) moe_top<2>(logits, experts, top, renormalize, expert, share);
+    else if (experts <= 256) moe_top<4>(logits, experts, top, renormalize, expert, share);
+    else moe_top<8>(logits, experts, top, renormalize, expert, share);
+}
+
+// A workgroup takes one expert and four tokens: its waves share hidden, f32
+// throughout. Workgroups also write their share of x's bf16 terms.
 template <class T, int TERMS>
-__global__ __launch_bounds__(kRouteThreads) void moe_route_kernel(
-    const T *__restrict__ x, const float *__restrict__ router, int tokens, int experts, int top, int d, int kbd,
-    int renormalize, int vec, MoePlan plan, int *ticket, int *ids_out, float *shares_out) {
-    constexpr int WAVES = kRouteThreads / 64;
-    __shared__ uint32_t mask[kMostExperts][4];
-    __shared__ uint32_t scan[kMostExperts];
-    __shared__ int last;
+__global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x, const float *__restrict__ router,
+                                                         int tokens, int experts, int d, int kbd, int vec,
+                                                         MoePlan plan) {
+    __shared__ float part[4][kRouteTokens];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    const int dp = kbd * 128;
-    const int e = blockIdx.x * WAVES + wave, first = blockIdx.y * kRouteTokens;
+    const int dp = kbd * 128, e = blockIdx.x, first = blockIdx.y * kRouteTokens;
     const int mine = min(kRouteTokens, tokens - first);
-    if (e < experts) {
-        const float *r = router + (size_t)e * dp;
-        float acc[kRouteTokens] = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = lane * 8; k0 < d; k0 += 512) {
-            const float4_t r0 = *(const float4_t *)(r + k0), r1 = *(const float4_t *)(r + k0 + 4);
-#pragma unroll
-            for (int i = 0; i < kRouteTokens; i++) {
-                if (i >= mine) break;
-                float v[8];
-                fp8_load8(x + (size_t)(first + i) * d, k0, d, vec, v);
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    acc[i] = __builtin_fmaf(r0[c], v[c], acc[i]);
-                    acc[i] = __builtin_fmaf(r1[c], v[4 + c], acc[i]);
-                }
-            }
-        }
+    const float *r = router + (size_t)e * dp;
+    float acc[kRouteTokens] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k0 = threadIdx.x * 8; k0 < d; k0 += 2048) {
+        const float4_t r0 = *(const float4_t *)(r + k0), r1 = *(const float4_t *)(r + k0 + 4);
 #pragma unroll
         for (int i = 0; i < kRouteTokens; i++) {
-            const float l = wave_sum_dpp(acc[i]);
-            if (lane == 0 && i < mine)
-                __hip_atomic_store(plan.logits + (size_t)(first + i) * experts + e, l, __ATOMIC_RELAXED,
-                                   __HIP_MEMORY_SCOPE_AGENT);
-        }
-    }
-    if (plan.x) {
-        const int units = dp / 8 * mine;
-        for (int u = blockIdx.x * kRouteThreads + threadIdx.x; u < units; u += gridDim.x * kRouteThreads) {
-            const int i = u / (dp / 8), k0 = u % (dp / 8) * 8;
+            if (i >= mine) break;
             float v[8];
             fp8_load8(x + (size_t)(first + i) * d, k0, d, vec, v);
-            bf16x8_t out[TERMS];
 #pragma unroll
-            for (int c = 0; c < 8; c++) {
-                bf16_t t[TERMS];
-                moe_split<TERMS>(v[c], t);
-#pragma unroll
-                for (int s = 0; s < TERMS; s++) out[s][c] = t[s];
+            for (int c = 0; c < 4; c++) {
+                acc[i] = __builtin_fmaf(r0[c], v[c], acc[i]);
+                acc[i] = __builtin_fmaf(r1[c], v[4 + c], acc[i]);
             }
-#pragma unroll
-            for (int s = 0; s < TERMS; s++)
-                *(bf16x8_t *)(plan.x + ((size_t)s * tokens + first + i) * dp + k0) = out[s];
         }
     }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        const int all = gridDim.x * gridDim.y;
-        last = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == all - 1;
-        if (last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = 0; i < mine; i++) {
+        const float l = wave_sum_dpp(acc[i]);
+        if (lane == 0) part[wave][i] = l;
     }
-    for (int i = threadIdx.x; i < kMostExperts * 4; i += kRouteThreads) (&mask[0][0])[i] = 0;
     __syncthreads();
-    if (!last) return;
+    if (threadIdx.x < mine)
+        plan.logits[(size_t)(first + threadIdx.x) * experts + e] =
+            (part[0][threadIdx.x] + part[1][threadIdx.x]) + (part[2][threadIdx.x] + part[3][threadIdx.x]);
+    if (!plan.x) return;
+    const int units = dp / 8 * mine;
+    for (int u = blockIdx.x * 256 + threadIdx.x; u < units; u += gridDim.x * 256) {
+        const int i = u / (dp / 8), k0 = u % (dp / 8) * 8;
+        float v[8];
+        fp8_load8(x + (size_t)(first + i) * d, k0, d, vec, v);
+        bf16x8_t out[TERMS];
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            bf16_t t[TERMS];
+            moe_split<TERMS>(v[c], t);
+#pragma unroll
+            for (int s = 0; s < TERMS; s++) out[s][c] = t[s];
+        }
+#pragma unroll
+        for (int s = 0; s < TERMS; s++) *(bf16x8_t *)(plan.x + ((size_t)s * tokens + first + i) * dp + k0) = out[s];
+    }
+}
 
-    // the experts of each token: lane l holds experts per * l .. + per - 1
-    const int per = (experts + 63) / 64;
-    __shared__ int pick_e[128][kMostTop];
-    __shared__ float pick_c[128][kMostTop];
-    for (int t = wave; t < tokens; t += WAVES) {
-        float l[kMostExperts / 64];
-        uint32_t key[kMostExperts / 64];
-        bool fine = true;
-        float most = -3.4028235e38f;
-#pragma unroll
-        for (int i = 0; i < kMostExperts / 64; i++) {
-            const int ex = lane * per + i;
-            const bool here = i < per && ex < experts;
-            l[i] = here ? __hip_atomic_load(plan.logits + (size_t)t * experts + ex, __ATOMIC_RELAXED,
-                                            __HIP_MEMORY_SCOPE_AGENT)
-                        : -3.4028235e38f;
-            key[i] = here ? moe_key(l[i]) : 0u;
-            if (here && !(fabsf(l[i]) <= 3.4028235e38f)) fine = false;
-            most = fmaxf(most, l[i]);
-        }
-        fine = __all(fine);
-        most = wave_max_dpp(most);
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kMostExperts / 64; i++)
-            if (i < per && lane * per + i < experts) sum += expf(l[i] - most);
-        sum = wave_sum_dpp(sum);
-        float picked = 0.0f;
-        for (int s = 0; s < top; s++) {
-            uint32_t best = 0;
-            int at = 0;
-#pragma unroll
-            for (int i = 0; i < kMostExperts / 64; i++)
-                if (key[i] > best) best = key[i], at = i;
-            const uint32_t top_key = moe_wave_max(best);
-            const int owner = __ffsll((unsigned long long)__ballot(best == top_key)) - 1;
-            float p = 0.0f;
-            if (lane == owner) {
-#pragma unroll
-                for (int i = 0; i < kMostExperts / 64; i++)
-                    if (i == at) {
-                        p = expf(l[i] - most);
-                        key[i] = 0;
-                    }
-                pick_e[t][s] = lane * per + at;
-                pick_c[t][s] = p;
-            }
-            picked += __shfl(p, owner);
-        }
-        const float whole = renormalize ? picked : sum;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the owners' picks, read by other lanes
-        if (lane < top) {
-            const float c = fine ? pick_c[t][lane] / whole : __builtin_nanf("");
-            const int ex = pick_e[t][lane];
-            pick_c[t][lane] = c;
-            atomicOr(&mask[ex][t / 32], 1u << (t % 32));
-            if (ids_out) ids_out[t * top + lane] = ex;
-            if (shares_out) shares_out[t * top + lane] = c;
-        }
-    }
-    if (!plan.active) return;
-    __syncthreads();
-    // scan[e]: (chosen experts << 16 | rows) up to and with e
-    static_assert(kMostExperts == kRouteThreads, "an expert a thread");
-    const int ex = threadIdx.x;
-    const int rows = __popc(mask[ex][0]) + __popc(mask[ex][1]) + __popc(mask[ex][2]) + __popc(mask[ex][3]);
-    const uint32_t own = rows ? 0x10000u + (uint32_t)rows : 0u;
-    uint32_t v = own;
-    scan[ex] = v;
-    __syncthreads();
-    for (int o = 1; o < kMostExperts; o *= 2) {
-        const uint32_t add = ex >= o ? scan[ex - o] : 0u;
-        __syncthreads();
-        v += add;
-        scan[ex] = v;
-        __syncthreads();
-    }
-    if (rows) {
-        int *entry = plan.active + 1 + 3 * ((v - own) >> 16);
-        entry[0] = ex;
-        entry[1] = (int)((v - own) & 0xffffu);
-        entry[2] = rows;
-    }
-    if (ex == kMostExperts - 1) plan.active[0] = (int)(v >> 16);
-    for (int u = threadIdx.x; u < tokens * top; u += kRouteThreads) {
-        const int t = u / top, s = u % top, pe = pick_e[t][s];
-        int at = pe ? (int)(scan[pe - 1] & 0xffffu) : 0;
-        for (int w = 0; w < t / 32; w++) at += __popc(mask[pe][w]);
-        at += __popc(mask[pe][t / 32] & ((1u << (t % 32)) - 1u));
-        plan.token[at] = t;
-        plan.share[at] = pick_c[t][s];
+// One wave per token.
+__global__ __launch_bounds__(64) void moe_top_kernel(const float *__restrict__ logits, int experts, int top,
+                                                     int renormalize, int *__restrict__ ids,
+                                                     float *__restrict__ shares) {
+    int e;
+    float c;
+    moe_top_any(logits + (size_t)blockIdx.x * experts, experts, top, renormalize, e, c);
+    if ((int)threadIdx.x < top) {
+        ids[blockIdx.x * top + threadIdx.x] = e;
+        shares[blockIdx.x * top + threadIdx.x] = c;
     }
 }
 
@@ -295,154 +265,435 @@ __device__ __forceinline__ float4_t moe_dot(const MoeWide &w, const MoeWide &x, 
     return d;
 }
 
-constexpr int kGateWaves = 8, kDownWaves = 16;
+constexpr int kGateWaves = 8;
 
-// One workgroup: 16 columns of ff of one chosen expert, gate and up, for all
-// its rows (16 MC at most). The waves split hidden (block b on wave b % 8), so
-// that a wave's loads are few and all in flight; their partials are added in
-// wave order. Columns past ff, up to a whole 128-block, are written as zero.
-template <int MC, int XT, int HT>
-__global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(const uint8_t *__restrict__ codes,
-                                                                      const float *__restrict__ gs,
-                                                                      const float *__restrict__ us, int tokens, int ff,
-                                                                      int kbd, int kbf, int all_rows, MoePlan plan) {
+// One workgroup: tiles of 16 columns of ff (blockIdx.x, + gridDim.x, ...) of one
+// chosen expert, gate and up, for its rows (16 at most). The waves share hidden
+// (block b on wave b % 8); their partials are added in wave order. Codes are
+// loaded a block ahead, across tiles too. Columns past ff, up to a whole 128-block, are written as
+// zero. With fewer slots than experts blockIdx.y is the first slot that chose an
+// expert, else the expert.
+template <int XT, int HT>
+__global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
+    const uint8_t *__restrict__ codes, const float *__restrict__ gs, const float *__restrict__ us, int tokens,
+    int experts, int top, int renormalize, int ff, int kbd, int kbf, MoePlan plan) {
     __shared__ __align__(16) float part[kGateWaves][2][256];
-    const int a = blockIdx.y;
-    if (a >= plan.active[0]) return;
-    const int expert = plan.active[1 + 3 * a], base = plan.active[2 + 3 * a], rows = plan.active[3 + 3 * a];
+    __shared__ int s_ids[kFewTokens * kMostTop], s_slot[kFewTokens];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    const int g = lane / 16, j = lane % 16, t = blockIdx.x, tiles = (ff + 15) / 16;
-    const size_t hp = (size_t)kbf * 128;
-    const int chunks = (rows + 15) / 16;
-    if (t >= tiles) {
-        for (int i = threadIdx.x; i < rows * 16; i += kGateWaves * 64)
-#pragma unroll
-            for (int s = 0; s < HT; s++)
-                plan.h[((size_t)s * all_rows + base + i / 16) * hp + t * 16 + i % 16] = (bf16_t)0.0f;
-        return;
-    }
-    const uint8_t *w = codes + (((size_t)expert * tiles + t) * kbd) * 4096 + lane * 16;
-    const size_t srow = ((size_t)expert * ((ff + 127) / 128) + t / 8) * kbd;
-    bool live[MC];
-    const bf16_t *xr[MC];
-#pragma unroll
-    for (int c = 0; c < MC; c++) {
-        const int r = 16 * c + j;
-        live[c] = r < rows;
-        xr[c] = plan.x + (size_t)(live[c] ? plan.token[base + r] : 0) * kbd * 128 + 16 * g;
-    }
-    float4_t acc[MC][2];
-#pragma unroll
-    for (int c = 0; c < MC; c++) acc[c][0] = acc[c][1] = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < kbd; kb += kGateWaves) {
-        const uint8_t *p = w + (size_t)kb * 4096;
-        MoeWide m[2];
-#pragma unroll
-        for (int o = 0; o < 2; o++)
-            m[o] = moe_widen(__builtin_nontemporal_load((const uint4_t *)(p + o * 2048)),
-                             __builtin_nontemporal_load((const uint4_t *)(p + o * 2048 + 1024)));
-        const float sg = gs[srow + kb], su = us[srow + kb];
-#pragma unroll
-        for (int c = 0; c < MC; c++) {
-            if (c >= chunks) break;
-            float4_t d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-#pragma unroll
-            for (int s = 0; s < XT; s++) {
-                const MoeWide x = moe_rows(xr[c] + (size_t)s * tokens * kbd * 128 + kb * 128, live[c]);
-                d[0] = moe_dot(m[0], x, d[0]);
-                d[1] = moe_dot(m[1], x, d[1]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                acc[c][0][e] = __builtin_fmaf(d[0][e], sg, acc[c][0][e]);
-                acc[c][1][e] = __builtin_fmaf(d[1][e], su, acc[c][1][e]);
-            }
+    const int g = lane / 16, j = lane % 16, tiles = (ff + 15) / 16, slots = tokens * top;
+    const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
+    for (int i = wave; i < tokens; i += kGateWaves) {
+        int e;
+        float c;
+        moe_top_any(plan.logits + (size_t)i * experts, experts, top, renormalize, e, c);
+        if (lane < top) {
+            s_ids[i * top + lane] = e;
+            if (writes) plan.ids[i * top + lane] = e, plan.shares[i * top + lane] = c;
         }
     }
+    __syncthreads();
+    const bool by_slot = slots <= experts;
+    const int expert = __builtin_amdgcn_readfirstlane(by_slot ? s_ids[blockIdx.y] : (int)blockIdx.y);
+    int rows = 0;
+    for (int s0 = 0; s0 < slots; s0 += 64) {
+        const int s = s0 + lane;
+        const bool hit = s < slots && s_ids[s] == expert;
+        const unsigned long long hits = __ballot(hit);
+        if (by_slot && hits && rows == 0 && s0 + __ffsll(hits) - 1 != (int)blockIdx.y) return;  // an earlier slot has it
+        if (hit) s_slot[rows + __popcll(hits & ((1ull << lane) - 1))] = s;  // every wave writes the same
+        rows += __popcll(hits);
+    }
+    if (rows == 0) return;
+    __syncthreads();
+    const size_t hp = (size_t)kbf * 128;
+    const uint8_t *w = codes + (size_t)expert * tiles * kbd * 4096 + lane * 16;
+    const size_t srow = (size_t)expert * ((ff + 127) / 128) * kbd;
+    // x is loaded ahead too where it is one term; two or three terms wait for
+    // the L2 instead of taking the registers of other waves
+    constexpr bool kAhead = XT == 1;
+    const bool live = j < rows;
+    const bf16_t *xr = plan.x + (size_t)(live ? s_slot[j] / top : 0) * kbd * 128 + 16 * g;
+    struct Block {
+        uint4_t w[2][2];
+        float s[2];
+        MoeWide x[kAhead ? XT : 1];
+    };
+    auto x_of = [&](int kb, int i) {
+        return moe_rows(xr + (size_t)i * tokens * kbd * 128 + kb * 128, live);
+    };
+    auto load = [&](int t, int kb, Block &b) {
+        const uint8_t *p = w + ((size_t)t * kbd + kb) * 4096;
 #pragma unroll
-    for (int c = 0; c < MC; c++) {
-        if (c >= chunks) break;
-        if (c) __syncthreads();
-        *(float4_t *)&part[wave][0][j * 16 + 4 * g] = acc[c][0];
-        *(float4_t *)&part[wave][1][j * 16 + 4 * g] = acc[c][1];
+        for (int o = 0; o < 2; o++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                b.w[o][h] = __builtin_nontemporal_load((const uint4_t *)(p + o * 2048 + h * 1024));
+        b.s[0] = gs[srow + (size_t)(t / 8) * kbd + kb];
+        b.s[1] = us[srow + (size_t)(t / 8) * kbd + kb];
+        if constexpr (kAhead) b.x[0] = x_of(kb, 0);
+    };
+    float4_t acc[2];
+    auto step = [&](int t, int kb, Block &now, Block &next) {
+        MoeWide x[XT];
+        if constexpr (kAhead) {
+            x[0] = now.x[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < XT; i++) x[i] = x_of(kb, i);
+        }
+        if (kb + kGateWaves < kbd) load(t, kb + kGateWaves, next);
+        else if (t + (int)gridDim.x < tiles) load(t + gridDim.x, wave, next);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int o = 0; o < 2; o++) {
+            const MoeWide m = moe_widen(now.w[o][0], now.w[o][1]);
+            float4_t d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < XT; i++) d = moe_dot(m, x[i], d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[o][e] = __builtin_fmaf(d[e], now.s[o], acc[o][e]);
+        }
+    };
+    Block b[2];
+    if (wave < kbd && (int)blockIdx.x < tiles) load(blockIdx.x, wave, b[0]);
+    for (int t = blockIdx.x; t < kbf * 8; t += gridDim.x) {
+        acc[0] = acc[1] = float4_t{0.f, 0.f, 0.f, 0.f};
+        if (wave < kbd && t < tiles) {
+            for (int kb = wave; kb < kbd; kb += 2 * kGateWaves) {
+                step(t, kb, b[0], b[1]);
+                if (kb + kGateWaves < kbd) step(t, kb + kGateWaves, b[1], b[0]);
+                else b[0] = b[1];  // the next tile's first block
+            }
+        }
         __syncthreads();
-        const int i = threadIdx.x;
-        if (i < 256 && 16 * c + i / 16 < rows) {
+        *(float4_t *)&part[wave][0][j * 16 + 4 * g] = acc[0];
+        *(float4_t *)&part[wave][1][j * 16 + 4 * g] = acc[1];
+        __syncthreads();
+        const int i = threadIdx.x, r = i / 16;
+        if (i < 256 && r < rows) {
             float gate = part[0][0][i], up = part[0][1][i];
 #pragma unroll
             for (int v = 1; v < kGateWaves; v++) gate += part[v][0][i], up += part[v][1][i];
             bf16_t out[HT];
-            moe_split<HT>(gate / (1.0f + expf(-gate)) * up, out);
+            moe_split<HT>(t < tiles ? gate / (1.0f + expf(-gate)) * up : 0.0f, out);
 #pragma unroll
-            for (int s = 0; s < HT; s++)
-                plan.h[((size_t)s * all_rows + base + 16 * c + i / 16) * hp + t * 16 + i % 16] = out[s];
+            for (int s = 0; s < HT; s++) plan.h[((size_t)s * slots + s_slot[r]) * hp + t * 16 + i % 16] = out[s];
         }
     }
 }
 
 // One workgroup: 16 columns of y. Units (chosen expert, 128-block of ff) in
-// order, an equal run of them to each wave; a wave adds its experts' rows,
-// times their shares, into its own copy of the 16 columns in LDS, and the
-// copies are added in wave order.
-template <int MC, int HT>
-__global__ __launch_bounds__(kDownWaves * 64) void moe_down_kernel(const uint8_t *__restrict__ codes,
-                                                                   const float *__restrict__ ds, int tokens, int d,
-                                                                   int kbf, int all_rows, MoePlan plan,
+// order, an equal run of them to each wave; a wave adds its rows, times
+// their shares, into its own copy of the 16 columns in LDS, and the copies are
+// added in wave order. The rows are sorted
+// by expert in LDS first, with bit masks of each expert's tokens: one trip to
+// memory for the slots' experts, not one for each list.
+template <int HT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__restrict__ codes,
+                                                                   const float *__restrict__ ds, int tokens,
+                                                                   int experts, int top, int d, int kbf, MoePlan plan,
                                                                    void *__restrict__ y, int dtype) {
-    __shared__ __align__(16) float sums[kDownWaves * MC * 256];  // [waves][tokens][16]
+    constexpr int THREADS = WAVES * 64, kSlots = kFewTokens * kMostTop, kStage = 16 * HT * 256;  // one unit of 16 rows
+    static_assert(kSlots <= THREADS && kFewTokens <= 16, "a slot a thread, a bit a token");
+    __shared__ __align__(16) uint8_t lds[WAVES * kStage];
+    __shared__ __align__(16) float sums[WAVES * kFewTokens * 16];  // [waves][tokens][16]
+    __shared__ uint32_t s_mask[kMostExperts];  // the expert's tokens, its first row << 16
+    __shared__ int s_first[kSlots];            // per chosen expert: its first row << 8 | rows
+    __shared__ short s_expert[kSlots];
+    __shared__ int s_slot[kSlots];
+    __shared__ float s_share[kSlots];
+    __shared__ int s_active;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    const int g = lane / 16, j = lane % 16, t = blockIdx.x, tiles = (d + 15) / 16;
+    const int g = lane / 16, j = lane % 16, t = blockIdx.x, tiles = (d + 15) / 16, slots = tokens * top;
     const size_t hp = (size_t)kbf * 128;
     float *mine = sums + (size_t)wave * tokens * 16;
+    const int my_slot = threadIdx.x, my_token = my_slot / top;
+    const int my_expert = my_slot < slots ? plan.ids[my_slot] : 0;
+    const float my_share = my_slot < slots ? plan.shares[my_slot] : 0.0f;
+    for (int i = threadIdx.x; i < experts; i += THREADS) s_mask[i] = 0;
     for (int i = lane; i < tokens * 4; i += 64) ((float4_t *)mine)[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const int units = plan.active[0] * kbf;
-    const int u0 = (int)((int64_t)units * wave / kDownWaves), u1 = (int)((int64_t)units * (wave + 1) / kDownWaves);
+    __syncthreads();
+    if (my_slot < slots) atomicOr(&s_mask[my_expert], 1u << my_token);
+    __syncthreads();
+    if (wave == 0) {  // first rows, expert by expert: lane l has experts 8 l .. 8 l + 7
+        uint32_t sum = 0;  // chosen << 16 | rows
+        int count[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            count[i] = lane * 8 + i < experts ? __popc(s_mask[lane * 8 + i]) : 0;
+            sum += count[i] ? 0x10000u + (uint32_t)count[i] : 0u;
+        }
+        uint32_t upto = sum;
+        for (int o = 1; o < 64; o *= 2) {
+            const uint32_t before = (uint32_t)__shfl_up((int)upto, o);
+            if (lane >= o) upto += before;
+        }
+        uint32_t at = upto - sum;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (count[i] == 0) continue;
+            s_mask[lane * 8 + i] |= at << 16;
+            s_first[at >> 16] = (int)(at & 0xffffu) << 8 | count[i];
+            s_expert[at >> 16] = (short)(lane * 8 + i);
+            at += 0x10000u + (uint32_t)count[i];
+        }
+        if (lane == 63) s_active = (int)(upto >> 16);
+    }
+    __syncthreads();
+    const int units = __builtin_amdgcn_readfirstlane(s_active) * kbf;
+    const int u0 = (int)((int64_t)units * wave / WAVES), u1 = (int)((int64_t)units * (wave + 1) / WAVES);
+    if (my_slot < slots) {
+        const uint32_t m = s_mask[my_expert];
+        const int at = (int)(m >> 16) + __popc(m & 0xffffu & ((1u << my_token) - 1u));
+        s_slot[at] = my_slot;
+        s_share[at] = my_share;
+    }
+    __syncthreads();
+    // A run of units of one expert at a time. h of a batch of units goes through
+    // this wave's part of LDS: whole rows of it, loaded without registers and all
+    // at once, while the operands in memory order would leave most lanes of a load
+    // idle where an expert has a row or two. Codes of up to four units together.
+    uint8_t *stage = lds + wave * kStage;
+    const uint32_t stage0 = __builtin_amdgcn_readfirstlane(lds_address(stage));
+    const int32x4_t rh = buffer_rsrc(plan.h, (uint32_t)((size_t)HT * slots * hp * 2));
     for (int u = u0; u < u1;) {
-        const int a = u / kbf, end = min(u1, (a + 1) * kbf);
-        const int expert = plan.active[1 + 3 * a], base = plan.active[2 + 3 * a], rows = plan.active[3 + 3 * a];
-        const int chunks = (rows + 15) / 16;
+        const int a = u / kbf, k0 = u - a * kbf, k1 = min(kbf, k0 + u1 - u);
+        u += k1 - k0;
+        const int expert = __builtin_amdgcn_readfirstlane((int)s_expert[a]);
+        const int group = __builtin_amdgcn_readfirstlane(s_first[a]), first = group >> 8, rows = group & 255;
         const uint8_t *w = codes + ((size_t)expert * tiles + t) * kbf * 2048 + lane * 16;
         const float *sw = ds + ((size_t)expert * ((d + 127) / 128) + t / 8) * kbf;
-        float4_t acc[MC];
-#pragma unroll
-        for (int c = 0; c < MC; c++) acc[c] = float4_t{0.f, 0.f, 0.f, 0.f};
-        for (; u < end; u++) {
-            const int kb = u - a * kbf;
-            const MoeWide m = moe_widen(__builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 2048)),
-                                        __builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 2048 + 1024)));
-            const float s = sw[kb];
-#pragma unroll
-            for (int c = 0; c < MC; c++) {
-                if (c >= chunks) break;
-                const int r = 16 * c + j;
-                float4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < HT; i++)
-                    v = moe_dot(m, moe_rows(plan.h + ((size_t)i * all_rows + base + r) * hp + kb * 128 + 16 * g, r < rows), v);
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[c][e] = __builtin_fmaf(v[e], s, acc[c][e]);
+        // the batch: the most units, a power of two, whose rows fit the stage
+        int log_nb = 0;
+        while (log_nb < 4 && (rows * HT * 256 << (log_nb + 1)) <= kStage && (1 << log_nb) < k1 - k0) log_nb++;
+        const int nb = 1 << log_nb, pieces = rows * HT << (log_nb + 4);
+        float4_t acc = {0.f, 0.f, 0.f, 0.f};
+        for (int kb0 = k0; kb0 < k1; kb0 += nb) {
+            // piece p: row and term p / (16 nb), 16 bytes p % (16 nb) of the batch's columns
+            for (int p0 = 0; p0 < pieces; p0 += 64) {
+                const int p = p0 + lane, rt = p >> (log_nb + 4), r = rt / HT, i = rt - r * HT;
+                const uint32_t at = p < pieces
+                                        ? (uint32_t)(((size_t)i * slots + s_slot[first + r]) * hp * 2 + kb0 * 256 +
+                                                     (p & ((16 << log_nb) - 1)) * 16)
+                                        : 0x80000000u;
+                dma16_at(stage0 + p0 * 16, at, rh, 0u);
             }
-        }
+            const int kend = min(k1, kb0 + nb);
+            for (int k = kb0; k < kend; k += 4) {
+                uint4_t wb[4][2];
+                float s[4];
 #pragma unroll
-        for (int c = 0; c < MC; c++) {
-            const int r = 16 * c + j;
-            if (c >= chunks || r >= rows) break;
-            float4_t *at = (float4_t *)(mine + plan.token[base + r] * 16 + 4 * g);
-            const float share = plan.share[base + r];
+                for (int i = 0; i < 4; i++) {
+                    const int kb = min(k + i, kend - 1);
+                    wb[i][0] = __builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 2048));
+                    wb[i][1] = __builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 2048 + 1024));
+                    s[i] = sw[kb];
+                }
+                if (k == kb0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (k + i >= kend) break;
+                    const MoeWide m = moe_widen(wb[i][0], wb[i][1]);
+                    float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int o = 0; o < HT; o++) {
+                        const uint8_t *at = stage + (((j * HT + o) << log_nb) + k + i - kb0) * 256 + 32 * g;
+                        MoeWide x;
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            x.h[q] = bf16x8_t{};
+                            if (j < rows) x.h[q] = *(const bf16x8_t *)(at + q / 2 * 128 + q % 2 * 16);
+                        }
+                        v = moe_dot(m, x, v);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(v[e], s[i], acc[e]);
+                }
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next batch lands
+        }
+        if (j < rows) {  // the run's rows into this wave's sums
+            float4_t *at = (float4_t *)(mine + s_slot[first + j] / top * 16 + 4 * g);
+            const float share = s_share[first + j];
             float4_t v = *at;
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(acc[c][e], share, v[e]);
+            for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(acc[e], share, v[e]);
             *at = v;
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < tokens * 16; i += kDownWaves * 64) {
+    for (int i = threadIdx.x; i < tokens * 16; i += THREADS) {
         const int col = t * 16 + i % 16;
         if (col >= d) continue;
         float v = sums[i];
-        for (int w = 1; w < kDownWaves; w++) v += sums[(size_t)w * tokens * 16 + i];
+        for (int w = 1; w < WAVES; w++) v += sums[(size_t)w * tokens * 16 + i];
         fp8_store(y, dtype, (size_t)(i / 16) * d + col, v);
     }
+}
+
+// ---- more tokens ------------------------------------------------------------------
+
+// The rows of an expert against its weight where tokens are many enough that
+// most experts have several rows: eight waves side by side, two 16-column tiles
+// each (GATE: gate and up of one tile of ff, and h = silu(gate) * up; else two
+// tiles of the output, f32 rows by slot that moe_combine_kernel sums). A step is
+// a 128-block of the width: a wave's own 4 KiB of codes and the block's rows,
+// which all waves share, through NS LDS stages by buffer_load ... lds. Loaded by
+// each wave for itself instead, the rows cost more than the weight (x of eight
+// rows in f32 is three times a tile's codes). A row's 256 bytes of a term are 16
+// pieces, piece p of row r in slot p ^ (r & 15), so that 16 rows' reads meet
+// distinct banks. 16 MC rows at a time; more read the weight again.
+template <int MC, int XT, int HT, bool GATE, int NS>
+__global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict__ codes,
+                                                       const float *__restrict__ s0, const float *__restrict__ s1,
+                                                       int tokens, int experts, int top, int n, int kbs, int out_width,
+                                                       const bf16_t *__restrict__ in, MoePlan plan) {
+    constexpr int WAVES = 8, RT = XT * 16 * MC, LOADS = RT / 4, XPW = (LOADS + WAVES - 1) / WAVES, PB = 4 + XPW;
+    constexpr int XB = WAVES * 4096, STAGE = XB + RT * 256;
+    static_assert((NS - 2) * PB <= 63, "vmcnt range");
+    __shared__ __align__(16) uint8_t lds[NS * STAGE];
+    __shared__ int s_slot[DZ_MOE_MAX_TOKENS];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int g = lane / 16, j = lane % 16, slots = tokens * top, tiles = (n + 15) / 16;
+    const bool by_slot = slots <= experts;
+    const int expert = __builtin_amdgcn_readfirstlane(by_slot ? plan.ids[blockIdx.y] : (int)blockIdx.y);
+    int rows = 0;
+    for (int b = 0; b < slots; b += 64) {
+        const int s = b + lane;
+        const bool hit = s < slots && plan.ids[s] == expert;
+        const unsigned long long hits = __ballot(hit);
+        if (by_slot && hits && rows == 0 && b + __ffsll(hits) - 1 != (int)blockIdx.y) return;  // an earlier slot has it
+        if (hit) s_slot[rows + __popcll(hits & ((1ull << lane) - 1))] = s;  // every wave writes the same
+        rows += __popcll(hits);
+    }
+    if (rows == 0) return;
+    __syncthreads();
+
+    // this wave's tiles: one of gate and up, or two; past the last one zeros are loaded
+    const int t0 = GATE ? blockIdx.x * WAVES + wave : (blockIdx.x * WAVES + wave) * 2;
+    const size_t matrix = (size_t)tiles * kbs * (GATE ? 4096 : 2048);
+    const uint8_t *wbase = codes + (size_t)expert * matrix + (size_t)t0 * kbs * (GATE ? 4096 : 2048);
+    const int have = max(0, min(GATE ? 1 : 2, tiles - t0));
+    const int32x4_t rw = buffer_rsrc(have ? wbase : codes, (uint32_t)have * kbs * (GATE ? 4096u : 2048u));
+    uint32_t woff[4];
+#pragma unroll
+    for (int p = 0; p < 4; p++)
+        woff[p] = GATE ? (uint32_t)(p * 1024 + lane * 16) : (uint32_t)(p / 2 * kbs * 2048 + p % 2 * 1024 + lane * 16);
+    const int blocks = (n + 127) / 128;
+    const float *sw[2];
+#pragma unroll
+    for (int o = 0; o < 2; o++)
+        sw[o] = (GATE && o ? s1 : s0) + ((size_t)expert * blocks + min((GATE ? t0 : t0 + o) / 8, blocks - 1)) * kbs;
+    const int in_rows = GATE ? tokens : slots, width = kbs * 128;
+    const int32x4_t rx = buffer_rsrc(in, (uint32_t)((size_t)XT * in_rows * width * 2));
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
+
+    for (int r0 = 0; r0 < rows; r0 += 16 * MC) {
+        const int chunks = min(MC, (rows - r0 + 15) / 16);
+        // load p of this wave: four (term, row)s, 16 lanes each
+        uint32_t xoff[XPW];
+        int xload[XPW];
+#pragma unroll
+        for (int p = 0; p < XPW; p++) {
+            xload[p] = (wave * XPW + p) % LOADS;
+            const int rt = xload[p] * 4 + lane / 16, i = rt / (16 * MC), r = rt % (16 * MC);
+            const int from = r0 + r < rows ? (GATE ? s_slot[r0 + r] / top : s_slot[r0 + r]) : -1;
+            xoff[p] = from < 0 ? 0x80000000u
+                               : (uint32_t)(((size_t)i * in_rows + from) * width * 2 + ((lane % 16) ^ (r & 15)) * 16);
+        }
+        // past the last block nothing is loaded (every offset out of range), so that all waits go by count
+        auto load_stage = [&](int stage, int kb) {
+            const bool live = kb < kbs;
+            const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u;
+#pragma unroll
+            for (int p = 0; p < XPW; p++)
+                dma16_at(at + XB + xload[p] * 1024, xoff[p] | past, rx, live ? (uint32_t)kb * 256 : 0u);
+#pragma unroll
+            for (int p = 0; p < 4; p++)
+                dma16_at(at + wave * 4096 + p * 1024, woff[p] | past, rw,
+                         live && have ? (uint32_t)kb * (GATE ? 4096u : 2048u) : 0u);
+        };
+        float4_t acc[MC][2];
+#pragma unroll
+        for (int c = 0; c < MC; c++) acc[c][0] = acc[c][1] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = 0; p < NS - 1; p++) load_stage(p, p);
+        float sc[2] = {sw[0][0], sw[1][0]};
+        int stage = 0;
+        for (int kb = 0; kb < kbs; kb++) {
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
+            load_stage(stage == 0 ? NS - 1 : stage - 1, kb + NS - 1);  // the stage that the step before read
+            const int after = min(kb + 1, kbs - 1);
+            const float next[2] = {sw[0][after], sw[1][after]};
+            const uint8_t *st = lds + stage * STAGE, *ws = st + wave * 4096 + lane * 16;
+            MoeWide m[2];
+#pragma unroll
+            for (int o = 0; o < 2; o++)
+                m[o] = moe_widen(*(const uint4_t *)(ws + o * 2048), *(const uint4_t *)(ws + o * 2048 + 1024));
+#pragma unroll
+            for (int c = 0; c < MC; c++) {
+                if (c >= chunks) break;
+                float4_t d[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                for (int i = 0; i < XT; i++) {
+                    const uint8_t *row = st + XB + ((i * MC + c) * 16 + j) * 256;
+                    MoeWide x;
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        x.h[q] = *(const bf16x8_t *)(row + ((q / 2 * 8 + 2 * g + q % 2) ^ j) * 16);
+                    d[0] = moe_dot(m[0], x, d[0]);
+                    d[1] = moe_dot(m[1], x, d[1]);
+                }
+#pragma unroll
+                for (int o = 0; o < 2; o++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[c][o][e] = __builtin_fmaf(d[o][e], sc[o], acc[c][o][e]);
+            }
+            sc[0] = next[0];
+            sc[1] = next[1];
+            stage = stage + 1 == NS ? 0 : stage + 1;
+        }
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // no LDS write in flight, every stage read
+#pragma unroll
+        for (int c = 0; c < MC; c++) {
+            const int r = r0 + 16 * c + j;
+            if (r >= rows) break;
+            const size_t slot = s_slot[r];
+            if constexpr (GATE) {
+                bf16_t out[4][HT];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float gate = acc[c][0][e];
+                    moe_split<HT>(gate / (1.0f + expf(-gate)) * acc[c][1][e], out[e]);
+                }
+#pragma unroll
+                for (int i = 0; i < HT; i++) {
+                    const bf16x2_t lo = {out[0][i], out[1][i]}, hi = {out[2][i], out[3][i]};
+                    *(uint2_t *)(plan.h + ((size_t)i * slots + slot) * out_width + t0 * 16 + 4 * g) =
+                        uint2_t{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+                }
+            } else {
+#pragma unroll
+                for (int o = 0; o < 2; o++)
+                    if (o < have) *(float4_t *)(plan.p + slot * out_width + (t0 + o) * 16 + 4 * g) = acc[c][o];
+            }
+        }
+    }
+}
+
+// y of a token: its slots' rows times their shares, in order.
+__global__ __launch_bounds__(256) void moe_combine_kernel(MoePlan plan, int top, int d, int width, void *__restrict__ y,
+                                                          int dtype, int vec) {
+    const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
+    if (c >= d) return;
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < top; i++) {
+        const float share = plan.shares[t * top + i];
+        const float4_t p = *(const float4_t *)(plan.p + (size_t)(t * top + i) * width + c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(p[e], share, v[e]);
+    }
+    fp8_store4(y, dtype, (size_t)t * d + c, v, d - c, vec);
 }
 
 template <class T>
@@ -473,48 +724,73 @@ size_t moe_plan(const dz_moe *e, size_t tokens, int dtype, bool forward, uint8_t
     MoePlan p{};
     p.logits = (float *)take(tokens * e->cfg.experts * sizeof(float));
     if (forward) {
-        p.active = (int *)take((1 + 3 * (size_t)e->cfg.experts) * sizeof(int));
-        p.token = (int *)take(rows * sizeof(int));
-        p.share = (float *)take(rows * sizeof(float));
+        p.ids = (int *)take(rows * sizeof(int));
+        p.shares = (float *)take(rows * sizeof(float));
         p.x = (bf16_t *)take(tokens * terms_of_x(dtype) * e->kbd * 256);
         p.h = (bf16_t *)take(rows * terms_of_h(dtype) * e->kbf * 256);
+        if (tokens > kFewTokens) p.p = (float *)take(rows * e->kbd * 512);
     }
     if (plan) *plan = p;
     return at;
 }
 
-void launch_route(const dz_moe *e, const void *x, int dtype, int tokens, const MoePlan &plan, int *ticket, int *ids,
-                  float *shares, hipStream_t s) {
+void launch_logits(const dz_moe *e, const void *x, int dtype, int tokens, const MoePlan &plan, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
-    const dim3 grid(cdiv(c.experts, kRouteThreads / 64), cdiv(tokens, kRouteTokens));
+    const dim3 grid(c.experts, cdiv(tokens, kRouteTokens));
     const int vec = c.hidden % 8 == 0 && ((uintptr_t)x & 15) == 0;
     if (dtype == DZ_F32)
-        hipLaunchKernelGGL((moe_route_kernel<float, 3>), grid, dim3(kRouteThreads), 0, s, (const float *)x, e->router,
-                           tokens, c.experts, c.top_k, c.hidden, e->kbd, c.renormalize, vec, plan, ticket, ids, shares);
+        hipLaunchKernelGGL((moe_logits_kernel<float, 3>), grid, dim3(256), 0, s, (const float *)x, e->router, tokens,
+                           c.experts, c.hidden, e->kbd, vec, plan);
     else if (dtype == DZ_F16)
-        hipLaunchKernelGGL((moe_route_kernel<half_t, 2>), grid, dim3(kRouteThreads), 0, s, (const half_t *)x, e->router,
-                           tokens, c.experts, c.top_k, c.hidden, e->kbd, c.renormalize, vec, plan, ticket, ids, shares);
+        hipLaunchKernelGGL((moe_logits_kernel<half_t, 2>), grid, dim3(256), 0, s, (const half_t *)x, e->router, tokens,
+                           c.experts, c.hidden, e->kbd, vec, plan);
     else
-        hipLaunchKernelGGL((moe_route_kernel<bf16_t, 1>), grid, dim3(kRouteThreads), 0, s, (const bf16_t *)x, e->router,
-                           tokens, c.experts, c.top_k, c.hidden, e->kbd, c.renormalize, vec, plan, ticket, ids, shares);
+        hipLaunchKernelGGL((moe_logits_kernel<bf16_t, 1>), grid, dim3(256), 0, s, (const bf16_t *)x, e->router, tokens,
+                           c.experts, c.hidden, e->kbd, vec, plan);
 }
 
-template <int MC, int XT, int HT>
-void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+void launch_top(const dz_moe *e, int tokens, const MoePlan &plan, int *ids, float *shares, hipStream_t s) {
+    hipLaunchKernelGGL(moe_top_kernel, dim3(tokens), dim3(64), 0, s, plan.logits, e->cfg.experts, e->cfg.top_k,
+                       e->cfg.renormalize, ids, shares);
+}
+
+template <int XT, int HT>
+void launch_few(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
-    const int rows = tokens * c.top_k;
-    hipLaunchKernelGGL((moe_gate_up_kernel<MC, XT, HT>), dim3(e->kbf * 8, std::min(rows, c.experts)),
-                       dim3(kGateWaves * 64), 0, s, e->gate_up, e->gate_scales, e->up_scales, tokens, c.ff, e->kbd,
-                       e->kbf, rows, plan);
-    hipLaunchKernelGGL((moe_down_kernel<MC, HT>), dim3(cdiv(c.hidden, 16)), dim3(kDownWaves * 64), 0, s, e->down,
-                       e->down_scales, tokens, c.hidden, e->kbf, rows, plan, y, dtype);
+    const int entries = std::min(tokens * c.top_k, c.experts);
+    // two workgroups a compute unit fit; each goes through its share of the tiles
+    const unsigned tiles = e->kbf * 8, share = std::max(1u, 2u * (unsigned)device_cus() / entries);
+    hipLaunchKernelGGL((moe_gate_up_kernel<XT, HT>), dim3(std::min(tiles, share), entries), dim3(kGateWaves * 64), 0, s,
+                       e->gate_up, e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.renormalize, c.ff,
+                       e->kbd, e->kbf, plan);
+    constexpr int WAVES = HT == 3 ? 8 : 16;  // a unit's rows of each wave fit LDS
+    hipLaunchKernelGGL((moe_down_kernel<HT, WAVES>), dim3(cdiv(c.hidden, 16)), dim3(WAVES * 64), 0, s, e->down,
+                       e->down_scales, tokens, c.experts, c.top_k, c.hidden, e->kbf, plan, y, dtype);
 }
 
-template <int MC>
-void launch_experts_dtype(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
-    if (dtype == DZ_F32) return launch_experts<MC, 3, 3>(e, dtype, tokens, plan, y, s);
-    if (dtype == DZ_F16) return launch_experts<MC, 2, 2>(e, dtype, tokens, plan, y, s);
-    return launch_experts<MC, 1, 2>(e, dtype, tokens, plan, y, s);
+template <int MC, int XT, int HT, int NSX, int NSH>
+void launch_wide(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+    const dz_moe_config &c = e->cfg;
+    const int entries = std::min(tokens * c.top_k, c.experts), width = e->kbd * 128;
+    hipLaunchKernelGGL((moe_wide_kernel<MC, XT, HT, true, NSX>), dim3(e->kbf, entries), dim3(512), 0, s, e->gate_up,
+                       e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.ff, e->kbd, e->kbf * 128, plan.x,
+                       plan);
+    hipLaunchKernelGGL((moe_wide_kernel<MC, HT, HT, false, NSH>), dim3(cdiv(c.hidden, 256), entries), dim3(512), 0, s,
+                       e->down, e->down_scales, nullptr, tokens, c.experts, c.top_k, c.hidden, e->kbf, width, plan.h,
+                       plan);
+    const int vec = c.hidden % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(c.hidden, 1024), tokens), dim3(256), 0, s, plan, c.top_k, c.hidden,
+                       width, y, dtype, vec);
+}
+
+// Stages of 32 KiB of codes and 4 (terms of the rows) KiB, twice that for 32
+// rows at a time: as many as fit a compute unit's 160 KiB.
+template <int XT, int HT>
+void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+    if (tokens <= kFewTokens) return launch_few<XT, HT>(e, dtype, tokens, plan, y, s);
+    launch_top(e, tokens, plan, plan.ids, plan.shares, s);
+    if (tokens * e->cfg.top_k <= 12 * e->cfg.experts) launch_wide<1, XT, HT, XT == 1 ? 4 : 3, 3>(e, dtype, tokens, plan, y, s);
+    else launch_wide<2, XT, HT, XT == 3 ? 2 : 3, HT == 3 ? 2 : 3>(e, dtype, tokens, plan, y, s);
 }
 
 void moe_release(dz_moe *e) {
@@ -625,7 +901,8 @@ int32_t moe_route(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, si
     if (int32_t rc = ctx_workspace(ctx, moe_plan(e, tokens, dtype, false, nullptr, nullptr), &work)) return rc;
     MoePlan plan;
     moe_plan(e, tokens, dtype, false, (uint8_t *)work, &plan);
-    launch_route(e, x, dtype, (int)tokens, plan, ctx_ticket(ctx), ids, shares, ctx_stream(ctx));
+    launch_logits(e, x, dtype, (int)tokens, plan, ctx_stream(ctx));
+    launch_top(e, (int)tokens, plan, ids, shares, ctx_stream(ctx));
     return ctx_launched(ctx, "mixture of experts route");
 }
 
@@ -637,12 +914,11 @@ int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, 
     MoePlan plan;
     moe_plan(e, tokens, dtype, true, (uint8_t *)work, &plan);
     hipStream_t s = ctx_stream(ctx);
-    launch_route(e, x, dtype, (int)tokens, plan, ctx_ticket(ctx), nullptr, nullptr, s);
     const int t = (int)tokens;
-    if (t <= 16) launch_experts_dtype<1>(e, dtype, t, plan, y, s);
-    else if (t <= 32) launch_experts_dtype<2>(e, dtype, t, plan, y, s);
-    else if (t <= 64) launch_experts_dtype<4>(e, dtype, t, plan, y, s);
-    else launch_experts_dtype<8>(e, dtype, t, plan, y, s);
+    launch_logits(e, x, dtype, t, plan, s);
+    if (dtype == DZ_F32) launch_experts<3, 3>(e, dtype, t, plan, y, s);
+    else if (dtype == DZ_F16) launch_experts<2, 2>(e, dtype, t, plan, y, s);
+    else launch_experts<1, 2>(e, dtype, t, plan, y, s);
     return ctx_launched(ctx, "mixture of experts");
 }
 

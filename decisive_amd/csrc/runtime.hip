@@ -33,8 +33,7 @@ struct dz_ctx {
     int cus = 0;
     int clock_khz = 0;
     // device ints: [0] validation / non-finite flag, [1..62] the product flag
-    // ring, [kTicketSlot] the ticket of the mixture-of-experts router (0 between
-    // calls), [kCaptureSlot0 ..] one flag per product recorded under stream capture
+    // ring, [kCaptureSlot0 ..] one flag per product recorded under stream capture
     int *flag = nullptr;
     uint64_t product_calls = 0;  // ring products since the last stream change (picks the slot)
     int captured_flags = 0;      // capture slots ever handed out (the high-water mark)
@@ -164,7 +163,6 @@ int variant(dz_ctx *ctx, const char *family) {
 }
 
 constexpr int kRingSlots = 62;
-constexpr int kTicketSlot = 63;
 constexpr int kCaptureSlot0 = 64;
 constexpr int kCaptureSlots = 4032;  // 16 KiB flag buffer
 constexpr size_t kFlagBytes = (size_t)(kCaptureSlot0 + kCaptureSlots) * sizeof(int);
@@ -1378,7 +1376,6 @@ int32_t ctx_fail(dz_ctx *ctx, int32_t code, const std::string &msg) { return fai
 int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what) { return hip_fail(ctx, e, what); }
 hipStream_t ctx_stream(dz_ctx *ctx) { return ctx->stream; }
 int *ctx_flag(dz_ctx *ctx) { return ctx->flag; }
-int *ctx_ticket(dz_ctx *ctx) { return ctx->flag + kTicketSlot; }
 int ctx_device(dz_ctx *ctx) { return ctx->device; }
 int32_t ctx_launched(dz_ctx *ctx, const char *what) { return launched(ctx, what); }
 // Waits for the work just enqueued, whose kernels report in the context's flag, and reads it.
