@@ -8,15 +8,16 @@
 // weight than they multiply (2 operations a byte and row), so the layer is
 // bound by the bytes of the experts that are chosen, each read once:
 //   1 moe_logits_kernel   logits, and x as bf16 terms
-// up to 16 tokens, where launches and trips to memory count:
 //   2 moe_gate_up_kernel  finds each token's experts; per (chosen expert, 16
-//                         columns of ff): h = silu(gate) * up of its rows
+//                         columns of ff): h = silu(gate) * up of its rows; or
+//     moe_top_kernel      the experts of each token, then
+//     moe_wide_kernel     h, 128 columns of ff a workgroup
 //   3 moe_down_kernel     per 16 columns of the output: every chosen expert's down
-//                         product, times the rows' shares, summed
-// and above:
-//   2 moe_top_kernel      the experts of each token
-//   3, 4 moe_wide_kernel  h, and then each slot's down product
-//   5 moe_combine_kernel  the shares' sum
+//                         product, times the rows' shares, summed; or
+//     moe_wide_kernel     each slot's down product, 256 columns a workgroup, then
+//     moe_combine_kernel  the shares' sum
+// The first of each are for few rows, where launches and trips to memory count
+// (launch_experts has the rule).
 // A token's i-th expert is slot = token * top_k + i, and h has a row for each
 // slot. Each workgroup finds the rows of its experts from the slots' experts,
 // expert by expert and in order of tokens; no order depends on timing.
@@ -60,7 +61,7 @@ namespace {
 
 constexpr int kMostExperts = 512, kMostTop = 16, kMostWidth = 65536;
 constexpr int kRouteTokens = 4;  // tokens a workgroup of the logits kernel takes together
-constexpr int kFewTokens = 16;   // tokens up to which a call goes through the kernels for few
+constexpr int kFewTokens = 16;   // tokens that the kernels for few take
 
 // What the kernels leave for the ones after, in the workspace.
 struct MoePlan {
@@ -69,7 +70,7 @@ struct MoePlan {
     float *shares;  // [slots]
     bf16_t *x;      // [terms][tokens][128 kbd]
     bf16_t *h;      // [terms][slots][128 kbf]
-    float *p;       // [slots][128 kbd] the experts' outputs, past kFewTokens
+    float *p;       // [slots][128 kbd] the experts' outputs, for moe_combine_kernel
 };
 
 // v as TERMS bf16 values that add up to it: each term the leading 8 bits of
@@ -157,12 +158,69 @@ __device__ __forceinline__ void moe_top(const float *__restrict__ logits, int ex
     share = fine ? share / whole : __builtin_nanf("");
 }
 
+// The same for up to 128 experts by counting, for each of a lane's experts (l
+// and l + 64), the larger logits: 64 or 128 comparisons that wait for nothing,
+// where each of moe_top's rounds is a chain of some 40 instructions. Counts that
+// are a permutation say that no two logits are equal; else moe_top decides.
+struct MoeTopShared {
+    uint32_t key[128];
+    int expert[kMostTop];
+    float p[kMostTop];
+};
 __device__ __forceinline__ void moe_top_any(const float *__restrict__ logits, int experts, int top, int renormalize,
-                                            int &expert, float &share) {
-    if (experts <= 64) moe_top<1>(logits, experts, top, renormalize, expert, share);
-    else if (experts <= 128) moe_top<2>(logits, experts, top, renormalize, expert, share);
-    else if (experts <= 256) moe_top<4>(logits, experts, top, renormalize, expert, share);
-    else moe_top<8>(logits, experts, top, renormalize, expert, share);
+                                            MoeTopShared &own, int &expert, float &share) {
+    if (experts > 256) return moe_top<8>(logits, experts, top, renormalize, expert, share);
+    if (experts > 128) return moe_top<4>(logits, experts, top, renormalize, expert, share);
+    const int lane = threadIdx.x % 64;
+    constexpr float kLeast = -3.4028235e38f;
+    float l[2], p[2];
+    uint32_t key[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const bool here = lane + 64 * i < experts;
+        l[i] = here ? logits[lane + 64 * i] : kLeast;
+        key[i] = here ? moe_key(l[i]) : 0u;
+        own.key[lane + 64 * i] = key[i];
+    }
+    const bool fine = __all(fabsf(l[0]) <= 3.4028235e38f && fabsf(l[1]) <= 3.4028235e38f);
+    const float most = wave_max_dpp(fmaxf(l[0], l[1]));
+#pragma unroll
+    for (int i = 0; i < 2; i++) p[i] = lane + 64 * i < experts ? expf(l[i] - most) : 0.0f;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int rank[2] = {0, 0};
+    for (int e0 = 0; e0 < experts; e0 += 16) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const uint4_t other = *(const uint4_t *)&own.key[e0 + e];
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                rank[0] += other[c] > key[0];
+                rank[1] += other[c] > key[1];
+            }
+        }
+    }
+    const int ranks = (lane < experts ? rank[0] : 0) + (lane + 64 < experts ? rank[1] : 0);
+    const float sum = wave_sum_dpp((float)ranks);  // at most 127 * 64: exact
+    if (sum != (float)(experts * (experts - 1) / 2)) {
+        if (experts > 64) moe_top<2>(logits, experts, top, renormalize, expert, share);
+        else moe_top<1>(logits, experts, top, renormalize, expert, share);
+        return;
+    }
+    float part = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+        if (lane + 64 * i < experts) {
+            if (rank[i] < top) {
+                own.expert[rank[i]] = lane + 64 * i;
+                own.p[rank[i]] = p[i];
+            }
+            if (!renormalize || rank[i] < top) part += p[i];
+        }
+    const float whole = wave_sum_dpp(part);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    expert = lane < top ? own.expert[lane] : 0;
+    share = fine ? (lane < top ? own.p[lane] : 0.0f) / whole : __builtin_nanf("");
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // before the wave's next token writes it
 }
 
 // A workgroup takes one expert and four tokens: its waves share hidden, f32
@@ -223,9 +281,10 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x
 __global__ __launch_bounds__(64) void moe_top_kernel(const float *__restrict__ logits, int experts, int top,
                                                      int renormalize, int *__restrict__ ids,
                                                      float *__restrict__ shares) {
+    __shared__ __align__(16) MoeTopShared shared;
     int e;
     float c;
-    moe_top_any(logits + (size_t)blockIdx.x * experts, experts, top, renormalize, e, c);
+    moe_top_any(logits + (size_t)blockIdx.x * experts, experts, top, renormalize, shared, e, c);
     if ((int)threadIdx.x < top) {
         ids[blockIdx.x * top + threadIdx.x] = e;
         shares[blockIdx.x * top + threadIdx.x] = c;
@@ -278,6 +337,7 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
     const uint8_t *__restrict__ codes, const float *__restrict__ gs, const float *__restrict__ us, int tokens,
     int experts, int top, int renormalize, int ff, int kbd, int kbf, MoePlan plan) {
     __shared__ __align__(16) float part[kGateWaves][2][256];
+    __shared__ __align__(16) MoeTopShared s_top[kGateWaves];
     __shared__ int s_ids[kFewTokens * kMostTop], s_slot[kFewTokens];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int g = lane / 16, j = lane % 16, tiles = (ff + 15) / 16, slots = tokens * top;
@@ -285,7 +345,7 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
     for (int i = wave; i < tokens; i += kGateWaves) {
         int e;
         float c;
-        moe_top_any(plan.logits + (size_t)i * experts, experts, top, renormalize, e, c);
+        moe_top_any(plan.logits + (size_t)i * experts, experts, top, renormalize, s_top[wave], e, c);
         if (lane < top) {
             s_ids[i * top + lane] = e;
             if (writes) plan.ids[i * top + lane] = e, plan.shares[i * top + lane] = c;
@@ -681,17 +741,27 @@ __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict
     }
 }
 
-// y of a token: its slots' rows times their shares, in order.
-__global__ __launch_bounds__(256) void moe_combine_kernel(MoePlan plan, int top, int d, int width, void *__restrict__ y,
-                                                          int dtype, int vec) {
-    const int t = blockIdx.y, c = (blockIdx.x * 256 + threadIdx.x) * 4;
+// y of a token: its slots' rows times their shares, in order, four loaded together.
+__global__ __launch_bounds__(64) void moe_combine_kernel(MoePlan plan, int top, int d, int width, void *__restrict__ y,
+                                                         int dtype, int vec) {
+    const int t = blockIdx.y, c = (blockIdx.x * 64 + threadIdx.x) * 4;
     if (c >= d) return;
+    const float *p = plan.p + (size_t)t * top * width + c, *shares = plan.shares + t * top;
     float4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < top; i++) {
-        const float share = plan.shares[t * top + i];
-        const float4_t p = *(const float4_t *)(plan.p + (size_t)(t * top + i) * width + c);
+    for (int i0 = 0; i0 < top; i0 += 4) {
+        float4_t row[4];
+        float share[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(p[e], share, v[e]);
+        for (int i = 0; i < 4; i++) {
+            const int at = min(i0 + i, top - 1);
+            row[i] = *(const float4_t *)(p + (size_t)at * width);
+            share[i] = shares[at];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i0 + i < top)
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(row[i][e], share[i], v[e]);
     }
     fp8_store4(y, dtype, (size_t)t * d + c, v, d - c, vec);
 }
@@ -712,6 +782,12 @@ size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
 int terms_of_x(int dtype) { return dtype == DZ_BF16 ? 1 : dtype == DZ_F16 ? 2 : 3; }
 int terms_of_h(int dtype) { return dtype == DZ_F32 ? 3 : 2; }
 
+bool moe_wide_gate(const dz_moe *e, int tokens, int x_terms) {
+    const size_t grid = (size_t)e->kbf * std::min(tokens * e->cfg.top_k, e->cfg.experts);
+    return tokens > kFewTokens || (x_terms == 3 && grid >= 2 * (size_t)device_cus());
+}
+bool moe_wide_down(const dz_moe *e, int tokens) { return tokens > kFewTokens || tokens * e->cfg.top_k >= 16; }
+
 // The workspace of a call: its size, and with `work` the plan's pointers into it.
 size_t moe_plan(const dz_moe *e, size_t tokens, int dtype, bool forward, uint8_t *work, MoePlan *plan) {
     const size_t rows = tokens * e->cfg.top_k;
@@ -728,7 +804,7 @@ size_t moe_plan(const dz_moe *e, size_t tokens, int dtype, bool forward, uint8_t
         p.shares = (float *)take(rows * sizeof(float));
         p.x = (bf16_t *)take(tokens * terms_of_x(dtype) * e->kbd * 256);
         p.h = (bf16_t *)take(rows * terms_of_h(dtype) * e->kbf * 256);
-        if (tokens > kFewTokens) p.p = (float *)take(rows * e->kbd * 512);
+        if (moe_wide_down(e, (int)tokens)) p.p = (float *)take(rows * e->kbd * 512);
     }
     if (plan) *plan = p;
     return at;
@@ -754,43 +830,60 @@ void launch_top(const dz_moe *e, int tokens, const MoePlan &plan, int *ids, floa
                        e->cfg.renormalize, ids, shares);
 }
 
-template <int XT, int HT>
-void launch_few(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+template <int MC, int XT, int HT, int NS>
+void launch_wide_gate(const dz_moe *e, int tokens, const MoePlan &plan, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
-    const int entries = std::min(tokens * c.top_k, c.experts);
-    // two workgroups a compute unit fit; each goes through its share of the tiles
-    const unsigned tiles = e->kbf * 8, share = std::max(1u, 2u * (unsigned)device_cus() / entries);
-    hipLaunchKernelGGL((moe_gate_up_kernel<XT, HT>), dim3(std::min(tiles, share), entries), dim3(kGateWaves * 64), 0, s,
-                       e->gate_up, e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.renormalize, c.ff,
-                       e->kbd, e->kbf, plan);
-    constexpr int WAVES = HT == 3 ? 8 : 16;  // a unit's rows of each wave fit LDS
-    hipLaunchKernelGGL((moe_down_kernel<HT, WAVES>), dim3(cdiv(c.hidden, 16)), dim3(WAVES * 64), 0, s, e->down,
-                       e->down_scales, tokens, c.experts, c.top_k, c.hidden, e->kbf, plan, y, dtype);
+    hipLaunchKernelGGL((moe_wide_kernel<MC, XT, HT, true, NS>), dim3(e->kbf, std::min(tokens * c.top_k, c.experts)),
+                       dim3(512), 0, s, e->gate_up, e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.ff,
+                       e->kbd, e->kbf * 128, plan.x, plan);
 }
 
-template <int MC, int XT, int HT, int NSX, int NSH>
-void launch_wide(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
+template <int MC, int HT, int NS>
+void launch_wide_down(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
-    const int entries = std::min(tokens * c.top_k, c.experts), width = e->kbd * 128;
-    hipLaunchKernelGGL((moe_wide_kernel<MC, XT, HT, true, NSX>), dim3(e->kbf, entries), dim3(512), 0, s, e->gate_up,
-                       e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.ff, e->kbd, e->kbf * 128, plan.x,
-                       plan);
-    hipLaunchKernelGGL((moe_wide_kernel<MC, HT, HT, false, NSH>), dim3(cdiv(c.hidden, 256), entries), dim3(512), 0, s,
-                       e->down, e->down_scales, nullptr, tokens, c.experts, c.top_k, c.hidden, e->kbf, width, plan.h,
-                       plan);
-    const int vec = c.hidden % 4 == 0 && ((uintptr_t)y & 15) == 0;
-    hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(c.hidden, 1024), tokens), dim3(256), 0, s, plan, c.top_k, c.hidden,
+    const int width = e->kbd * 128, vec = c.hidden % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    hipLaunchKernelGGL((moe_wide_kernel<MC, HT, HT, false, NS>),
+                       dim3(cdiv(c.hidden, 256), std::min(tokens * c.top_k, c.experts)), dim3(512), 0, s, e->down,
+                       e->down_scales, nullptr, tokens, c.experts, c.top_k, c.hidden, e->kbf, width, plan.h, plan);
+    hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(c.hidden, 256), tokens), dim3(64), 0, s, plan, c.top_k, c.hidden,
                        width, y, dtype, vec);
 }
 
-// Stages of 32 KiB of codes and 4 (terms of the rows) KiB, twice that for 32
-// rows at a time: as many as fit a compute unit's 160 KiB.
+// Which kernels. Measured (us; few / wide, the choice's and the sum's kernels not counted):
+//  gate and up, 8 of 64 experts of 2560x1024 in bf16: 1 token 11.6 / 16.4, 4 28.4 /
+//    27.1, 16 56 / 53; 2 of 16 of 1024x512 in f16, 8 tokens 7.6 / 10.2; 8 of 128 of
+//    2048x768 in f32, 16 tokens 90 / 61: the wide kernel past 16 tokens, where it
+//    needs a launch for the choice anyway, and for f32 on grids of two workgroups a
+//    compute unit, since few's waves load three terms of x for themselves;
+//  down: the same, 1 token 9.4 / 8.8 + 2.5 for the sum, 8 tokens 9.9 / 6.0 + 2.5,
+//    3 of 24 of 1000x700 in bf16, 13 tokens 18.4 / 7.8 + 2.5: the wide kernel from 16 slots on.
+// Stages of the wide kernel are 32 KiB of codes and 4 KiB a term of the rows,
+// twice that for 32 rows at a time: as many as fit a compute unit's 160 KiB.
 template <int XT, int HT>
 void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
-    if (tokens <= kFewTokens) return launch_few<XT, HT>(e, dtype, tokens, plan, y, s);
-    launch_top(e, tokens, plan, plan.ids, plan.shares, s);
-    if (tokens * e->cfg.top_k <= 12 * e->cfg.experts) launch_wide<1, XT, HT, XT == 1 ? 4 : 3, 3>(e, dtype, tokens, plan, y, s);
-    else launch_wide<2, XT, HT, XT == 3 ? 2 : 3, HT == 3 ? 2 : 3>(e, dtype, tokens, plan, y, s);
+    const dz_moe_config &c = e->cfg;
+    const int slots = tokens * c.top_k, entries = std::min(slots, c.experts);
+    const unsigned tiles = e->kbf * 8, cus = (unsigned)device_cus();
+    const bool many = slots > 12 * c.experts;  // rows an expert, on average
+    if (moe_wide_gate(e, tokens, XT)) {
+        launch_top(e, tokens, plan, plan.ids, plan.shares, s);
+        if (many) launch_wide_gate<2, XT, HT, XT == 3 ? 2 : 3>(e, tokens, plan, s);
+        else launch_wide_gate<1, XT, HT, XT == 1 ? 4 : 3>(e, tokens, plan, s);
+    } else {
+        // two workgroups a compute unit fit; each goes through its share of the tiles
+        const unsigned share = std::max(1u, 2u * cus / entries);
+        hipLaunchKernelGGL((moe_gate_up_kernel<XT, HT>), dim3(std::min(tiles, share), entries), dim3(kGateWaves * 64),
+                           0, s, e->gate_up, e->gate_scales, e->up_scales, tokens, c.experts, c.top_k, c.renormalize,
+                           c.ff, e->kbd, e->kbf, plan);
+    }
+    if (moe_wide_down(e, tokens)) {
+        if (many) launch_wide_down<2, HT, HT == 3 ? 2 : 3>(e, dtype, tokens, plan, y, s);
+        else launch_wide_down<1, HT, 3>(e, dtype, tokens, plan, y, s);
+    } else {
+        constexpr int WAVES = HT == 3 ? 8 : 16;  // a unit's rows of each wave fit LDS
+        hipLaunchKernelGGL((moe_down_kernel<HT, WAVES>), dim3(cdiv(c.hidden, 16)), dim3(WAVES * 64), 0, s, e->down,
+                           e->down_scales, tokens, c.experts, c.top_k, c.hidden, e->kbf, plan, y, dtype);
+    }
 }
 
 void moe_release(dz_moe *e) {

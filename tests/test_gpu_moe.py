@@ -81,7 +81,8 @@ def forward(ctx, layer, xd, dtype, tokens, hidden):
 CASES = [(1, 1, 1, 1, 1, 1), (1, 8, 2, 128, 128, 1), (1, 64, 8, 520, 200, 0), (2, 5, 5, 130, 17, 1),
          (7, 20, 3, 1000, 70, 0), (16, 4, 2, 256, 300, 1), (17, 3, 1, 200, 129, 0), (33, 6, 4, 384, 100, 1),
          (64, 16, 2, 260, 144, 1), (65, 2, 2, 129, 40, 0), (128, 9, 3, 300, 96, 1), (3, 130, 16, 64, 48, 1),
-         (5, 512, 4, 72, 16, 0)]
+         (5, 512, 4, 72, 16, 0), (16, 128, 8, 130, 2100, 1), (15, 40, 1, 300, 200, 0), (8, 2, 2, 1100, 257, 1),
+         (100, 300, 2, 140, 33, 0), (19, 30, 1, 257, 513, 1)]
 
 
 @pytest.mark.parametrize("dtype", [rocm.F32, rocm.F16, rocm.BF16])
