@@ -196,6 +196,72 @@ __global__ __launch_bounds__(kRowsWaves * 64) void fp8_rows_kernel(const uint8_t
     }
 }
 
+// The same for one row straight from x, sparing the launch that quantizes it:
+// each workgroup makes the codes it needs, a wave those of its own k-blocks, four
+// at a time and while their weights are on the way, 16 lanes a block as
+// fp8_quantize_kernel does, and hands them to its lanes as operands through LDS.
+// The same bits as fp8_rows_kernel on fp8_quantize_kernel's codes.
+template <class T, bool WIDE>
+__global__ __launch_bounds__(kRowsWaves * 64) void fp8_one_kernel(const uint8_t *__restrict__ codes,
+                                                                  const float *__restrict__ scales, int n, int kbs,
+                                                                  const T *__restrict__ x, int k, int vec,
+                                                                  void *__restrict__ y, int dtype) {
+    constexpr int NB = 4;  // k-blocks of a batch, one for each 16 lanes
+    __shared__ __align__(16) uint8_t s_codes[kRowsWaves][NB * 128];
+    __shared__ float s_scale[kRowsWaves][NB];
+    __shared__ float part[kRowsWaves][16];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int g = lane / 16, j = lane % 16, t = blockIdx.x;
+    const uint8_t *wbase = codes + (size_t)t * kbs * 2048 + lane * 16;
+    const float *swrow = scales + (size_t)(t / 8) * kbs;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int b0 = wave; b0 < kbs; b0 += kRowsWaves * NB) {
+        uint4_t w[NB][2];
+        float sw[NB];
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const int kb = min(b0 + i * kRowsWaves, kbs - 1);
+            w[i][0] = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048));
+            w[i][1] = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048 + 1024));
+            sw[i] = swrow[kb];
+        }
+        float v[8];
+        const int mine = b0 + g * kRowsWaves;
+        fp8_load8(x, mine < kbs ? mine * 128 + j * 8 : k, k, vec, v);
+        uint2_t c;
+        const float scale = fp8_quantize8(v, c);
+        *(uint2_t *)&s_codes[wave][g * 128 + j * 8] = c;
+        if (j == 0) s_scale[wave][g] = scale;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            if (b0 + i * kRowsWaves >= kbs) break;
+            uint4_t x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
+            float s = 0.0f;
+            if (j == 0) {
+                x0 = *(const uint4_t *)&s_codes[wave][i * 128 + 16 * g];
+                x1 = *(const uint4_t *)&s_codes[wave][i * 128 + 16 * g + 64];
+                s = s_scale[wave][i] * sw[i];
+            }
+            const float4_t d = WIDE ? fp8_mfma_wide(fp8_widen(w[i][0], w[i][1]), fp8_widen(x0, x1))
+                                    : fp8_mfma(w[i][0], w[i][1], x0, x1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(d[e], s, acc[e]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next batch is written
+    }
+    if (j == 0)
+#pragma unroll
+        for (int e = 0; e < 4; e++) part[wave][4 * g + e] = acc[e];
+    __syncthreads();
+    const int i = threadIdx.x, col = t * 16 + i;
+    if (i >= 16 || col >= n) return;
+    float sum = part[0][i];
+#pragma unroll
+    for (int u = 1; u < kRowsWaves; u++) sum += part[u][i];
+    fp8_store(y, dtype, col, sum);
+}
+
 template <int MB>
 void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
     const dim3 grid(cdiv(w.rows, 16) * cdiv(m, 16 * MB));
@@ -466,6 +532,24 @@ void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, i
                        dim3(512), 0, s, w.codes, w.scales, w.rows, w.kbs, q, sx, m, y, dtype);
 }
 
+// One row quantized by the product's own kernel, in each of its workgroups: up
+// to four of them a compute unit (us, against two launches: K=1024, N=1024 3.7 /
+// 4.4; K=N=4096 5.1 / 7.0; K=4096, N=14336 11.3 / 12.7; K=1024, N=32000 13.9 /
+// 8.9; two rows 5.8 / 7.1, 9.4 / 8.2 at K=2560, N=9216).
+bool fp8_one(const Fp8Weight &w, size_t m) { return m == 1 && cdiv(w.rows, 16) <= 4u * (unsigned)device_cus(); }
+
+template <class T>
+void launch_fp8_one(const Fp8Weight &w, const T *x, void *y, int dtype, hipStream_t s) {
+    const dim3 grid(cdiv(w.rows, 16)), block(kRowsWaves * 64);
+    const int vec = w.cols % 8 == 0 && ((uintptr_t)x & 15) == 0;
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL((fp8_one_kernel<T, true>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, x, w.cols,
+                           vec, y, dtype);
+    else
+        hipLaunchKernelGGL((fp8_one_kernel<T, false>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, x, w.cols,
+                           vec, y, dtype);
+}
+
 bool fp8_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }
 
 int32_t fp8_alloc(dz_ctx *ctx, size_t rows, size_t cols, dz_fp8_weight **out) {
@@ -620,6 +704,13 @@ int32_t fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x
     if (!fp8_dtype(x_dtype) || !fp8_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
     if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (m == 0) return DZ_OK;
+    if (fp8_one(w->w, m) && ctx_variant(ctx, "fp8") == 0) {
+        hipStream_t s = ctx_stream(ctx);
+        if (x_dtype == DZ_F32) launch_fp8_one(w->w, (const float *)x, y, y_dtype, s);
+        else if (x_dtype == DZ_F16) launch_fp8_one(w->w, (const half_t *)x, y, y_dtype, s);
+        else launch_fp8_one(w->w, (const bf16_t *)x, y, y_dtype, s);
+        return ctx_launched(ctx, "fp8 linear");
+    }
     const size_t qbytes = m * (size_t)w->w.kbs * 128, at = (qbytes + 255) / 256 * 256;
     void *work = nullptr;
     if (int32_t rc = ctx_workspace(ctx, at + m * (size_t)w->w.kbs * sizeof(float), &work)) return rc;

@@ -127,8 +127,27 @@ __device__ __forceinline__ float fp8_quantize8(const float v[8], uint2_t &codes)
     const bool finite = most < 0x7f800000u;
     const float s = fmaxf(__fdiv_rn(word_as_float(most), 448.0f), 1.17549435e-38f);
     float q[8];
+    if (s > 0x1p-60f) {
+        // v / s, correctly rounded, in half a division's instructions: q = v r with
+        // r = 1 / s to nearest, then twice q += r (v - q s), whose residual is exact
+        // (the first leaves q within an ulp, the second is Markstein's theorem, IBM
+        // J. Res. Dev. 34, 1990). Where a residual underflows q is below 2^-40 and
+        // its code 0 all the same.
+        const float r = __frcp_rn(s);
 #pragma unroll
-    for (int e = 0; e < 8; e++) q[e] = finite ? __fdiv_rn(v[e], s) : 0.0f;
+        for (int e = 0; e < 8; e++) {
+            float t = v[e] * r;
+            t = __builtin_fmaf(__builtin_fmaf(-t, s, v[e]), r, t);
+            q[e] = __builtin_fmaf(__builtin_fmaf(-t, s, v[e]), r, t);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = __fdiv_rn(v[e], s);
+    }
+    if (!finite) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) q[e] = 0.0f;
+    }
     int lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
     lo = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], lo, true);
     int hi = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], 0, false);

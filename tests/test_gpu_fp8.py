@@ -146,6 +146,29 @@ def test_quantize_at_the_ends_of_f32_and_with_values_that_are_not_finite(ctx):
     assert bits_equal(host(ctx, q), wq)
 
 
+def test_quantize_next_to_the_borders_of_codes(ctx):
+    """Quotients on, and an ulp or two to either side of, the middle between two codes, for scales of any
+    mantissa: a quotient that is not correctly rounded falls on the wrong side."""
+    import torch
+    rng = np.random.default_rng(17)
+    m, k = 4000, 128
+    most = (1 + rng.random(m)) * 2.0 ** rng.integers(-110, 110, m)
+    s = (most.astype(np.float32) / np.float32(448)).astype(np.float64)
+    middles = (VALUES[:126] + VALUES[1:127]) / 2
+    x = (rng.choice(middles, (m, k)) * s[:, None]).astype(np.float32)
+    for _ in range(2):
+        x = np.where(rng.random((m, k)) < 0.4, np.nextafter(x, np.float32(np.inf)), x)
+        x = np.where(rng.random((m, k)) < 0.4, np.nextafter(x, np.float32(0)), x)
+    x = np.minimum(x, most.astype(np.float32)[:, None])
+    x *= rng.choice([-1, 1], (m, k)).astype(np.float32)
+    x[np.arange(m), rng.integers(0, k, m)] = most.astype(np.float32)
+    q, sx = empty((m, 128), torch.uint8), empty((1, m), torch.float32)
+    ctx.fp8_quantize(dev(x), rocm.F32, m, k, q, sx)
+    wq, ws = quantize(x)
+    assert bits_equal(host(ctx, sx), ws)
+    assert bits_equal(host(ctx, q), wq)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (130, 300), (515, 129)])
 def test_weight_quantize_then_dequant(ctx, dtype, n, k):
@@ -168,7 +191,7 @@ def test_weight_quantize_then_dequant(ctx, dtype, n, k):
 
 
 # rows kernels, tiles and their edges; every pair of types once per shape class
-SHAPES = [(1, 1, 1), (1, 17, 128), (1, 4096, 1024), (2, 100, 257), (4, 300, 4096), (5, 33, 640), (16, 255, 1000),
+SHAPES = [(1, 1, 1), (1, 9000, 300), (1, 40, 9000), (1, 17000, 40), (2, 520, 5000), (1, 17, 128), (1, 4096, 1024), (2, 100, 257), (4, 300, 4096), (5, 33, 640), (16, 255, 1000),
           (17, 16, 384), (31, 1000, 129), (40, 520, 2560), (64, 129, 1111), (65, 128, 130), (130, 260, 300),
           (300, 512, 256), (513, 777, 645), (1030, 1300, 128)]
 
