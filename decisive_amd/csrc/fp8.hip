@@ -126,12 +126,12 @@ __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t *__restr
 // block of 128 values; a workgroup takes the same block of 16 rows, so that it
 // writes their scales side by side. Bound by memory: (sizeof(T) + 1) bytes per value.
 template <class T>
-__global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs, int vec,
+__global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
                                                            uint8_t *__restrict__ q, float *__restrict__ sx) {
     const int row = blockIdx.x * 16 + threadIdx.x / 16, kb = blockIdx.y, k0 = kb * 128 + threadIdx.x % 16 * 8;
     float v[8];
     const bool live = row < m;  // whole DPP rows of lanes
-    fp8_load8(x + (size_t)(live ? row : 0) * k, k0, k, vec, v);
+    fp8_load8(x + (size_t)(live ? row : 0) * k, k0, k, v);
     uint2_t codes;
     const float s = fp8_quantize8(v, codes);
     if (!live) return;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void fp8_rows_kernel(const uint8_t
 template <class T, bool WIDE>
 __global__ __launch_bounds__(kRowsWaves * 64) void fp8_one_kernel(const uint8_t *__restrict__ codes,
                                                                   const float *__restrict__ scales, int n, int kbs,
-                                                                  const T *__restrict__ x, int k, int vec,
+                                                                  const T *__restrict__ x, int k,
                                                                   void *__restrict__ y, int dtype) {
     constexpr int NB = 4;  // k-blocks of a batch, one for each 16 lanes
     __shared__ __align__(16) uint8_t s_codes[kRowsWaves][NB * 128];
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(kRowsWaves * 64) void fp8_one_kernel(const uint8_t 
         }
         float v[8];
         const int mine = b0 + g * kRowsWaves;
-        fp8_load8(x, mine < kbs ? mine * 128 + j * 8 : k, k, vec, v);
+        fp8_load8(x, mine < kbs ? mine * 128 + j * 8 : k, k, v);
         uint2_t c;
         const float scale = fp8_quantize8(v, c);
         *(uint2_t *)&s_codes[wave][g * 128 + j * 8] = c;
@@ -432,7 +432,6 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
 #pragma unroll
                 for (int b = 0; b < MT; b++) acc[a][b] += sums[(((h - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane];
     }
-    const bool vec = (n & 3) == 0 && ((uintptr_t)y & 15) == 0;
 #pragma unroll
     for (int b = 0; b < MT; b++) {
         const int row = row0 + wm * TM + b * 16 + j;
@@ -440,7 +439,7 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
 #pragma unroll
         for (int a = 0; a < NT; a++) {
             const int col = col0 + wn * TN + a * 16 + 4 * g;
-            if (col < n) fp8_store4(y, dtype, (size_t)row * n + col, acc[a][b], n - col, vec);
+            if (col < n) fp8_store4(y, dtype, (size_t)row * n + col, acc[a][b], n - col);
         }
     }
 }
@@ -459,14 +458,13 @@ void fp8_tile_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
 
 void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, float *sx, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
-    const int vec = k % 8 == 0 && ((uintptr_t)x & 15) == 0;
     const dim3 grid(cdiv(m, 16), kbs);
     if (dtype == DZ_F32)
-        hipLaunchKernelGGL(fp8_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, vec, q, sx);
+        hipLaunchKernelGGL(fp8_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, q, sx);
     else if (dtype == DZ_F16)
-        hipLaunchKernelGGL(fp8_quantize_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)x, m, k, kbs, vec, q, sx);
+        hipLaunchKernelGGL(fp8_quantize_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)x, m, k, kbs, q, sx);
     else
-        hipLaunchKernelGGL(fp8_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, vec, q, sx);
+        hipLaunchKernelGGL(fp8_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx);
 }
 
 // The tiles, in the order of the "fp8" family's variants from kTile0 on. Where a
@@ -541,13 +539,12 @@ bool fp8_one(const Fp8Weight &w, size_t m) { return m == 1 && cdiv(w.rows, 16) <
 template <class T>
 void launch_fp8_one(const Fp8Weight &w, const T *x, void *y, int dtype, hipStream_t s) {
     const dim3 grid(cdiv(w.rows, 16)), block(kRowsWaves * 64);
-    const int vec = w.cols % 8 == 0 && ((uintptr_t)x & 15) == 0;
     if (dtype == DZ_F32)
         hipLaunchKernelGGL((fp8_one_kernel<T, true>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, x, w.cols,
-                           vec, y, dtype);
+                           y, dtype);
     else
         hipLaunchKernelGGL((fp8_one_kernel<T, false>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, x, w.cols,
-                           vec, y, dtype);
+                           y, dtype);
 }
 
 bool fp8_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }

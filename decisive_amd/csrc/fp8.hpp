@@ -76,17 +76,22 @@ __device__ __forceinline__ float4_t fp8_mfma_wide(const Fp8Wide &a, const Fp8Wid
     return d;
 }
 
-// Eight consecutive values of a row from k0 on, as f32; past k zero. `vec`:
-// every such eight is one aligned load.
+// Vectors at any address their elements may have: rows of odd lengths start
+// anywhere, and the memory takes whole vectors there.
+typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned int uint4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned int uint2_any_t __attribute__((ext_vector_type(2), aligned(2)));
+
+// Eight consecutive values of a row from k0 on, as f32; past k zero.
 template <class T>
-__device__ __forceinline__ void fp8_load8(const T *__restrict__ row, int k0, int k, bool vec, float v[8]) {
-    if (vec && k0 + 8 <= k) {
+__device__ __forceinline__ void fp8_load8(const T *__restrict__ row, int k0, int k, float v[8]) {
+    if (k0 + 8 <= k) {
         if constexpr (sizeof(T) == 4) {
-            const float4_t a = *(const float4_t *)(row + k0), b = *(const float4_t *)(row + k0 + 4);
+            const float4_t a = *(const float4_any_t *)(row + k0), b = *(const float4_any_t *)(row + k0 + 4);
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
         } else {
-            const uint4_t w = *(const uint4_t *)(row + k0);
+            const uint4_t w = *(const uint4_any_t *)(row + k0);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 if constexpr (__is_same(T, half_t)) {
@@ -164,19 +169,19 @@ __device__ __forceinline__ void fp8_store(void *__restrict__ y, int dtype, size_
 }
 
 // Four consecutive outputs at element `at`, `left` of them inside the row.
-__device__ __forceinline__ void fp8_store4(void *__restrict__ y, int dtype, size_t at, float4_t v, int left, bool vec) {
-    if (!vec) {
+__device__ __forceinline__ void fp8_store4(void *__restrict__ y, int dtype, size_t at, float4_t v, int left) {
+    if (left < 4) {
 #pragma unroll
-        for (int e = 0; e < 4; e++)
+        for (int e = 0; e < 3; e++)
             if (e < left) fp8_store(y, dtype, at + e, v[e]);
     } else if (dtype == 0) {
-        *(float4_t *)((float *)y + at) = v;
+        *(float4_any_t *)((float *)y + at) = v;
     } else if (dtype == 1) {
         const half2_t a = {(half_t)v[0], (half_t)v[1]}, b = {(half_t)v[2], (half_t)v[3]};
-        *(uint2_t *)((half_t *)y + at) = uint2_t{half2_as_word(a), half2_as_word(b)};
+        *(uint2_any_t *)((half_t *)y + at) = uint2_t{half2_as_word(a), half2_as_word(b)};
     } else {
         const bf16x2_t a = {(bf16_t)v[0], (bf16_t)v[1]}, b = {(bf16_t)v[2], (bf16_t)v[3]};
-        *(uint2_t *)((bf16_t *)y + at) = uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+        *(uint2_any_t *)((bf16_t *)y + at) = uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
     }
 }
 

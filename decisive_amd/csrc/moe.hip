@@ -227,7 +227,7 @@ __device__ __forceinline__ void moe_top_any(const float *__restrict__ logits, in
 // throughout. Workgroups also write their share of x's bf16 terms.
 template <class T, int TERMS>
 __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x, const float *__restrict__ router,
-                                                         int tokens, int experts, int d, int kbd, int vec,
+                                                         int tokens, int experts, int d, int kbd,
                                                          MoePlan plan) {
     __shared__ float part[4][kRouteTokens];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x
         for (int i = 0; i < kRouteTokens; i++) {
             if (i >= mine) break;
             float v[8];
-            fp8_load8(x + (size_t)(first + i) * d, k0, d, vec, v);
+            fp8_load8(x + (size_t)(first + i) * d, k0, d, v);
 #pragma unroll
             for (int c = 0; c < 4; c++) {
                 acc[i] = __builtin_fmaf(r0[c], v[c], acc[i]);
@@ -263,7 +263,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x
     for (int u = blockIdx.x * 256 + threadIdx.x; u < units; u += gridDim.x * 256) {
         const int i = u / (dp / 8), k0 = u % (dp / 8) * 8;
         float v[8];
-        fp8_load8(x + (size_t)(first + i) * d, k0, d, vec, v);
+        fp8_load8(x + (size_t)(first + i) * d, k0, d, v);
         bf16x8_t out[TERMS];
 #pragma unroll
         for (int c = 0; c < 8; c++) {
@@ -743,7 +743,7 @@ __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict
 
 // y of a token: its slots' rows times their shares, in order, four loaded together.
 __global__ __launch_bounds__(64) void moe_combine_kernel(MoePlan plan, int top, int d, int width, void *__restrict__ y,
-                                                         int dtype, int vec) {
+                                                         int dtype) {
     const int t = blockIdx.y, c = (blockIdx.x * 64 + threadIdx.x) * 4;
     if (c >= d) return;
     const float *p = plan.p + (size_t)t * top * width + c, *shares = plan.shares + t * top;
@@ -763,7 +763,7 @@ __global__ __launch_bounds__(64) void moe_combine_kernel(MoePlan plan, int top, 
 #pragma unroll
                 for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(row[i][e], share[i], v[e]);
     }
-    fp8_store4(y, dtype, (size_t)t * d + c, v, d - c, vec);
+    fp8_store4(y, dtype, (size_t)t * d + c, v, d - c);
 }
 
 template <class T>
@@ -813,16 +813,15 @@ size_t moe_plan(const dz_moe *e, size_t tokens, int dtype, bool forward, uint8_t
 void launch_logits(const dz_moe *e, const void *x, int dtype, int tokens, const MoePlan &plan, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
     const dim3 grid(c.experts, cdiv(tokens, kRouteTokens));
-    const int vec = c.hidden % 8 == 0 && ((uintptr_t)x & 15) == 0;
     if (dtype == DZ_F32)
         hipLaunchKernelGGL((moe_logits_kernel<float, 3>), grid, dim3(256), 0, s, (const float *)x, e->router, tokens,
-                           c.experts, c.hidden, e->kbd, vec, plan);
+                           c.experts, c.hidden, e->kbd, plan);
     else if (dtype == DZ_F16)
         hipLaunchKernelGGL((moe_logits_kernel<half_t, 2>), grid, dim3(256), 0, s, (const half_t *)x, e->router, tokens,
-                           c.experts, c.hidden, e->kbd, vec, plan);
+                           c.experts, c.hidden, e->kbd, plan);
     else
         hipLaunchKernelGGL((moe_logits_kernel<bf16_t, 1>), grid, dim3(256), 0, s, (const bf16_t *)x, e->router, tokens,
-                           c.experts, c.hidden, e->kbd, vec, plan);
+                           c.experts, c.hidden, e->kbd, plan);
 }
 
 void launch_top(const dz_moe *e, int tokens, const MoePlan &plan, int *ids, float *shares, hipStream_t s) {
@@ -841,12 +840,12 @@ void launch_wide_gate(const dz_moe *e, int tokens, const MoePlan &plan, hipStrea
 template <int MC, int HT, int NS>
 void launch_wide_down(const dz_moe *e, int dtype, int tokens, const MoePlan &plan, void *y, hipStream_t s) {
     const dz_moe_config &c = e->cfg;
-    const int width = e->kbd * 128, vec = c.hidden % 4 == 0 && ((uintptr_t)y & 15) == 0;
+    const int width = e->kbd * 128;
     hipLaunchKernelGGL((moe_wide_kernel<MC, HT, HT, false, NS>),
                        dim3(cdiv(c.hidden, 256), std::min(tokens * c.top_k, c.experts)), dim3(512), 0, s, e->down,
                        e->down_scales, nullptr, tokens, c.experts, c.top_k, c.hidden, e->kbf, width, plan.h, plan);
     hipLaunchKernelGGL(moe_combine_kernel, dim3(cdiv(c.hidden, 256), tokens), dim3(64), 0, s, plan, c.top_k, c.hidden,
-                       width, y, dtype, vec);
+                       width, y, dtype);
 }
 
 // Which kernels. Measured (us; few / wide, the choice's and the sum's kernels not counted):
