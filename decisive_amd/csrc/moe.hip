@@ -61,7 +61,8 @@ namespace {
 
 constexpr int kMostExperts = 512, kMostTop = 16, kMostWidth = 65536;
 constexpr int kRouteTokens = 4;  // tokens a workgroup of the logits kernel takes together
-constexpr int kFewTokens = 16;   // tokens that the kernels for few take
+constexpr int kFewTokens = 16;   // tokens that moe_gate_up_kernel takes
+constexpr int kFewSlots = 16;    // moe_down_kernel takes fewer
 
 // What the kernels leave for the ones after, in the workspace.
 struct MoePlan {
@@ -442,73 +443,55 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
     }
 }
 
-// One workgroup: 16 columns of y. Units (chosen expert, 128-block of ff) in
-// order, an equal run of them to each wave; a wave adds its rows, times
-// their shares, into its own copy of the 16 columns in LDS, and the copies are
-// added in wave order. The rows are sorted
-// by expert in LDS first, with bit masks of each expert's tokens: one trip to
-// memory for the slots' experts, not one for each list.
+// One workgroup: 16 columns of y, for fewer than kFewSlots slots. Units (chosen
+// expert, 128-block of ff) in order, an equal run of them to each wave; a wave
+// adds its rows, times their shares, into its own copy of the 16 columns in LDS,
+// and the copies are added in wave order. Every wave first sorts the slots by
+// expert for itself, comparing each with all: no barrier, and one trip to memory.
 template <int HT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__restrict__ codes,
-                                                                   const float *__restrict__ ds, int tokens,
-                                                                   int experts, int top, int d, int kbf, MoePlan plan,
-                                                                   void *__restrict__ y, int dtype) {
-    constexpr int THREADS = WAVES * 64, kSlots = kFewTokens * kMostTop, kStage = 16 * HT * 256;  // one unit of 16 rows
-    static_assert(kSlots <= THREADS && kFewTokens <= 16, "a slot a thread, a bit a token");
+                                                              const float *__restrict__ ds, int tokens, int top, int d,
+                                                              int kbf, MoePlan plan, void *__restrict__ y, int dtype) {
+    constexpr int THREADS = WAVES * 64, kStage = 16 * HT * 256;  // one unit of 16 rows
+    static_assert(kFewTokens <= 16 && kFewSlots <= 16, "an expert's rows fit a tile");
     __shared__ __align__(16) uint8_t lds[WAVES * kStage];
     __shared__ __align__(16) float sums[WAVES * kFewTokens * 16];  // [waves][tokens][16]
-    __shared__ uint32_t s_mask[kMostExperts];  // the expert's tokens, its first row << 16
-    __shared__ int s_first[kSlots];            // per chosen expert: its first row << 8 | rows
-    __shared__ short s_expert[kSlots];
-    __shared__ int s_slot[kSlots];
-    __shared__ float s_share[kSlots];
-    __shared__ int s_active;
+    __shared__ __align__(16) int s_ids[WAVES][16];
+    __shared__ int s_slot[WAVES][16], s_first[WAVES][16], s_expert[WAVES][16];  // slots by expert; per expert
+    __shared__ float s_share[WAVES][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int g = lane / 16, j = lane % 16, t = blockIdx.x, tiles = (d + 15) / 16, slots = tokens * top;
     const size_t hp = (size_t)kbf * 128;
     float *mine = sums + (size_t)wave * tokens * 16;
-    const int my_slot = threadIdx.x, my_token = my_slot / top;
-    const int my_expert = my_slot < slots ? plan.ids[my_slot] : 0;
-    const float my_share = my_slot < slots ? plan.shares[my_slot] : 0.0f;
-    for (int i = threadIdx.x; i < experts; i += THREADS) s_mask[i] = 0;
+    const int my_expert = lane < slots ? plan.ids[lane] : kMostExperts;
+    const float my_share = lane < slots ? plan.shares[lane] : 0.0f;
     for (int i = lane; i < tokens * 4; i += 64) ((float4_t *)mine)[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-    __syncthreads();
-    if (my_slot < slots) atomicOr(&s_mask[my_expert], 1u << my_token);
-    __syncthreads();
-    if (wave == 0) {  // first rows, expert by expert: lane l has experts 8 l .. 8 l + 7
-        uint32_t sum = 0;  // chosen << 16 | rows
-        int count[8];
+    if (lane < 16) s_ids[wave][lane] = my_expert;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    int ids[16], rank = 0, before = 0, rows_of = 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            count[i] = lane * 8 + i < experts ? __popc(s_mask[lane * 8 + i]) : 0;
-            sum += count[i] ? 0x10000u + (uint32_t)count[i] : 0u;
-        }
-        uint32_t upto = sum;
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t before = (uint32_t)__shfl_up((int)upto, o);
-            if (lane >= o) upto += before;
-        }
-        uint32_t at = upto - sum;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if (count[i] == 0) continue;
-            s_mask[lane * 8 + i] |= at << 16;
-            s_first[at >> 16] = (int)(at & 0xffffu) << 8 | count[i];
-            s_expert[at >> 16] = (short)(lane * 8 + i);
-            at += 0x10000u + (uint32_t)count[i];
-        }
-        if (lane == 63) s_active = (int)(upto >> 16);
+    for (int i = 0; i < 16; i++) {
+        ids[i] = s_ids[wave][i];
+        rank += ids[i] < my_expert || (ids[i] == my_expert && i < lane);
+        before += ids[i] == my_expert && i < lane;
+        rows_of += ids[i] == my_expert;
     }
-    __syncthreads();
-    const int units = __builtin_amdgcn_readfirstlane(s_active) * kbf;
+    const bool leads = lane < slots && before == 0;  // its expert's first slot
+    const unsigned long long leaders = __ballot(leads);
+    int group = 0;
+#pragma unroll
+    for (int i = 0; i < 16; i++) group += (leaders >> i & 1) && ids[i] < my_expert;
+    if (lane < slots) {
+        s_slot[wave][rank] = lane;
+        s_share[wave][rank] = my_share;
+    }
+    if (leads) {
+        s_first[wave][group] = rank << 8 | rows_of;
+        s_expert[wave][group] = my_expert;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int units = __popcll(leaders) * kbf;
     const int u0 = (int)((int64_t)units * wave / WAVES), u1 = (int)((int64_t)units * (wave + 1) / WAVES);
-    if (my_slot < slots) {
-        const uint32_t m = s_mask[my_expert];
-        const int at = (int)(m >> 16) + __popc(m & 0xffffu & ((1u << my_token) - 1u));
-        s_slot[at] = my_slot;
-        s_share[at] = my_share;
-    }
-    __syncthreads();
     // A run of units of one expert at a time. h of a batch of units goes through
     // this wave's part of LDS: whole rows of it, loaded without registers and all
     // at once, while the operands in memory order would leave most lanes of a load
@@ -519,8 +502,8 @@ __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__r
     for (int u = u0; u < u1;) {
         const int a = u / kbf, k0 = u - a * kbf, k1 = min(kbf, k0 + u1 - u);
         u += k1 - k0;
-        const int expert = __builtin_amdgcn_readfirstlane((int)s_expert[a]);
-        const int group = __builtin_amdgcn_readfirstlane(s_first[a]), first = group >> 8, rows = group & 255;
+        const int expert = __builtin_amdgcn_readfirstlane(s_expert[wave][a]);
+        const int group = __builtin_amdgcn_readfirstlane(s_first[wave][a]), first = group >> 8, rows = group & 255;
         const uint8_t *w = codes + ((size_t)expert * tiles + t) * kbf * 2048 + lane * 16;
         const float *sw = ds + ((size_t)expert * ((d + 127) / 128) + t / 8) * kbf;
         // the batch: the most units, a power of two, whose rows fit the stage
@@ -533,7 +516,7 @@ __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__r
             for (int p0 = 0; p0 < pieces; p0 += 64) {
                 const int p = p0 + lane, rt = p >> (log_nb + 4), r = rt / HT, i = rt - r * HT;
                 const uint32_t at = p < pieces
-                                        ? (uint32_t)(((size_t)i * slots + s_slot[first + r]) * hp * 2 + kb0 * 256 +
+                                        ? (uint32_t)(((size_t)i * slots + s_slot[wave][first + r]) * hp * 2 + kb0 * 256 +
                                                      (p & ((16 << log_nb) - 1)) * 16)
                                         : 0x80000000u;
                 dma16_at(stage0 + p0 * 16, at, rh, 0u);
@@ -573,8 +556,8 @@ __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__r
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next batch lands
         }
         if (j < rows) {  // the run's rows into this wave's sums
-            float4_t *at = (float4_t *)(mine + s_slot[first + j] / top * 16 + 4 * g);
-            const float share = s_share[first + j];
+            float4_t *at = (float4_t *)(mine + s_slot[wave][first + j] / top * 16 + 4 * g);
+            const float share = s_share[wave][first + j];
             float4_t v = *at;
 #pragma unroll
             for (int e = 0; e < 4; e++) v[e] = __builtin_fmaf(acc[e], share, v[e]);
@@ -786,7 +769,7 @@ bool moe_wide_gate(const dz_moe *e, int tokens, int x_terms) {
     const size_t grid = (size_t)e->kbf * std::min(tokens * e->cfg.top_k, e->cfg.experts);
     return tokens > kFewTokens || (x_terms == 3 && grid >= 2 * (size_t)device_cus());
 }
-bool moe_wide_down(const dz_moe *e, int tokens) { return tokens > kFewTokens || tokens * e->cfg.top_k >= 16; }
+bool moe_wide_down(const dz_moe *e, int tokens) { return tokens * e->cfg.top_k >= kFewSlots; }
 
 // The workspace of a call: its size, and with `work` the plan's pointers into it.
 size_t moe_plan(const dz_moe *e, size_t tokens, int dtype, bool forward, uint8_t *work, MoePlan *plan) {
@@ -881,7 +864,7 @@ void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan,
     } else {
         constexpr int WAVES = HT == 3 ? 8 : 16;  // a unit's rows of each wave fit LDS
         hipLaunchKernelGGL((moe_down_kernel<HT, WAVES>), dim3(cdiv(c.hidden, 16)), dim3(WAVES * 64), 0, s, e->down,
-                           e->down_scales, tokens, c.experts, c.top_k, c.hidden, e->kbf, plan, y, dtype);
+                           e->down_scales, tokens, c.top_k, c.hidden, e->kbf, plan, y, dtype);
     }
 }
 

@@ -169,6 +169,26 @@ def test_a_token_that_is_not_finite_touches_no_other(ctx, dtype):
     layer.moe.free()
 
 
+@pytest.mark.parametrize("dtype", [rocm.F32, rocm.F16, rocm.BF16])
+def test_rows_at_odd_addresses_and_bytes_around_the_output_left_alone(ctx, dtype):
+    import torch
+    rng = np.random.default_rng(15)
+    hidden = 131
+    layer = Layer(ctx, rng, 6, 2, hidden, 77, 1)
+    for tokens in (1, 5, 13, 40):
+        xd, xf = rows_to(rng.standard_normal((tokens, hidden)).astype(np.float32), dtype)
+        room = torch.zeros(tokens * hidden + 1, dtype=xd.dtype, device="cuda")
+        room[1:] = xd.flatten()
+        out = torch.full((tokens * hidden + 9,), 7.0, dtype=xd.dtype, device="cuda")
+        torch.cuda.synchronize()
+        layer.moe.forward(room[1:], dtype, tokens, out[3:])
+        ctx.sync()
+        want, tol = layer(xf.astype(np.float64), dtype)
+        assert (np.abs(f64(out[3:3 + tokens * hidden].view(tokens, hidden)) - want) <= tol).all()
+        assert (out[:3] == 7).all() and (out[3 + tokens * hidden:] == 7).all()
+    layer.moe.free()
+
+
 def test_large_values_keep_their_range(ctx):
     """x near bf16's and f32's ends: the terms of an activation do not overflow."""
     rng = np.random.default_rng(13)
