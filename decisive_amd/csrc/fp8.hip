@@ -33,25 +33,32 @@ namespace {
 
 // ---- weights -------------------------------------------------------------------
 
-// One thread per 16-byte piece of the native layout.
-__global__ __launch_bounds__(256) void fp8_retile_kernel(const uint8_t *__restrict__ codes, int rows, int cols,
-                                                         int np, int kbs, uint8_t *__restrict__ dst,
-                                                         size_t tile_bytes, size_t kb_bytes, int *bad) {
-    // consecutive threads take consecutive pieces of a row: whole lines are read
-    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < (size_t)np * kbs * 8; id += gridDim.x * (size_t)256) {
-        const int piece = (int)(id % 8), kb = (int)(id / 8 % kbs), n = (int)(id / 8 / kbs);
-        const int h = piece / 4, g = piece % 4, k0 = kb * 128 + 16 * piece;
-        const uint8_t *src = codes + (size_t)n * cols + k0;
+// One thread per 16-byte piece of the native layout; consecutive threads take
+// consecutive pieces of a row, so that whole lines are read.
+__global__ __launch_bounds__(256) void fp8_retile_kernel(const uint8_t *__restrict__ codes, size_t pieces, int rows,
+                                                         int cols, int np, int kbs, uint8_t *__restrict__ dst,
+                                                         size_t matrix_bytes, size_t tile_bytes, size_t kb_bytes,
+                                                         int *bad) {
+    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < pieces; id += gridDim.x * (size_t)256) {
+        const int piece = (int)(id % 8), kb = (int)(id / 8 % kbs);
+        const size_t line = id / 8 / kbs;
+        const int n = (int)(line % np), h = piece / 4, g = piece % 4, k0 = kb * 128 + 16 * piece;
+        const size_t matrix = line / np;
+        const uint8_t *src = codes + (matrix * rows + n) * cols + k0;
         uint32_t w[4] = {0, 0, 0, 0};
-        bool nan = false;
-        for (int e = 0; e < 16; e++) {
-            const uint32_t c = n < rows && k0 + e < cols ? src[e] : 0u;
-            nan |= (c & 127u) == 127u;
-            w[e / 4] |= c << (8 * (e % 4));
+        if (n < rows && k0 + 16 <= cols) {
+            const uint4_t v = *(const uint4_bytes_t *)src;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = v[e];
+        } else if (n < rows) {
+            for (int e = 0; e < 16 && k0 + e < cols; e++) w[e / 4] |= (uint32_t)src[e] << (8 * (e % 4));
         }
+        bool nan = false;  // a byte whose low seven bits are all set
+#pragma unroll
+        for (int e = 0; e < 4; e++) nan |= (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0;
         if (nan) atomicOr(bad, 1);
-        *(uint4_t *)(dst + (size_t)(n / 16) * tile_bytes + (size_t)kb * kb_bytes + h * 1024 + (g * 16 + n % 16) * 16) =
-            uint4_t{w[0], w[1], w[2], w[3]};
+        *(uint4_t *)(dst + matrix * matrix_bytes + (size_t)(n / 16) * tile_bytes + (size_t)kb * kb_bytes + h * 1024 +
+                     (g * 16 + n % 16) * 16) = uint4_t{w[0], w[1], w[2], w[3]};
     }
 }
 
@@ -560,10 +567,9 @@ int32_t fp8_alloc(dz_ctx *ctx, size_t rows, size_t cols, dz_fp8_weight **out) {
     w.cols = (int)cols;
     w.np = (int)((rows + 15) / 16 * 16);
     w.kbs = (int)((cols + 127) / 128);
-    hipError_t e = hipMalloc(&w.codes, w.code_bytes());
-    if (e == hipSuccess) e = hipMalloc(&w.scales, w.scale_bytes());
+    const hipError_t e = hipMalloc(&w.codes, w.code_bytes() + w.scale_bytes());
+    w.scales = (float *)(w.codes + w.code_bytes());
     if (e != hipSuccess) {
-        if (w.codes) hipFree(w.codes);
         delete h;
         return ctx_hip_fail(ctx, e, "weight allocation");
     }
@@ -574,7 +580,6 @@ int32_t fp8_alloc(dz_ctx *ctx, size_t rows, size_t cols, dz_fp8_weight **out) {
 void fp8_release(dz_fp8_weight *h) {
     if (!h) return;
     hipFree(h->w.codes);
-    hipFree(h->w.scales);
     delete h;
 }
 
@@ -586,11 +591,12 @@ int32_t fp8_weight_ok(dz_ctx *ctx, const dz_fp8_weight *w) {
 
 }  // namespace
 
-void launch_fp8_retile(const uint8_t *codes, int rows, int cols, uint8_t *dst, size_t tile_bytes, size_t kb_bytes,
-                       int *bad, hipStream_t s) {
+void launch_fp8_retile(const uint8_t *codes, int count, int rows, int cols, uint8_t *dst, size_t matrix_bytes,
+                       size_t tile_bytes, size_t kb_bytes, int *bad, hipStream_t s) {
     const int np = (rows + 15) / 16 * 16, kbs = (cols + 127) / 128;
-    hipLaunchKernelGGL(fp8_retile_kernel, dim3(std::min(cdiv((size_t)np * kbs * 8, 256), 1u << 20)), dim3(256), 0, s, codes, rows, cols, np,
-                       kbs, dst, tile_bytes, kb_bytes, bad);
+    const size_t pieces = (size_t)count * np * kbs * 8;
+    hipLaunchKernelGGL(fp8_retile_kernel, dim3((unsigned)std::min((pieces + 255) / 256, (size_t)1 << 20)), dim3(256), 0,
+                       s, codes, pieces, rows, cols, np, kbs, dst, matrix_bytes, tile_bytes, kb_bytes, bad);
 }
 
 void launch_fp8_scales(const float *src, float *dst, size_t n, int *bad, hipStream_t s) {
@@ -608,7 +614,7 @@ int32_t fp8_weight_create(dz_ctx *ctx, const uint8_t *codes, const float *scales
     int *bad = ctx_flag(ctx), value = 0;
     hipStream_t s = ctx_stream(ctx);
     launch_fill_i32(bad, 0, 1, s);
-    launch_fp8_retile(codes, h->w.rows, h->w.cols, h->w.codes, (size_t)h->w.kbs * 2048, 2048, bad, s);
+    launch_fp8_retile(codes, 1, h->w.rows, h->w.cols, h->w.codes, 0, (size_t)h->w.kbs * 2048, 2048, bad, s);
     launch_fp8_scales(scales, h->w.scales, h->w.scale_bytes() / sizeof(float), bad, s);
     rc = ctx_flag_value(ctx, &value);
     if (!rc && value) rc = ctx_fail(ctx, DZ_INVALID_CHECKPOINT, "invalid 8-bit floating point weight");
@@ -666,7 +672,7 @@ int32_t fp8_weight_info(const dz_fp8_weight *w, size_t *rows, size_t *cols, size
 int32_t fp8_dequant(dz_ctx *ctx, const dz_fp8_weight *w, float *y) {
     if (int32_t rc = fp8_weight_ok(ctx, w)) return rc;
     if (!y) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
-    hipLaunchKernelGGL(fp8_dequant_kernel, dim3(std::min(cdiv((size_t)w->w.rows * w->w.cols, 256), 1u << 20)),
+    hipLaunchKernelGGL(fp8_dequant_kernel, dim3((unsigned)std::min(((size_t)w->w.rows * w->w.cols + 255) / 256, (size_t)1 << 20)),
                        dim3(256), 0, ctx_stream(ctx), w->w.codes, w->w.scales, w->w.rows, w->w.cols, w->w.kbs, y);
     return ctx_launched(ctx, "fp8 dequant");
 }

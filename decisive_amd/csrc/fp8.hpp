@@ -28,7 +28,7 @@ struct Fp8Weight {
     int rows = 0, cols = 0;
     int np = 0, kbs = 0;        // rows padded to 16, 128-wide blocks of cols
     uint8_t *codes = nullptr;   // device, tile16x128
-    float *scales = nullptr;    // device, [ceil(rows/128)][kbs]
+    float *scales = nullptr;    // device, [ceil(rows/128)][kbs], behind the codes in the same allocation
     size_t code_bytes() const { return (size_t)np * kbs * kFp8Block; }
     size_t scale_bytes() const { return (size_t)((rows + kFp8Block - 1) / kFp8Block) * kbs * sizeof(float); }
 };
@@ -81,6 +81,7 @@ __device__ __forceinline__ float4_t fp8_mfma_wide(const Fp8Wide &a, const Fp8Wid
 typedef float float4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 typedef unsigned int uint4_any_t __attribute__((ext_vector_type(4), aligned(2)));
 typedef unsigned int uint2_any_t __attribute__((ext_vector_type(2), aligned(2)));
+typedef unsigned int uint4_bytes_t __attribute__((ext_vector_type(4), aligned(1)));
 
 // Eight consecutive values of a row from k0 on, as f32; past k zero.
 template <class T>
@@ -188,10 +189,11 @@ __device__ __forceinline__ void fp8_store4(void *__restrict__ y, int dtype, size
 }  // namespace
 
 // ---- launchers (fp8.hip) -----------------------------------------------------
-// Row-major codes [rows x cols] into the native layout, tile t of the matrix at
-// dst + t * tile_bytes and k-block kb kb_bytes further; sets *bad on a NaN code.
-void launch_fp8_retile(const uint8_t *codes, int rows, int cols, uint8_t *dst, size_t tile_bytes, size_t kb_bytes,
-                       int *bad, hipStream_t s);
+// Row-major codes of `count` matrices [rows x cols] (one after the other) into the
+// native layout: matrix i at dst + i * matrix_bytes, its tile t tile_bytes and
+// k-block kb kb_bytes further; sets *bad on a NaN code.
+void launch_fp8_retile(const uint8_t *codes, int count, int rows, int cols, uint8_t *dst, size_t matrix_bytes,
+                       size_t tile_bytes, size_t kb_bytes, int *bad, hipStream_t s);
 // Copies block scales; sets *bad where one is not finite or is negative.
 void launch_fp8_scales(const float *src, float *dst, size_t n, int *bad, hipStream_t s);
 

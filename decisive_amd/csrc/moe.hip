@@ -43,6 +43,7 @@ struct dz_moe {
     float *up_scales = nullptr;
     float *down_scales = nullptr;   // [experts][hidden/128][kbf]
     float *router = nullptr;        // [experts][128 kbd], zero past hidden
+    uint8_t *memory = nullptr;      // all of these
     size_t bytes = 0;
 };
 
@@ -870,9 +871,7 @@ void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan,
 
 void moe_release(dz_moe *e) {
     if (!e) return;
-    for (void *p : {(void *)e->gate_up, (void *)e->down, (void *)e->gate_scales, (void *)e->up_scales,
-                    (void *)e->down_scales, (void *)e->router})
-        if (p) hipFree(p);
+    hipFree(e->memory);
     delete e;
 }
 
@@ -908,6 +907,7 @@ int32_t moe_create(dz_ctx *ctx, const dz_moe_config *cfg, const void *router, in
     e->kbd = (d + 127) / 128;
     e->kbf = (ff + 127) / 128;
     const size_t ftiles = (ff + 15) / 16, dtiles = (d + 15) / 16, blocks = (size_t)e->kbd * e->kbf;
+    // one allocation, each part at a multiple of 256 bytes
     struct {
         void **p;
         size_t bytes;
@@ -917,31 +917,29 @@ int32_t moe_create(dz_ctx *ctx, const dz_moe_config *cfg, const void *router, in
                  {(void **)&e->up_scales, E * blocks * sizeof(float)},
                  {(void **)&e->down_scales, E * blocks * sizeof(float)},
                  {(void **)&e->router, (size_t)E * e->kbd * 128 * sizeof(float)}};
+    for (auto &part : parts) e->bytes += aligned(part.bytes);
+    const hipError_t err = hipMalloc(&e->memory, e->bytes);
+    if (err != hipSuccess) {
+        delete e;
+        return ctx_hip_fail(ctx, err, "layer allocation");
+    }
+    size_t at = 0;
     for (auto &part : parts) {
-        const hipError_t err = hipMalloc(part.p, part.bytes);
-        if (err != hipSuccess) {
-            *part.p = nullptr;
-            moe_release(e);
-            return ctx_hip_fail(ctx, err, "layer allocation");
-        }
-        e->bytes += part.bytes;
+        *part.p = e->memory + at;
+        at += aligned(part.bytes);
     }
     int *bad = ctx_flag(ctx), value = 0;
     hipStream_t s = ctx_stream(ctx);
     launch_fill_i32(bad, 0, 1, s);
-    for (int i = 0; i < E; i++) {
-        const size_t src = (size_t)i * ff * d;
-        uint8_t *gu = e->gate_up + (size_t)i * ftiles * e->kbd * 4096;
-        launch_fp8_retile(gate + src, ff, d, gu, (size_t)e->kbd * 4096, 4096, bad, s);
-        launch_fp8_retile(up + src, ff, d, gu + 2048, (size_t)e->kbd * 4096, 4096, bad, s);
-        launch_fp8_retile(down + src, d, ff, e->down + (size_t)i * dtiles * e->kbf * 2048, (size_t)e->kbf * 2048, 2048,
-                          bad, s);
-    }
+    const size_t gu = ftiles * e->kbd * 4096, dn = dtiles * e->kbf * 2048;
+    launch_fp8_retile(gate, E, ff, d, e->gate_up, gu, (size_t)e->kbd * 4096, 4096, bad, s);
+    launch_fp8_retile(up, E, ff, d, e->gate_up + 2048, gu, (size_t)e->kbd * 4096, 4096, bad, s);
+    launch_fp8_retile(down, E, d, ff, e->down, dn, (size_t)e->kbf * 2048, 2048, bad, s);
     launch_fp8_scales(gate_scales, e->gate_scales, E * blocks, bad, s);
     launch_fp8_scales(up_scales, e->up_scales, E * blocks, bad, s);
     launch_fp8_scales(down_scales, e->down_scales, E * blocks, bad, s);
     const int dp = e->kbd * 128;
-    const dim3 grid(std::min(cdiv((size_t)E * dp, 256), 1u << 20));
+    const dim3 grid((unsigned)std::min(((size_t)E * dp + 255) / 256, (size_t)1 << 20));
     if (router_dtype == DZ_F32)
         hipLaunchKernelGGL(moe_router_kernel<float>, grid, dim3(256), 0, s, (const float *)router, E, d, dp, e->router, bad);
     else if (router_dtype == DZ_F16)
