@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__
 // four output columns.
 constexpr int kRowsWaves = 8;
 
-template <int MB, bool WIDE>
+template <int MB, bool WIDE, bool AHEAD>
 __global__ __launch_bounds__(kRowsWaves * 64) void fp8_rows_kernel(const uint8_t *__restrict__ codes,
                                                                    const float *__restrict__ scales, int n, int kbs,
                                                                    const uint8_t *__restrict__ q,
@@ -170,24 +170,54 @@ __global__ __launch_bounds__(kRowsWaves * 64) void fp8_rows_kernel(const uint8_t
     float4_t acc[MB];
 #pragma unroll
     for (int b = 0; b < MB; b++) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
-    for (int kb = wave; kb < kbs; kb += kRowsWaves) {
-        const uint4_t w0 = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048));
-        const uint4_t w1 = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048 + 1024));
-        const float sw = swrow[kb];
+    struct Block {
+        uint4_t w[2], x[MB][2];
+        float sw, sx[MB];
+    };
+    auto load = [&](int kb, Block &o) {
+        o.w[0] = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048));
+        o.w[1] = __builtin_nontemporal_load((const uint4_t *)(wbase + (size_t)kb * 2048 + 1024));
+        o.sw = swrow[kb];
 #pragma unroll
         for (int b = 0; b < MB; b++) {
             const int row = row0 + 16 * b + j;
-            uint4_t x0 = {0, 0, 0, 0}, x1 = {0, 0, 0, 0};
-            float s = 0.0f;
+            o.x[b][0] = o.x[b][1] = uint4_t{0, 0, 0, 0};
+            o.sx[b] = 0.0f;
             if (row < m) {
                 const uint8_t *xr = q + ((size_t)row * kbs + kb) * 128 + 16 * g;
-                x0 = *(const uint4_t *)xr;
-                x1 = *(const uint4_t *)(xr + 64);
-                s = sx[(size_t)kb * m + row] * sw;
+                o.x[b][0] = *(const uint4_t *)xr;
+                o.x[b][1] = *(const uint4_t *)(xr + 64);
+                o.sx[b] = sx[(size_t)kb * m + row];
             }
-            const float4_t d = WIDE ? fp8_mfma_wide(fp8_widen(w0, w1), fp8_widen(x0, x1)) : fp8_mfma(w0, w1, x0, x1);
+        }
+    };
+    auto add = [&](const Block &now) {
+#pragma unroll
+        for (int b = 0; b < MB; b++) {
+            const float4_t d = WIDE ? fp8_mfma_wide(fp8_widen(now.w[0], now.w[1]), fp8_widen(now.x[b][0], now.x[b][1]))
+                                    : fp8_mfma(now.w[0], now.w[1], now.x[b][0], now.x[b][1]);
+            const float s = now.sx[b] * now.sw;
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[b][e] = __builtin_fmaf(d[e], s, acc[b][e]);
+        }
+    };
+    if constexpr (AHEAD) {
+        Block two[2];
+        auto step = [&](int kb, const Block &now, Block &next) {
+            if (kb + kRowsWaves < kbs) load(kb + kRowsWaves, next);
+            __builtin_amdgcn_sched_barrier(0);
+            add(now);
+        };
+        if (wave < kbs) load(wave, two[0]);
+        for (int kb = wave; kb < kbs; kb += 2 * kRowsWaves) {
+            step(kb, two[0], two[1]);
+            if (kb + kRowsWaves < kbs) step(kb + kRowsWaves, two[1], two[0]);
+        }
+    } else {
+        for (int kb = wave; kb < kbs; kb += kRowsWaves) {
+            Block one;
+            load(kb, one);
+            add(one);
         }
     }
 #pragma unroll
@@ -269,15 +299,25 @@ __global__ __launch_bounds__(kRowsWaves * 64) void fp8_one_kernel(const uint8_t 
     fp8_store(y, dtype, col, sum);
 }
 
+// From three blocks a wave on, its loads run one block ahead (us, without / with:
+// 4 rows, K=9216, N=2560 8.2 / 7.2; 32 rows 13.1 / 11.2; 32 rows, K=N=4096 7.5 / 7.0;
+// below that the registers cost more waves than it gives: 20 rows, K=1024, N=32000,
+// f32 10.6 / 13.7).
+template <int MB, bool WIDE>
+void fp8_rows_form(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
+    const dim3 grid(cdiv(w.rows, 16) * cdiv(m, 16 * MB)), block(kRowsWaves * 64);
+    if (w.kbs > 3 * kRowsWaves)
+        hipLaunchKernelGGL((fp8_rows_kernel<MB, WIDE, true>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, q, sx,
+                           m, y, dtype);
+    else
+        hipLaunchKernelGGL((fp8_rows_kernel<MB, WIDE, false>), grid, block, 0, s, w.codes, w.scales, w.rows, w.kbs, q,
+                           sx, m, y, dtype);
+}
+
 template <int MB>
 void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
-    const dim3 grid(cdiv(w.rows, 16) * cdiv(m, 16 * MB));
-    if (dtype == DZ_F32)
-        hipLaunchKernelGGL((fp8_rows_kernel<MB, true>), grid, dim3(kRowsWaves * 64), 0, s, w.codes, w.scales, w.rows,
-                           w.kbs, q, sx, m, y, dtype);
-    else
-        hipLaunchKernelGGL((fp8_rows_kernel<MB, false>), grid, dim3(kRowsWaves * 64), 0, s, w.codes, w.scales, w.rows,
-                           w.kbs, q, sx, m, y, dtype);
+    if (dtype == DZ_F32) fp8_rows_form<MB, true>(w, q, sx, m, y, dtype, s);
+    else fp8_rows_form<MB, false>(w, q, sx, m, y, dtype, s);
 }
 
 // ---- products: tiles over many rows ----------------------------------------------
@@ -290,13 +330,15 @@ void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
 // rows meet distinct banks. NS - 1 steps' loads are in flight or in use. Each
 // block's dots come from a zero accumulator and are folded by sx * sw with one fma
 // per output, in the shadow of the next MFMAs. The groups' sums are added in group
-// order, through LDS.
+// order, through LDS. Where k is cut, workgroup b / tiles takes `per` of its blocks
+// and writes their sums as f32 for fp8_join_kernel.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS, bool WIDE>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const float *__restrict__ scales, int n, int kbs,
                                                                      const uint8_t *__restrict__ q,
                                                                      const float *__restrict__ sx, int m,
-                                                                     void *__restrict__ y, int dtype) {
+                                                                     void *__restrict__ y, int dtype, int tiles,
+                                                                     int per) {
     constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
     constexpr int XPW = BM / 8 / WAVES, WPW = BN / 8 / WAVES;  // 1 KiB loads per wave and stage
     constexpr int PB = XPW + WPW + 1;                          // and the row scales
@@ -313,7 +355,8 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
     const int wm = wave / WGN, wn = wave % WGN, g = lane / 16, j = lane % 16;
     const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
     int tm, tn;
-    xcd_tile(blockIdx.x, gridDim.x, tiles_m, tiles_n, tm, tn);
+    const int split = blockIdx.x / tiles, first = split * per, last = min(kbs, first + per);  // its blocks of k
+    xcd_tile(blockIdx.x - split * tiles, tiles, tiles_m, tiles_n, tm, tn);
     const int row0 = tm * BM, col0 = tn * BN, rows = min(BM, m - row0);
     const int kp = kbs * 128, tile0 = col0 / 16, tvalid = min(BN / 16, (n + 15) / 16 - tile0);
     const int32x4_t rx = buffer_rsrc(q + (size_t)row0 * kp, (uint32_t)(rows * kp));
@@ -336,8 +379,8 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
 
     // Blocks past the last one load nothing (every offset out of range, zeros in LDS), so that all waits go by count.
     auto load_stage = [&](int stage, int step) {
-        const int kb = step * KS + group;
-        const bool live = kb < kbs;
+        const int kb = first + step * KS + group;
+        const bool live = kb < last;
         const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u;
 #pragma unroll
         for (int p = 0; p < XPW; p++)
@@ -404,16 +447,16 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
         }
     };
 
-    const int steps = (kbs + KS - 1) / KS;
+    const int steps = (last - first + KS - 1) / KS;
 #pragma unroll
     for (int p = 0; p < NS - 1; p++) load_stage(p, p);
-    float scale = sw[min(group, kbs - 1)];
+    float scale = sw[min(first + group, last - 1)];
     int stage = 0;
     for (int i = 0; i < steps; i++) {
         // this wave's loads of step i are done once only the later steps' are left; then the barrier covers every wave
         asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
         load_stage(stage == 0 ? NS - 1 : stage - 1, i + NS - 1);  // the stage that the step before read
-        const float next = sw[min((i + 1) * KS + group, kbs - 1)];
+        const float next = sw[min(first + (i + 1) * KS + group, last - 1)];
         compute(stage, scale);
         scale = next;
         stage = stage + 1 == NS ? 0 : stage + 1;
@@ -446,22 +489,61 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
 #pragma unroll
         for (int a = 0; a < NT; a++) {
             const int col = col0 + wn * TN + a * 16 + 4 * g;
-            if (col < n) fp8_store4(y, dtype, (size_t)row * n + col, acc[a][b], n - col);
+            if (col < n) fp8_store4(y, dtype, ((size_t)split * m + row) * n + col, acc[a][b], n - col);
         }
     }
 }
 
-template <int BM, int BN, int WGM, int WGN, int KS, int NS>
-void fp8_tile_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, hipStream_t s) {
-    const dim3 grid(cdiv(m, BM) * cdiv(w.rows, BN)), block(WGM * WGN * KS * 64);
-    if (dtype == DZ_F32)
-        hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WGM, WGN, KS, NS, true>), grid, block, 0, s, w.codes, w.scales,
-                           w.rows, w.kbs, q, sx, m, y, dtype);
-    else
-        hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WGM, WGN, KS, NS, false>), grid, block, 0, s, w.codes, w.scales,
-                           w.rows, w.kbs, q, sx, m, y, dtype);
+// y from the sums of `splits` runs of blocks, [splits][count] f32, added in
+// their order; four loads of a thread are under way together.
+__global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__ part, int splits, size_t count,
+                                                       void *__restrict__ y, int dtype) {
+    const size_t at = (blockIdx.x * (size_t)256 + threadIdx.x) * 4;
+    if (at >= count) return;
+    const int left = (int)min(count - at, (size_t)4);
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < splits; i0 += 4) {
+        float4_t p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float *from = part + min(i0 + i, splits - 1) * count + at;
+            if (left == 4) p[i] = *(const float4_any_t *)from;
+            else p[i] = float4_t{from[0], left > 1 ? from[1] : 0.0f, left > 2 ? from[2] : 0.0f, 0.0f};
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (i0 + i < splits) v += p[i];
+    }
+    fp8_store4(y, dtype, at, v, left);
 }
 
+// What a product needs beside its operands: how its tile cuts k (`splits` runs of
+// blocks), and where the runs' sums go.
+struct Fp8Split {
+    int splits = 1;
+    float *part = nullptr;  // [splits][m][n]
+};
+
+template <int BM, int BN, int WGM, int WGN, int KS, int NS, bool WIDE>
+void fp8_tile_form(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, Fp8Split cut,
+                   hipStream_t s) {
+    const unsigned tiles = cdiv(m, BM) * cdiv(w.rows, BN);
+    const int per = (int)cdiv(w.kbs, cut.splits), splits = (int)cdiv(w.kbs, per);
+    hipLaunchKernelGGL((fp8_tile_kernel<BM, BN, WGM, WGN, KS, NS, WIDE>), dim3(tiles * splits),
+                       dim3(WGM * WGN * KS * 64), 0, s, w.codes, w.scales, w.rows, w.kbs, q, sx, m,
+                       splits > 1 ? cut.part : y, splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, per);
+    if (splits > 1) {
+        const size_t count = (size_t)m * w.rows;
+        hipLaunchKernelGGL(fp8_join_kernel, dim3(cdiv(count, 1024)), dim3(256), 0, s, cut.part, splits, count, y, dtype);
+    }
+}
+
+template <int BM, int BN, int WGM, int WGN, int KS, int NS>
+void fp8_tile_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype, Fp8Split cut,
+                     hipStream_t s) {
+    if (dtype == DZ_F32) fp8_tile_form<BM, BN, WGM, WGN, KS, NS, true>(w, q, sx, m, y, dtype, cut, s);
+    else fp8_tile_form<BM, BN, WGM, WGN, KS, NS, false>(w, q, sx, m, y, dtype, cut, s);
+}
 
 void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, float *sx, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
@@ -499,42 +581,69 @@ constexpr Fp8Tile kFp8Tiles[] = {{32, 32, 1, 3.0f, 0.13f, 0.165f}, {64, 32, 1, 2
                                  {128, 128, 1, 3.5f, 0.66f, 1.07f}, {256, 128, 1, 7.5f, 1.05f, 1.75f},
                                  {256, 256, 1, 8.0f, 1.95f, 1e9f}};
 constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 7;
+constexpr int kMostSplits = 16;
 
-int fp8_pick(int m, int n, int kbs, bool wide) {
-    if (m <= 32) return m <= 16 ? 1 : 2;
+struct Fp8Pick {
+    int variant, splits;
+};
+
+// A forced variant keeps its tile. Where a tile leaves units idle, k is cut into
+// runs of blocks that fill one round; their sums go through memory and another
+// launch, 2.5 us, 0.12 us a run (that kernel reads them in order) and 8 bytes a
+// value at some 4 TB/s. Measured (us, whole / cut, the tile of each): 229 rows, K=9216,
+// N=2560, f32 out 26.0 (64x64k4) / 23.3 (128x128, 6 runs), bf16 20.9 / 18.6; 600 rows,
+// f16 35.5 (64x64) / 32.2 (128x128, 2 runs); 128 rows, K=9000, N=500, f32 13.2 / 8.2
+// (32x32k4, 4 runs); 60 rows, K=9600, N=300 10.9 / 7.3 (8 runs). Not worth it for
+// 512 rows, K=4096, N=2560 (17.7 / 18.0) or 100 rows, K=4096, N=1024 (6.3 / 7.1).
+Fp8Pick fp8_pick(int variant, int m, int n, int kbs, bool wide) {
+    if (variant == 0 && m <= 32) variant = m <= 16 ? 1 : 2;
+    if (variant && variant < kTile0) return {variant, 1};
+    if (wide && variant == kTile0 + kTiles - 1) variant--;
     const size_t cus = (size_t)device_cus();
-    int best = 0;
+    Fp8Pick best{variant, 1};
     float least = 1e30f;
     for (int i = 0; i < kTiles; i++) {
+        if (variant && variant != kTile0 + i) continue;
         const Fp8Tile &t = kFp8Tiles[i];
-        const size_t blocks = (size_t)cdiv(m, t.bm) * cdiv(n, t.bn), round = cus * t.resident;
-        float c = wide ? t.wide_c : t.c;
-        if (t.resident > 1 && blocks > cus) c *= 1.45f;
-        const float us = (float)((blocks + round - 1) / round) * (t.f + (float)kbs * c);
-        if (us < least) least = us, best = i;
+        const size_t tiles = (size_t)cdiv(m, t.bm) * cdiv(n, t.bn), round = cus * t.resident;
+        for (int splits = 1; splits <= kMostSplits && splits <= kbs; splits++) {
+            const size_t blocks = tiles * splits;
+            if (splits > 1 && blocks > round) break;
+            float c = wide ? t.wide_c : t.c;
+            if (t.resident > 1 && blocks > cus) c *= 1.45f;
+            float us = (float)((blocks + round - 1) / round) * (t.f + (float)cdiv(kbs, splits) * c);
+            if (splits > 1) us += 2.5f + (float)splits * (0.12f + (float)m * (float)n * 2e-6f);
+            if (us < least) least = us, best = {kTile0 + i, splits};
+        }
     }
-    return kTile0 + best;
+    return best;
+}
+
+// f32 values that a product of m rows needs for its runs' sums.
+size_t fp8_parts(const Fp8Weight &w, size_t m, int dtype, int variant) {
+    const int splits = fp8_pick(variant, (int)m, w.rows, w.kbs, dtype == DZ_F32).splits;
+    return splits > 1 ? splits * m * w.rows : 0;
 }
 
 // The product of m > 0 rows of codes. Few rows stream the weight (up to 32 rows:
 // K=N=4096 7.6 us against 8.0 on 32x32 tiles, and N many times K far less).
 void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype,
-                        int variant, hipStream_t s) {
-    switch (variant ? variant : fp8_pick(m, w.rows, w.kbs, dtype == DZ_F32)) {
+                        int variant, float *part, hipStream_t s) {
+    const Fp8Pick pick = fp8_pick(variant, m, w.rows, w.kbs, dtype == DZ_F32);
+    const Fp8Split cut{pick.splits, part};
+    switch (pick.variant) {
         case 1: return fp8_rows_launch<1>(w, q, sx, m, y, dtype, s);
         case 2: return fp8_rows_launch<2>(w, q, sx, m, y, dtype, s);
-        case 3: return fp8_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, s);
-        case 4: return fp8_tile_launch<64, 32, 2, 2, 2, 4>(w, q, sx, m, y, dtype, s);
-        case 5: return fp8_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, s);
-        case 6: return fp8_tile_launch<64, 64, 2, 2, 1, 4>(w, q, sx, m, y, dtype, s);
-        case 7: return fp8_tile_launch<128, 128, 2, 4, 1, 3>(w, q, sx, m, y, dtype, s);
-        case 8: return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, s);
+        case 3: return fp8_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 4: return fp8_tile_launch<64, 32, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 5: return fp8_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 6: return fp8_tile_launch<64, 64, 2, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 7: return fp8_tile_launch<128, 128, 2, 4, 1, 3>(w, q, sx, m, y, dtype, cut, s);
+        case 8: return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, cut, s);
         default: break;
     }
-    // 256x256: its f32-accurate form would not fit the registers
-    if (dtype == DZ_F32) return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, s);
-    hipLaunchKernelGGL((fp8_tile_kernel<256, 256, 2, 4, 1, 2, false>), dim3(cdiv(m, 256) * cdiv(w.rows, 256)),
-                       dim3(512), 0, s, w.codes, w.scales, w.rows, w.kbs, q, sx, m, y, dtype);
+    // its f32-accurate form would not fit the registers: fp8_pick takes 256x128 instead
+    fp8_tile_form<256, 256, 2, 4, 1, 2, false>(w, q, sx, m, y, dtype, cut, s);
 }
 
 // One row quantized by the product's own kernel, in each of its workgroups: up
@@ -696,7 +805,12 @@ int32_t fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q, con
     if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (((uintptr_t)q & 15) != 0) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes must be 16-byte aligned");
     if (m == 0) return DZ_OK;
-    launch_fp8_product(w->w, q, s, (int)m, y, y_dtype, ctx_variant(ctx, "fp8"), ctx_stream(ctx));
+    const int variant = ctx_variant(ctx, "fp8");
+    const size_t parts = fp8_parts(w->w, m, y_dtype, variant);
+    void *work = nullptr;
+    if (parts)
+        if (int32_t rc = ctx_workspace(ctx, parts * sizeof(float), &work)) return rc;
+    launch_fp8_product(w->w, q, s, (int)m, y, y_dtype, variant, (float *)work, ctx_stream(ctx));
     return ctx_launched(ctx, "fp8 linear");
 }
 
@@ -707,20 +821,23 @@ int32_t fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x, int32_t x
     if (!fp8_dtype(x_dtype) || !fp8_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
     if (m > kFp8MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (m == 0) return DZ_OK;
-    if (fp8_one(w->w, m) && ctx_variant(ctx, "fp8") == 0) {
+    const int variant = ctx_variant(ctx, "fp8");
+    if (fp8_one(w->w, m) && variant == 0) {
         hipStream_t s = ctx_stream(ctx);
         if (x_dtype == DZ_F32) launch_fp8_one(w->w, (const float *)x, y, y_dtype, s);
         else if (x_dtype == DZ_F16) launch_fp8_one(w->w, (const half_t *)x, y, y_dtype, s);
         else launch_fp8_one(w->w, (const bf16_t *)x, y, y_dtype, s);
         return ctx_launched(ctx, "fp8 linear");
     }
-    const size_t qbytes = m * (size_t)w->w.kbs * 128, at = (qbytes + 255) / 256 * 256;
+    const size_t codes = (m * (size_t)w->w.kbs * 128 + 255) / 256 * 256;
+    const size_t scales = (m * (size_t)w->w.kbs * sizeof(float) + 255) / 256 * 256;
     void *work = nullptr;
-    if (int32_t rc = ctx_workspace(ctx, at + m * (size_t)w->w.kbs * sizeof(float), &work)) return rc;
+    if (int32_t rc = ctx_workspace(ctx, codes + scales + fp8_parts(w->w, m, y_dtype, variant) * sizeof(float), &work))
+        return rc;
     uint8_t *q = (uint8_t *)work;
-    float *sx = (float *)(q + at);
+    float *sx = (float *)(q + codes), *part = (float *)(q + codes + scales);
     launch_fp8_quantize(x, x_dtype, (int)m, w->w.cols, q, sx, ctx_stream(ctx));
-    launch_fp8_product(w->w, q, sx, (int)m, y, y_dtype, ctx_variant(ctx, "fp8"), ctx_stream(ctx));
+    launch_fp8_product(w->w, q, sx, (int)m, y, y_dtype, variant, part, ctx_stream(ctx));
     return ctx_launched(ctx, "fp8 linear");
 }
 

@@ -364,13 +364,15 @@ int32_t dz_fp8_quantize(dz_ctx *ctx, const void *x_dev, int32_t x_dtype, size_t 
  * acc = fma(dot, sx * sw, acc), and rounded once. f16 and bf16 outputs take the
  * dots from the matrix unit's 8-bit products, whose adder drops what is 2^-14
  * of a neighbouring product (1.5e-5 of a dot of normal values); f32 outputs
- * take them in f32's accuracy, at about half the rate. The order of a row's sum
+ * take them in f32's accuracy, at about half the rate. Where sx * sw or a sum
+ * leaves f32's range the output is infinite or NaN. The order of a row's sum
  * may depend on m. Uses the context workspace (run the call once before
- * capturing it). m may be 0, and is at most 2^24. */
+ * capturing it; one replay at a time). m may be 0, and is at most 2^24. */
 int32_t dz_fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x_dev, int32_t x_dtype, size_t m,
                       void *y_dev, int32_t y_dtype);
 /* dz_fp8_linear on activations already quantized (dz_fp8_quantize with
- * k = cols(w)): several weights can share one quantization. No workspace. */
+ * k = cols(w)): several weights can share one quantization. The same bits as
+ * dz_fp8_linear's, and the context workspace as there. */
 int32_t dz_fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q_dev, const float *s_dev, size_t m,
                          void *y_dev, int32_t y_dtype);
 

@@ -420,3 +420,98 @@ def test_captured_products_replayed(ctx):
     finally:
         ctx.set_stream(None)
     w.free()
+
+
+# Long sums with few tiles: k is cut into runs whose sums meet in a second launch. No more additions stand in a row
+# then (nb blocks in S runs: nb / S + S of them, at most nb + 1), so the same tolerances hold.
+LONG = [(24, 300, 9600), (33, 17, 4100), (60, 301, 9600), (128, 500, 9000), (229, 2560, 9216), (600, 515, 5000)]
+
+
+@pytest.mark.parametrize("m,n,k", LONG)
+def test_long_sums_with_few_tiles(ctx, m, n, k):
+    import torch
+    rng = np.random.default_rng(m + n + k)
+    codes, scales = make_weight(rng, n, k)
+    xd, xf = rows_to((0.1 * rng.standard_normal((m, k))).astype(np.float32), rocm.BF16)
+    q, s = quantize(xf)
+    want, mags = product(q, s, codes, scales, n, k)
+    assert np.abs(want).max() < 6e4
+    w = ctx.fp8_weight(dev(codes), dev(scales), n, k)
+    qd, sd = dev(q), dev(s)
+    guard = 64
+    for y_dtype in DTYPES:
+        whole = torch.full((m * n + 2 * guard,), 7.0, dtype=_torch(y_dtype), device="cuda")
+        y = whole[guard:guard + m * n].view(m, n)
+        other = empty((m, n), _torch(y_dtype))
+        torch.cuda.synchronize()
+        ctx.fp8_linear(w, xd, rocm.BF16, m, y, y_dtype)
+        ctx.fp8_linear_q8(w, qd, sd, m, other, y_dtype)
+        ctx.sync()
+        check(f64(y), want, mags, k, y_dtype)
+        assert torch.equal(y, other)
+        assert (whole[:guard] == 7).all() and (whole[guard + m * n:] == 7).all()
+    w.free()
+
+
+@pytest.mark.parametrize("variant", VARIANTS[2:])
+@pytest.mark.parametrize("m,n,k", [(70, 131, 2600), (300, 70, 1111)])
+def test_every_tile_on_long_sums(ctx, variant, m, n, k):
+    """A forced tile cuts k by the same rule, into short and uneven last runs here."""
+    rng = np.random.default_rng(m + n + k)
+    codes, scales = make_weight(rng, n, k)
+    q, s = quantize(rng.standard_normal((m, k)).astype(np.float32))
+    want, mags = product(q, s, codes, scales, n, k)
+    w = ctx.fp8_weight(dev(codes), dev(scales), n, k)
+    ctx.select_variant("fp8", variant)
+    try:
+        for y_dtype in DTYPES:
+            y = empty((m, n), _torch(y_dtype))
+            ctx.fp8_linear_q8(w, dev(q), dev(s), m, y, y_dtype)
+            ctx.sync()
+            check(f64(y), want, mags, k, y_dtype)
+    finally:
+        ctx.select_variant("fp8", "auto")
+    w.free()
+
+
+def test_captured_long_sums_replayed(ctx):
+    """Two products of one recording take the workspace in turn; every replay gives the eager bits."""
+    import torch
+    rng = np.random.default_rng(22)
+    m, n, k = 70, 260, 5000
+    codes, scales = make_weight(rng, n, k)
+    w = ctx.fp8_weight(dev(codes), dev(scales), n, k)
+    back = ctx.fp8_weight(dev(np.ascontiguousarray(codes[:, :n])), dev(np.ascontiguousarray(scales[:, :3])), n, n)
+    stream = torch.cuda.Stream()
+    ctx.set_stream(stream.cuda_stream)
+    try:
+        x, h, y = empty((m, k), torch.bfloat16), empty((m, n), torch.float32), empty((m, n), torch.bfloat16)
+        eager = torch.empty_like(y)
+        x.zero_()
+        torch.cuda.synchronize()
+
+        def run(out):
+            ctx.fp8_linear(w, x, rocm.BF16, m, h, rocm.F32)
+            ctx.fp8_linear(back, h, rocm.F32, m, out, rocm.BF16)
+
+        run(y)
+        ctx.sync()
+        graph = torch.cuda.CUDAGraph()
+        with rocm.capture(graph, stream):
+            run(y)
+            capture = ctx.capture_id()
+        for i in range(4):
+            x.copy_(torch.from_numpy(rng.standard_normal((m, k)).astype(np.float32)))
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                graph.replay()
+            torch.cuda.synchronize()
+            run(eager)
+            ctx.sync()
+            assert y.abs().max() > 0 and torch.equal(y, eager), i
+        del graph
+        ctx.capture_release(capture)
+    finally:
+        ctx.set_stream(None)
+    w.free()
+    back.free()
