@@ -131,7 +131,9 @@ __global__ __launch_bounds__(256) void fp8_dequant_kernel(const uint8_t *__restr
 
 // Codes [m x 128 kbs] and scales [kbs x m] of the rows of x. 16 lanes take a
 // block of 128 values; a workgroup takes the same block of 16 rows, so that it
-// writes their scales side by side. Bound by memory: (sizeof(T) + 1) bytes per value.
+// writes their scales side by side, and its neighbours go on along the rows (down the
+// rows instead: 8192 x 4096 bf16 20.1 us). Bound by memory, (sizeof(T) + 1) bytes a
+// value: 8192 x 4096 bf16 16.2 us, 6.2 TB/s; a few rows 1.8 us, a launch's time.
 template <class T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
                                                            uint8_t *__restrict__ q, float *__restrict__ sx) {
@@ -155,7 +157,9 @@ __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__
 // the k-blocks in turn (block b on wave b % 8), operands straight from memory,
 // and their f32 partials are added in wave order, from LDS. The matrix unit's
 // operands are swapped (weight first), so a lane holds one activation row and
-// four output columns.
+// four output columns. Bound by the weight's bytes: 16 rows, K=4096, N=14336 13.9 us,
+// 4.2 TB/s; K=1024, N=32000 in f32 8.7 us, 4.0 TB/s; smaller ones by one trip to memory
+// and the launch (K=N=4096 5.5 us).
 constexpr int kRowsWaves = 8;
 
 template <int MB, bool WIDE, bool AHEAD>
@@ -335,6 +339,11 @@ void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
 // per output, in the shadow of the next MFMAs. The groups' sums are added in group
 // order, through LDS. Where k is cut, workgroup b / tiles takes `per` of its blocks
 // and writes their sums as f32 for fp8_join_kernel.
+//
+// 256x256 (8192 rows, K=N=4096): 127 us, 2.16 PFLOP/s of the 3.39 that MFMAs and
+// fold alone reach from registers; 82 us of it are those, 78 the loads into LDS, 94
+// loads and LDS reads, which the two waves of a SIMD hide in part. Small tiles are
+// bound by their loads, about 60 bytes a nanosecond into each unit.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS, bool WIDE>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const float *__restrict__ scales, int n, int kbs,
@@ -784,8 +793,9 @@ int32_t fp8_weight_info(const dz_fp8_weight *w, size_t *rows, size_t *cols, size
 int32_t fp8_dequant(dz_ctx *ctx, const dz_fp8_weight *w, float *y) {
     if (int32_t rc = fp8_weight_ok(ctx, w)) return rc;
     if (!y) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
-    hipLaunchKernelGGL(fp8_dequant_kernel, dim3((unsigned)std::min(((size_t)w->w.rows * w->w.cols + 255) / 256, (size_t)1 << 20)),
-                       dim3(256), 0, ctx_stream(ctx), w->w.codes, w->w.scales, w->w.rows, w->w.cols, w->w.kbs, y);
+    const size_t blocks = ((size_t)w->w.rows * w->w.cols + 255) / 256;
+    hipLaunchKernelGGL(fp8_dequant_kernel, dim3((unsigned)std::min(blocks, (size_t)1 << 20)), dim3(256), 0,
+                       ctx_stream(ctx), w->w.codes, w->w.scales, w->w.rows, w->w.cols, w->w.kbs, y);
     return ctx_launched(ctx, "fp8 dequant");
 }
 

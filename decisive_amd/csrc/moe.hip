@@ -226,7 +226,8 @@ __device__ __forceinline__ void moe_top_any(const float *__restrict__ logits, in
 }
 
 // A workgroup takes one expert and four tokens: its waves share hidden, f32
-// throughout. Workgroups also write their share of x's bf16 terms.
+// throughout. Workgroups also write their share of x's bf16 terms. A launch and a
+// trip to memory: 64 experts of 2560, one token 2.2 us; 32 of 4096, 64 tokens in f32 7.1.
 template <class T, int TERMS>
 __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x, const float *__restrict__ router,
                                                          int tokens, int experts, int d, int kbd,
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(256) void moe_logits_kernel(const T *__restrict__ x
     }
 }
 
-// One wave per token.
+// One wave per token; a chain of dependent steps, 4.6 us for 64 tokens and 32 experts.
 __global__ __launch_bounds__(64) void moe_top_kernel(const float *__restrict__ logits, int experts, int top,
                                                      int renormalize, int *__restrict__ ids,
                                                      float *__restrict__ shares) {
@@ -328,12 +329,19 @@ __device__ __forceinline__ float4_t moe_dot(const MoeWide &w, const MoeWide &x, 
 
 constexpr int kGateWaves = 8;
 
+// Where a wave keeps columns 4 p .. 4 p + 3 of row r of a 16-column tile in LDS:
+// the pieces of four rows change places, so that 16 rows' vectors meet distinct
+// banks (13 tokens, 3 of 24 experts of 1000x700: a layer 26.8 us without, 26.3 with).
+__device__ __forceinline__ int moe_part_at(int r, int p) { return r * 16 + (p ^ (r >> 2 & 3)) * 4; }
+
 // One workgroup: tiles of 16 columns of ff (blockIdx.x, + gridDim.x, ...) of one
 // chosen expert, gate and up, for its rows (16 at most). The waves share hidden
 // (block b on wave b % 8); their partials are added in wave order. Codes are
 // loaded a block ahead, across tiles too. Columns past ff, up to a whole 128-block, are written as
 // zero. With fewer slots than experts blockIdx.y is the first slot that chose an
-// expert, else the expert.
+// expert, else the expert. One token, 8 of 64 experts of 2560x1024 in bf16: 11.4 us for
+// 42 MB, 3.7 TB/s, some 4 us of it the launch, the choice and the sum over the waves;
+// 8 tokens, 2 of 16 of 1024x512 6.8 us, nearly all of it those.
 template <int XT, int HT>
 __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
     const uint8_t *__restrict__ codes, const float *__restrict__ gs, const float *__restrict__ us, int tokens,
@@ -428,14 +436,15 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
             }
         }
         __syncthreads();
-        *(float4_t *)&part[wave][0][j * 16 + 4 * g] = acc[0];
-        *(float4_t *)&part[wave][1][j * 16 + 4 * g] = acc[1];
+        *(float4_t *)&part[wave][0][moe_part_at(j, g)] = acc[0];
+        *(float4_t *)&part[wave][1][moe_part_at(j, g)] = acc[1];
         __syncthreads();
         const int i = threadIdx.x, r = i / 16;
         if (i < 256 && r < rows) {
-            float gate = part[0][0][i], up = part[0][1][i];
+            const int at = moe_part_at(r, i / 4 % 4) + i % 4;
+            float gate = part[0][0][at], up = part[0][1][at];
 #pragma unroll
-            for (int v = 1; v < kGateWaves; v++) gate += part[v][0][i], up += part[v][1][i];
+            for (int v = 1; v < kGateWaves; v++) gate += part[v][0][at], up += part[v][1][at];
             bf16_t out[HT];
             moe_split<HT>(t < tiles ? gate / (1.0f + expf(-gate)) * up : 0.0f, out);
 #pragma unroll
@@ -448,7 +457,9 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
 // expert, 128-block of ff) in order, an equal run of them to each wave; a wave
 // adds its rows, times their shares, into its own copy of the 16 columns in LDS,
 // and the copies are added in wave order. Every wave first sorts the slots by
-// expert for itself, comparing each with all: no barrier, and one trip to memory.
+// expert for itself, comparing each with all: no barrier, and one trip to memory. One
+// token, 8 experts of 2560x1024: 8.6 us for 21 MB (2.4 TB/s): 160 workgroups, the
+// slots, h and the codes one after another.
 template <int HT, int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__restrict__ codes,
                                                               const float *__restrict__ ds, int tokens, int top, int d,
@@ -586,7 +597,9 @@ __global__ __launch_bounds__(WAVES * 64) void moe_down_kernel(const uint8_t *__r
 // each wave for itself instead, the rows cost more than the weight (x of eight
 // rows in f32 is three times a tile's codes). A row's 256 bytes of a term are 16
 // pieces, piece p of row r in slot p ^ (r & 15), so that 16 rows' reads meet
-// distinct banks. 16 MC rows at a time; more read the weight again.
+// distinct banks. 16 MC rows at a time; more read the weight again. Bound by the
+// codes' bytes: 64 tokens, 4 of 32 experts of 4096x1536 in f32 89 us for gate and up
+// (403 MB, 4.5 TB/s) and 43 for down (201 MB, 4.6 TB/s).
 template <int MC, int XT, int HT, bool GATE, int NS>
 __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict__ codes,
                                                        const float *__restrict__ s0, const float *__restrict__ s1,
@@ -725,7 +738,8 @@ __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict
     }
 }
 
-// y of a token: its slots' rows times their shares, in order, four loaded together.
+// y of a token: its slots' rows times their shares, in order, four loaded together
+// (2.1 us, a launch's time; 64 tokens of 4 x 4096 4.4).
 __global__ __launch_bounds__(64) void moe_combine_kernel(MoePlan plan, int top, int d, int width, void *__restrict__ y,
                                                          int dtype) {
     const int t = blockIdx.y, c = (blockIdx.x * 64 + threadIdx.x) * 4;
@@ -941,11 +955,14 @@ int32_t moe_create(dz_ctx *ctx, const dz_moe_config *cfg, const void *router, in
     const int dp = e->kbd * 128;
     const dim3 grid((unsigned)std::min(((size_t)E * dp + 255) / 256, (size_t)1 << 20));
     if (router_dtype == DZ_F32)
-        hipLaunchKernelGGL(moe_router_kernel<float>, grid, dim3(256), 0, s, (const float *)router, E, d, dp, e->router, bad);
+        hipLaunchKernelGGL(moe_router_kernel<float>, grid, dim3(256), 0, s, (const float *)router, E, d, dp, e->router,
+                           bad);
     else if (router_dtype == DZ_F16)
-        hipLaunchKernelGGL(moe_router_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)router, E, d, dp, e->router, bad);
+        hipLaunchKernelGGL(moe_router_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)router, E, d, dp, e->router,
+                           bad);
     else
-        hipLaunchKernelGGL(moe_router_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)router, E, d, dp, e->router, bad);
+        hipLaunchKernelGGL(moe_router_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)router, E, d, dp, e->router,
+                           bad);
     int32_t rc = ctx_flag_value(ctx, &value);
     if (!rc && value) rc = ctx_fail(ctx, DZ_INVALID_CHECKPOINT, "invalid mixture-of-experts weight");
     if (rc) {
