@@ -568,31 +568,37 @@ void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, flo
         hipLaunchKernelGGL(fp8_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx);
 }
 
-// The tiles, in the order of the "fp8" family's variants from kTile0 on. Where a
-// grid takes r rounds of the chip (`resident` blocks a compute unit), a product
-// takes about r (f + blocks-of-k c) us; the least is taken. f covers a block's
-// first loads and its stores; c, the time of one 128-block, is measured with 8-bit
-// and with f32-accurate dots (two blocks a unit: 64x64 takes c 1.45 times). A
-// smaller tile walks k faster and loads more for it: a unit loads about 60 bytes
-// a nanosecond into LDS whatever the tile, which bounds all but the largest.
-// Measured (us, f16 or bf16 out; 32x32k4 / 64x32k2 / 64x64k4 / 64x64 / 128x128 /
-// 256x128 / 256x256): 64 rows, K=N=4096 8.0 / 9.8 / 14.1 / 14.1 / 23.3 / - / -;
-// 128 rows, K=N=2560 9.0 / 6.9 / 7.5 / 9.4 / 16.4; 229 rows, K=9216, N=2560
-// 28.9 / 32.5 / 20.6 / 27.4 / 48.5; 308 rows, K=1024, N=4096 14.9 / 11.4 / 10.3 /
-// 7.0 / 9.1 / 13.7; 600 rows, K=N=4096 - / - / 30.4 / 27.9 / 24.4 / 37.8 / 57.7;
-// 1024 rows, K=2560, N=8192 - / - / 59.7 / 44.5 / 33.9 / 29.3 / 42.6; 4096 rows,
-// K=1024, N=4096 - / - / - / 45.3 / 35.0 / 30.3 / 25.4; 8192 rows, K=N=4096 194 /
-// 160 / 133 on the last three. f32 out: 229 rows 37.3 / 42.8 / 25.7 / 39.3 / 79;
-// 1024 rows - / - / 73 / 64 / 53 / 44.
+// The tiles, in the order of the "fp8" family's variants from kTile0 on. A grid
+// takes rounds of the chip (`resident` blocks a compute unit), each about f + blocks
+// of k * c us, and the least sum is taken. f covers a block's first loads and its
+// stores; c, the time of one 128-block, is measured with 8-bit and with f32-accurate
+// dots; `share` is what c grows by where two blocks share a unit. A smaller tile
+// walks k faster and loads more for it; a wave's larger part of a tile reads and, for
+// f32, converts less for each MFMA (64x64k2's waves have 32x64, 64x64's 32x32), and
+// needs deeper k to fill. Measured (us, 32x32k4 / 64x32k4 / 64x64k4 / 64x64 / 64x64k2 /
+// 128x128 / 256x128, f16 or bf16 out; long sums cut as below):
+//   64 rows, K=N=4096         8.0 / 9.8 / 11.4 / 10.2 / 11.4 / 14.6 / 15.9
+//   128 rows, K=N=4096        11.9 / 8.5 / 10.9 / 12.4 / 12.0 / 15.5 / 18.2
+//   40 rows, K=2560, N=9216   15.0 / 13.4 / 11.4 / 10.3 / 12.3 / 15.0 / 15.6
+//   366 rows, K=4096, N=2560  22.3 / 15.0 / 11.6 / 14.1 / 15.4 / 18.5 / 21.7
+//   308 rows, K=1024, N=4096  15.4 / 11.5 / 10.5 / 7.0 / 6.9 / 9.7 / 13.6
+//   512 rows, K=4096, N=2560  27.8 / 21.8 / 20.4 / 17.7 / 15.0 / 18.8 / 22.1
+//   600 rows, K=N=4096        53.8 / 35.6 / 31.2 / 28.4 / 25.8 / 23.2 / 29.4
+//   1024 rows, K=2560, N=8192 131 / 84 / 62 / 45 / 41.6 / 34.6 / 29.2
+//   229 rows, K=9216, N=2560  29.0 / 26.4 / 20.8 / 18.2 / 16.1 / 19.2 / 22.0; f32 out
+//                             37.8 / 34.6 / 26.0 / 24.0 / 21.8 / 22.8 / 27.1
+// 256x256: 8192 rows, K=N=4096 127 against 151 on 256x128; 4096 rows, K=1024 25.3, 28.8.
+// Over a hundred shapes drawn at random the choice is 1% slower than the best tile.
 struct Fp8Tile {
     int bm, bn, resident;
-    float f, c, wide_c;
+    float f, c, wide_c, share;
 };
-constexpr Fp8Tile kFp8Tiles[] = {{32, 32, 1, 3.0f, 0.13f, 0.165f}, {64, 32, 1, 2.5f, 0.215f, 0.28f},
-                                 {64, 64, 1, 3.0f, 0.265f, 0.345f}, {64, 64, 2, 3.0f, 0.36f, 0.53f},
-                                 {128, 128, 1, 3.5f, 0.66f, 1.07f}, {256, 128, 1, 7.5f, 1.05f, 1.75f},
-                                 {256, 256, 1, 8.0f, 1.95f, 1e9f}};
-constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 7;
+constexpr Fp8Tile kFp8Tiles[] = {
+    {32, 32, 1, 3.0f, 0.13f, 0.165f, 1.0f},   {64, 32, 1, 3.2f, 0.166f, 0.22f, 1.0f},
+    {64, 64, 1, 3.6f, 0.25f, 0.335f, 1.0f},   {64, 64, 2, 2.7f, 0.36f, 0.53f, 1.45f},
+    {64, 64, 2, 3.8f, 0.40f, 0.63f, 1.0f},    {128, 128, 1, 5.0f, 0.57f, 0.95f, 1.0f},
+    {256, 128, 1, 7.5f, 1.05f, 1.75f, 1.0f},  {256, 256, 1, 8.0f, 1.72f, 1e9f, 1.0f}};
+constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 8;
 constexpr int kMostSplits = 16;
 
 struct Fp8Pick {
@@ -601,12 +607,11 @@ struct Fp8Pick {
 
 // A forced variant keeps its tile. Where a tile leaves units idle, k is cut into
 // runs of blocks that fill one round; their sums go through memory and another
-// launch, 2.5 us, 0.12 us a run (that kernel reads them in order) and 8 bytes a
-// value at some 4 TB/s. Measured (us, whole / cut, the tile of each): 229 rows, K=9216,
-// N=2560, f32 out 26.0 (64x64k4) / 23.3 (128x128, 6 runs), bf16 20.9 / 18.6; 600 rows,
-// f16 35.5 (64x64) / 32.2 (128x128, 2 runs); 128 rows, K=9000, N=500, f32 13.2 / 8.2
-// (32x32k4, 4 runs); 60 rows, K=9600, N=300 10.9 / 7.3 (8 runs). Not worth it for
-// 512 rows, K=4096, N=2560 (17.7 / 18.0) or 100 rows, K=4096, N=1024 (6.3 / 7.1).
+// launch, 2.5 us, 0.12 us a run (that kernel reads them in order) and some time a
+// value. Measured (us, whole / cut, the best tile of each): 229 rows, K=9216, N=2560,
+// f32 out 26.0 (64x64k4) / 21.8 (64x64k2, 3 runs), bf16 20.8 / 16.1; 128 rows, K=9000,
+// N=500, f32 13.2 / 8.3 (32x32k4, 4 runs); 60 rows, K=9600, N=300 10.9 / 7.3 (8 runs).
+// Not worth it for 100 rows, K=4096, N=1024 (6.3 / 7.1).
 Fp8Pick fp8_pick(int variant, int m, int n, int kbs, bool wide) {
     if (variant == 0 && m <= 32) variant = m <= 16 ? 1 : 2;
     if (variant && variant < kTile0) return {variant, 1};
@@ -621,10 +626,11 @@ Fp8Pick fp8_pick(int variant, int m, int n, int kbs, bool wide) {
         for (int splits = 1; splits <= kMostSplits && splits <= kbs; splits++) {
             const size_t blocks = tiles * splits;
             if (splits > 1 && blocks > round) break;
-            float c = wide ? t.wide_c : t.c;
-            if (t.resident > 1 && blocks > cus) c *= 1.45f;
-            float us = (float)((blocks + round - 1) / round) * (t.f + (float)cdiv(kbs, splits) * c);
-            if (splits > 1) us += 2.5f + (float)splits * (0.12f + (float)m * (float)n * 2e-6f);
+            const float c = (float)cdiv(kbs, splits) * (wide ? t.wide_c : t.c);
+            const size_t full = blocks / round, rest = blocks % round;
+            float us = (float)full * (t.f + t.share * c);
+            if (rest) us += t.f + (rest > cus ? t.share : full && t.resident > 1 ? 0.67f * t.share : 1.0f) * c;
+            if (splits > 1) us += 2.5f + (float)splits * (0.12f + (float)m * (float)n * 1.2e-6f);
             if (us < least) least = us, best = {kTile0 + i, splits};
         }
     }
@@ -647,11 +653,12 @@ void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, i
         case 1: return fp8_rows_launch<1>(w, q, sx, m, y, dtype, s);
         case 2: return fp8_rows_launch<2>(w, q, sx, m, y, dtype, s);
         case 3: return fp8_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 4: return fp8_tile_launch<64, 32, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 4: return fp8_tile_launch<64, 32, 2, 1, 4, 3>(w, q, sx, m, y, dtype, cut, s);
         case 5: return fp8_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, cut, s);
         case 6: return fp8_tile_launch<64, 64, 2, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 7: return fp8_tile_launch<128, 128, 2, 4, 1, 3>(w, q, sx, m, y, dtype, cut, s);
-        case 8: return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, cut, s);
+        case 7: return fp8_tile_launch<64, 64, 2, 1, 2, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 8: return fp8_tile_launch<128, 128, 2, 2, 2, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 9: return fp8_tile_launch<256, 128, 4, 2, 1, 3>(w, q, sx, m, y, dtype, cut, s);
         default: break;
     }
     // its f32-accurate form would not fit the registers: fp8_pick takes 256x128 instead

@@ -2524,8 +2524,8 @@ const char *const kMlpNames[] = {"pipe-auto", "pipe256x64w8", "pipe128x64w4", "w
                                   "pipe64x64n4"};
 const char *const kDeltaNames[] = {"chunked64", "chunked64-c32", "recurrent", "recurrent-rolled", "auto"};
 const char *const kNormNames[] = {"fused", "separate"};
-const char *const kFp8Names[] = {"auto",  "rows16",  "rows32",  "32x32k4", "64x32k2",
-                                 "64x64k4", "64x64", "128x128", "256x128", "256x256"};
+const char *const kFp8Names[] = {"auto",  "rows16",  "rows32",  "32x32k4", "64x32k4",
+                                 "64x64k4", "64x64", "64x64k2", "128x128", "256x128", "256x256"};
 
 template <int W, int MPAD, bool G32, int NP>
 void gemv_launch_np(const Weight &w, const half_t *x, int m, float *y, hipStream_t s) {

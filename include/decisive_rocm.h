@@ -723,7 +723,7 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *                 share, or the norm then one quantization per product; the
  *                 same bits)
  *   "fp8"         auto, rows16, rows32 (the weight streamed over 16 or 32 rows at a
- *                 time), 32x32k4, 64x32k2, 64x64k4, 64x64, 128x128, 256x128, 256x256
+ *                 time), 32x32k4, 64x32k4, 64x64k4, 64x64, 64x64k2, 128x128, 256x128, 256x256
  *                 (tiles; k2 and k4 share the 128-blocks of k among two or four
  *                 groups of waves). For tests and benchmarks: "auto" picks by the
  *                 grid, dz_tune leaves it alone, and the variants add a row's blocks

@@ -243,7 +243,8 @@ def test_products_of_whole_numbers_lose_nothing(ctx, m, n, k, y_dtype):
     w.free()
 
 
-VARIANTS = ["rows16", "rows32", "32x32k4", "64x32k2", "64x64k4", "64x64", "128x128", "256x128", "256x256"]
+VARIANTS = ["rows16", "rows32", "32x32k4", "64x32k4", "64x64k4", "64x64", "64x64k2", "128x128", "256x128",
+            "256x256"]
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
