@@ -596,7 +596,7 @@ struct Fp8Tile {
 constexpr Fp8Tile kFp8Tiles[] = {
     {32, 32, 1, 3.0f, 0.13f, 0.165f, 1.0f},   {64, 32, 1, 3.2f, 0.166f, 0.22f, 1.0f},
     {64, 64, 1, 3.6f, 0.25f, 0.335f, 1.0f},   {64, 64, 2, 2.7f, 0.36f, 0.53f, 1.45f},
-    {64, 64, 2, 3.8f, 0.40f, 0.63f, 1.0f},    {128, 128, 1, 5.0f, 0.57f, 0.95f, 1.0f},
+    {64, 64, 2, 3.8f, 0.40f, 0.62f, 1.0f},    {128, 128, 1, 5.0f, 0.57f, 0.96f, 1.0f},
     {256, 128, 1, 7.5f, 1.05f, 1.75f, 1.0f},  {256, 256, 1, 8.0f, 1.72f, 1e9f, 1.0f}};
 constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 8;
 constexpr int kMostSplits = 16;
