@@ -644,7 +644,7 @@ size_t fp8_parts(const Fp8Weight &w, size_t m, int dtype, int variant) {
 }
 
 // The product of m > 0 rows of codes. Few rows stream the weight (up to 32 rows:
-// K=N=4096 7.6 us against 8.0 on 32x32 tiles, and N many times K far less).
+// K=N=4096 7.0 us against 8.0 on 32x32 tiles, and N many times K far less).
 void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, int m, void *y, int dtype,
                         int variant, float *part, hipStream_t s) {
     const Fp8Pick pick = fp8_pick(variant, m, w.rows, w.kbs, dtype == DZ_F32);
