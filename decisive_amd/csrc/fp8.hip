@@ -666,9 +666,10 @@ void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, i
 }
 
 // One row quantized by the product's own kernel, in each of its workgroups: up
-// to four of them a compute unit (us, against two launches: K=1024, N=1024 3.7 /
-// 4.4; K=N=4096 5.1 / 7.0; K=4096, N=14336 11.3 / 12.7; K=1024, N=32000 13.9 /
-// 8.9; two rows 5.8 / 7.1, 9.4 / 8.2 at K=2560, N=9216).
+// to four of them a compute unit (us, against two launches: K=N=1024 3.7 / 4.4;
+// K=N=4096 4.6 / 7.0; K=4096, N=14336 11.7 / 13.5; K=1024, N=32000 13.9 / 9.0). Two
+// rows so measured 6.1 / 7.0 at K=N=4096, but 5.1 / 4.5 at 1024 and 12.0 / 8.3 at K=2560,
+// N=9216.
 bool fp8_one(const Fp8Weight &w, size_t m) { return m == 1 && cdiv(w.rows, 16) <= 4u * (unsigned)device_cus(); }
 
 template <class T>
