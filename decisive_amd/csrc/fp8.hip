@@ -138,17 +138,15 @@ template <class T>
 __global__ __launch_bounds__(256) void fp8_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
                                                            uint8_t *__restrict__ q, float *__restrict__ sx) {
     const int kb = blockIdx.x, k0 = kb * 128 + threadIdx.x % 16 * 8;
-    for (int row0 = blockIdx.y * 16; row0 < m; row0 += gridDim.y * 16) {
-        const int row = row0 + threadIdx.x / 16;
-        float v[8];
-        const bool live = row < m;  // whole DPP rows of lanes
-        fp8_load8(x + (size_t)(live ? row : 0) * k, k0, k, v);
-        uint2_t codes;
-        const float s = fp8_quantize8(v, codes);
-        if (!live) return;
-        *(uint2_t *)(q + ((size_t)row * kbs + kb) * 128 + threadIdx.x % 16 * 8) = codes;
-        if (threadIdx.x % 16 == 0) sx[(size_t)kb * m + row] = s;
-    }
+    const int row = (blockIdx.z * gridDim.y + blockIdx.y) * 16 + threadIdx.x / 16;
+    float v[8];
+    const bool live = row < m;  // whole DPP rows of lanes
+    fp8_load8(x + (size_t)(live ? row : 0) * k, k0, k, v);
+    uint2_t codes;
+    const float s = fp8_quantize8(v, codes);
+    if (!live) return;
+    *(uint2_t *)(q + ((size_t)row * kbs + kb) * 128 + threadIdx.x % 16 * 8) = codes;
+    if (threadIdx.x % 16 == 0) sx[(size_t)kb * m + row] = s;
 }
 
 // ---- products: the weight streamed over a few rows -----------------------------
@@ -559,7 +557,8 @@ void fp8_tile_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
 
 void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, float *sx, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
-    const dim3 grid(kbs, std::min(cdiv(m, 16), 65535u));
+    const unsigned rows = cdiv(m, 16), most = 32768;  // a grid's y ends at 65535
+    const dim3 grid(kbs, std::min(rows, most), cdiv(rows, most));
     if (dtype == DZ_F32)
         hipLaunchKernelGGL(fp8_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, q, sx);
     else if (dtype == DZ_F16)
