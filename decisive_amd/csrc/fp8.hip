@@ -463,8 +463,9 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8
     float scale = sw[min(first + group, last - 1)];
     int stage = 0;
     for (int i = 0; i < steps; i++) {
-        // this wave's loads of step i are done once only the later steps' are left; then the barrier covers every wave
-        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
+        // This wave's loads of step i are done once only the later steps' are left, and its reads of the stage that the
+        // next loads overwrite at lgkmcnt(0); then the barrier covers every wave.
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
         load_stage(stage == 0 ? NS - 1 : stage - 1, i + NS - 1);  // the stage that the step before read
         const float next = sw[min(first + (i + 1) * KS + group, last - 1)];
         compute(stage, scale);

@@ -678,7 +678,8 @@ __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict
         float sc[2] = {sw[0][0], sw[1][0]};
         int stage = 0;
         for (int kb = 0; kb < kbs; kb++) {
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
+            // lgkmcnt: this wave's reads of the stage that the next loads overwrite are done too
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
             load_stage(stage == 0 ? NS - 1 : stage - 1, kb + NS - 1);  // the stage that the step before read
             const int after = min(kb + 1, kbs - 1);
             const float next[2] = {sw[0][after], sw[1][after]};
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(512) void moe_wide_kernel(const uint8_t *__restrict
             sc[1] = next[1];
             stage = stage + 1 == NS ? 0 : stage + 1;
         }
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");  // no LDS write in flight, every stage read
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");  // no LDS write in flight, every stage read
 #pragma unroll
         for (int c = 0; c < MC; c++) {
             const int r = r0 + 16 * c + j;
