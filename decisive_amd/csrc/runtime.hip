@@ -119,7 +119,10 @@ int32_t fail(dz_ctx *ctx, int32_t code, const std::string &msg) {
     return code;
 }
 
+// An error is reported once: the runtime keeps a thread's last error until it is
+// read, whatever succeeds in between, and the next call's launched() would find it.
 int32_t hip_fail(dz_ctx *ctx, hipError_t e, const char *what) {
+    (void)hipGetLastError();
     std::string msg = std::string(what) + ": " + hipGetErrorString(e);
     int32_t code = (e == hipErrorOutOfMemory || e == hipErrorMemoryAllocation) ? DZ_RESOURCE_LIMIT
                                                                                : DZ_INFERENCE_FAILED;
