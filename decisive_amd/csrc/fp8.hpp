@@ -135,16 +135,17 @@ __device__ __forceinline__ float fp8_quantize8(const float v[8], uint2_t &codes)
     float q[8];
     if (s > 0x1p-60f) {
         // v / s, correctly rounded, in half a division's instructions: q = v r with
-        // r = 1 / s to nearest, then twice q += r (v - q s), whose residual is exact
+        // r = 1 / s to nearest, then twice q -= r (q s - v), whose residual is exact
         // (the first leaves q within an ulp, the second is Markstein's theorem, IBM
         // J. Res. Dev. 34, 1990). Where a residual underflows q is below 2^-40 and
-        // its code 0 all the same.
+        // its code 0 all the same. With the residual this way round -0 stays -0: its
+        // residual is +0 and -0 - (+0) = -0, where -0 + (+0) would be +0.
         const float r = __frcp_rn(s);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             float t = v[e] * r;
-            t = __builtin_fmaf(__builtin_fmaf(-t, s, v[e]), r, t);
-            q[e] = __builtin_fmaf(__builtin_fmaf(-t, s, v[e]), r, t);
+            t = __builtin_fmaf(-__builtin_fmaf(t, s, -v[e]), r, t);
+            q[e] = __builtin_fmaf(-__builtin_fmaf(t, s, -v[e]), r, t);
         }
     } else {
 #pragma unroll
