@@ -411,9 +411,12 @@ int32_t dz_moe_route(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t 
  * rounded once at the end; the activations between the projections keep at
  * least 16 bits (24 for f32). A token's output does not depend on how a call
  * is repeated, but its bits may on the other tokens of the call. A token whose
- * logits are not all finite gives NaN outputs (and shares), the others are
- * not touched by it. Uses the context workspace (run the call once before
- * capturing it; one replay at a time). */
+ * logits are not all finite gives NaN outputs (and shares). Where the dot of
+ * 128 activations with their codes (before the block's scale; x and the
+ * activations between the projections up to 5.9e33 stay clear of it), a
+ * projection, or silu(gate_e x) * up_e x leaves f32's range, the token's
+ * outputs are infinite or NaN. Neither touches another token. Uses the context
+ * workspace (run the call once before capturing it; one replay at a time). */
 int32_t dz_moe_forward(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t dtype, size_t tokens, void *y_dev);
 
 /* ---- layer epilogues --------------------------------------------------------- */
