@@ -588,7 +588,9 @@ void launch_fp8_quantize(const void *x, int dtype, int m, int k, uint8_t *q, flo
 //   229 rows, K=9216, N=2560  29.0 / 26.4 / 20.8 / 18.2 / 16.1 / 19.2 / 22.0; f32 out
 //                             37.8 / 34.6 / 26.0 / 24.0 / 21.8 / 22.8 / 27.1
 // 256x256: 8192 rows, K=N=4096 127 against 151 on 256x128; 4096 rows, K=1024 25.3, 28.8.
-// Over a hundred shapes drawn at random the choice is 1% slower than the best tile.
+// Over 120 shapes drawn at random (33 to 3000 rows, K 100 to 9600, N 40 to 14400, every
+// type out) the choice is 0.7% slower than the best tile in the geometric mean, within
+// 3% on 112 of them and at most 21% (1506 rows, K=583, N=11248, f32 out 49.6 / 41.0).
 struct Fp8Tile {
     int bm, bn, resident;
     float f, c, wide_c, share;
@@ -596,7 +598,7 @@ struct Fp8Tile {
 constexpr Fp8Tile kFp8Tiles[] = {
     {32, 32, 1, 3.0f, 0.13f, 0.165f, 1.0f},   {64, 32, 1, 3.2f, 0.166f, 0.22f, 1.0f},
     {64, 64, 1, 3.6f, 0.25f, 0.335f, 1.0f},   {64, 64, 2, 2.7f, 0.36f, 0.53f, 1.45f},
-    {64, 64, 2, 3.8f, 0.40f, 0.62f, 1.0f},    {128, 128, 1, 5.0f, 0.57f, 0.96f, 1.0f},
+    {64, 64, 2, 3.8f, 0.40f, 0.63f, 1.0f},    {128, 128, 1, 5.0f, 0.57f, 0.95f, 1.0f},
     {256, 128, 1, 7.5f, 1.05f, 1.75f, 1.0f},  {256, 256, 1, 8.0f, 1.72f, 1e9f, 1.0f}};
 constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 8;
 constexpr int kMostSplits = 16;
