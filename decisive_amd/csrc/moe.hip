@@ -23,7 +23,7 @@
 // expert by expert and in order of tokens; no order depends on timing.
 // The products run on the bf16 matrix unit: e4m3 is exact in bf16, and an
 // activation is a sum of bf16 terms: x is one term (bf16), two (f16, exactly)
-// or three (f32, exactly); h, which never leaves the layer, is two terms (16
+// or three (f32, exactly down to bf16's smallest step, 2^-133); h, which never leaves the layer, is two terms (16
 // bits of it: 2^-16 off at most, against the 2^-9 or 2^-12 of the result's own
 // rounding) or three for f32. Sums are f32.
 #include <algorithm>

@@ -361,7 +361,8 @@ int32_t dz_fp8_quantize(dz_ctx *ctx, const void *x_dev, int32_t x_dtype, size_t 
 /* y = q(x) W^T: x_dev [m x cols(w)] of `x_dtype`, quantized as dz_fp8_quantize
  * does, y_dev [m x rows(w)] of `y_dtype` (each at any address its type
  * allows; y may not overlap x). The blocks' dots are folded in f32,
- * acc = fma(dot, sx * sw, acc), and rounded once. f16 and bf16 outputs take the
+ * acc = fma(dot, sx * sw, acc), and rounded once (sx * sw too is an f32: below
+ * 2^-126 it has steps of 2^-149). f16 and bf16 outputs take the
  * dots from the matrix unit's 8-bit products, whose adder drops what is 2^-14
  * of a neighbouring product (1.5e-5 of a dot of normal values); f32 outputs
  * take them in f32's accuracy, at about half the rate. Where sx * sw or a sum
@@ -409,7 +410,8 @@ int32_t dz_moe_route(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t 
 /* The layer: x_dev and y_dev [tokens x hidden] of `dtype` (y may not overlap
  * x), tokens 0..DZ_MOE_MAX_TOKENS (more: DZ_INPUT_TOO_LONG). Sums are f32 and
  * rounded once at the end; the activations between the projections keep at
- * least 16 bits (24 for f32). A token's output does not depend on how a call
+ * least 16 bits (24 for f32). Neither these nor x keep steps finer than 2^-133
+ * (so all of their bits from 2^-109 on). A token's output does not depend on how a call
  * is repeated, but its bits may on the other tokens of the call. A token whose
  * logits are not all finite gives NaN outputs (and shares). Where the dot of
  * 128 activations with their codes (before the block's scale; x and the

@@ -92,7 +92,7 @@ class Scaled(Layer):
         for name, (n, k) in dict(gate=(ff, hidden), up=(ff, hidden), down=(hidden, ff)).items():
             made = [make_weight(rng, n, k) for _ in range(experts)]
             codes = np.stack([c for c, _ in made])
-            s = (np.stack([s for _, s in made]) * (scales[name] / 0.006)).astype(np.float32)
+            s = (np.stack([s for _, s in made]).astype(np.float64) * (scales[name] / 0.006)).astype(np.float32)
             assert (s > 2.0 ** -126).all() and np.isfinite(s).all()
             self.wide[name] = [VALUES[c] * spread(b, *c.shape) for c, b in zip(codes, s)]
             held[name] = dev(codes), dev(s)
@@ -139,6 +139,49 @@ def test_h_up_to_the_documented_range(ctx, dtype, tokens):
     assert 1e-3 < np.abs(want).max() < 6e4
     assert (np.abs(f64(y) - want) <= tol).all()
     layer.moe.free()
+
+
+@pytest.mark.parametrize("tokens", [3, 20])
+@pytest.mark.parametrize("dtype", [rocm.F32, rocm.BF16])
+@pytest.mark.parametrize("exponent", [-109, -126, -132])
+def test_activations_down_to_the_documented_steps(ctx, exponent, dtype, tokens):
+    """x, then h, of 2^exponent to 2^(exponent + 1): off by half a step of 2^-133 more than other activations."""
+    rng = np.random.default_rng(90 + dtype)
+    hidden, ff, size = 300, 140, 2.0 ** exponent
+    x = rng.choice([-1.0, 1.0], (tokens, hidden)) * (1 + rng.random((tokens, hidden)))
+    xd, xf = rows_to((x * size).astype(np.float32), dtype)
+    scale = 1 / (size * 100 * np.sqrt(hidden))
+    layer = Scaled(ctx, rng, 4, 2, hidden, ff, gate=scale, up=scale, down=1e-3)
+    y = forward(ctx, layer, xd, dtype, tokens, hidden)
+    rows = xf.astype(np.float64)
+    want, tol = layer(rows, dtype)
+    assert 1e-3 < np.abs(want).max() < 6e4
+    assert (np.abs(f64(y) - want) <= tol + stepped(layer, rows, dtype, 2.0 ** -134)[0]).all()
+    layer.moe.free()
+
+    xd, xf = rows_to(x.astype(np.float32), dtype)
+    scale = np.sqrt(size) / (100 * np.sqrt(hidden))
+    layer = Scaled(ctx, rng, 4, 2, hidden, ff, gate=scale, up=scale, down=1e-3 / size)
+    y = forward(ctx, layer, xd, dtype, tokens, hidden)
+    rows = xf.astype(np.float64)
+    want, tol = layer(rows, dtype)
+    assert 1e-3 < np.abs(want).max() < 6e4
+    assert (np.abs(f64(y) - want) <= tol + stepped(layer, rows, dtype, 2.0 ** -134)[1]).all()
+    layer.moe.free()
+
+
+def stepped(layer, x, dtype, off):
+    """What y may move by where each value of x, or of h, is `off`: silu(a') b' - silu(a) b is at most
+    1.1 |a' - a| |b'| + |a| |b' - b|, since silu's slope is below 1.1; and 1% for the roundings of what moved."""
+    ids, c, _ = layer.route(x)
+    of_x, of_h = np.zeros(x.shape), np.zeros(x.shape)
+    for t in range(x.shape[0]):
+        for e, share in zip(ids[t], c[t]):
+            g, u, d = (layer.wide[p][e] for p in ("gate", "up", "down"))
+            a, b, da, db = g @ x[t], u @ x[t], np.abs(g).sum(1) * off, np.abs(u).sum(1) * off
+            of_x[t] += share * (np.abs(d) @ (1.1 * da * (np.abs(b) + db) + np.abs(a) * db))
+            of_h[t] += share * np.abs(d).sum(1) * off
+    return 1.01 * of_x, 1.01 * of_h
 
 
 @pytest.mark.parametrize("tokens", [3, 20])
