@@ -730,7 +730,7 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *   "fp8"         auto, rows16, rows32 (the weight streamed over 16 or 32 rows at a
  *                 time), 32x32k4, 64x32k4, 64x64k4, 64x64, 64x64k2, 128x128, 256x128, 256x256
  *                 (tiles; k2 and k4 share the 128-blocks of k among two or four
- *                 groups of waves). For tests and benchmarks: "auto" picks by the
+ *                 groups of waves; f32 outputs of 256x256 take 256x128). For tests and benchmarks: "auto" picks by the
  *                 grid, dz_tune leaves it alone, and the variants add a row's blocks
  *                 in orders of their own, so their f32 sums agree to rounding */
 int32_t dz_select_variant(dz_ctx *ctx, const char *family, const char *variant);
