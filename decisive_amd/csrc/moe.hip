@@ -855,6 +855,13 @@ void launch_wide_down(const dz_moe *e, int dtype, int tokens, const MoePlan &pla
 //    compute unit, since few's waves load three terms of x for themselves;
 //  down: the same, 1 token 9.4 / 8.8 + 2.5 for the sum, 8 tokens 9.9 / 6.0 + 2.5,
 //    3 of 24 of 1000x700 in bf16, 13 tokens 18.4 / 7.8 + 2.5: the wide kernel from 16 slots on.
+//  32 rows of an expert at a time (MC = 2) where experts have more than 12 on average,
+//    since past 16 rows the 16-row form reads their weight again (us a layer, 16 / 32
+//    rows at a time): 4 of 32 of 4096x1536, 8 rows on average bf16 135.6 / 137.0, f32
+//    145.2 / 159.3; 12 rows 169.4 / 144.0, 187.0 / 166.9; 16 rows 189.7 / 149.1, 208.4 /
+//    169.5. 2 of 8 of the same, 10 rows 52.3 / 51.6, f32 62.3 / 71.5; 14 rows 76.0 / 58.5,
+//    103.4 / 76.7; 32 rows 110.4 / 87.9, 150.2 / 119.4. Below the line the larger stages
+//    leave fewer of them (f32 keeps two of three), above it a reading is saved.
 // Stages of the wide kernel are 32 KiB of codes and 4 KiB a term of the rows,
 // twice that for 32 rows at a time: as many as fit a compute unit's 160 KiB.
 template <int XT, int HT>
