@@ -338,10 +338,10 @@ void fp8_rows_launch(const Fp8Weight &w, const uint8_t *q, const float *sx, int 
 // order, through LDS. Where k is cut, workgroup b / tiles takes `per` of its blocks
 // and writes their sums as f32 for fp8_join_kernel.
 //
-// 256x256 (8192 rows, K=N=4096): 127 us, 2.16 PFLOP/s of the 3.39 that MFMAs and
-// fold alone reach from registers; 82 us of it are those, 78 the loads into LDS, 94
-// loads and LDS reads, which the two waves of a SIMD hide in part. Small tiles are
-// bound by their loads, about 60 bytes a nanosecond into each unit.
+// 256x256 (8192 rows, K=N=4096): 127 to 140 us by the card, at 127 2.16 PFLOP/s of the
+// 3.39 that MFMAs and fold alone reach from registers; 82 us of it are those, 78 the
+// loads into LDS, 94 loads and LDS reads, which the two waves of a SIMD hide in part.
+// Small tiles are bound by their loads, about 60 bytes a nanosecond into each unit.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS, bool WIDE>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void fp8_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const float *__restrict__ scales, int n, int kbs,
@@ -669,7 +669,7 @@ void launch_fp8_product(const Fp8Weight &w, const uint8_t *q, const float *sx, i
 
 // One row quantized by the product's own kernel, in each of its workgroups: up
 // to four of them a compute unit (us, against two launches: K=N=1024 3.7 / 4.4;
-// K=N=4096 4.6 / 7.0; K=4096, N=14336 11.7 / 13.5; K=1024, N=32000 13.9 / 9.0). Two
+// K=N=4096 4.6 / 7.0 (5.0 on another card); K=4096, N=14336 11.7 / 13.5; K=1024, N=32000 13.9 / 9.0). Two
 // rows so measured 6.1 / 7.0 at K=N=4096, but 5.1 / 4.5 at 1024 and 12.0 / 8.3 at K=2560,
 // N=9216.
 bool fp8_one(const Fp8Weight &w, size_t m) { return m == 1 && cdiv(w.rows, 16) <= 4u * (unsigned)device_cus(); }
