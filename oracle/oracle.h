@@ -1,7 +1,7 @@
 /*
  * oracle.h -- CPU restatement of decisive's quantized matrix-product path.
  *
- * TEST INFRASTRUCTURE ONLY. This library is the checker for the HIP kernels in
+ * TEST INFRASTRUCTURE ONLY. This library is the oracle of the HIP kernels in
  * decisive_amd/csrc: only tests/, __graft_entry__.smoke() and bench.py's
  * cpu_baseline leg may load it. The product never links or calls it.
  *

@@ -1,7 +1,7 @@
 """numpy front end for the C oracle (liboracle.so).
 
 TEST INFRASTRUCTURE ONLY: tests/, __graft_entry__.smoke() and bench.py's
-cpu_baseline leg use this module as the checker. The product package
+cpu_baseline leg use this module as the oracle. The product package
 (decisive_amd) never imports it.
 
 Every wrapper names the function of oracle.c it calls; oracle.c cites the
