@@ -67,7 +67,7 @@ constexpr int kFewSlots = 16;    // moe_down_kernel takes fewer
 
 // What the kernels leave for the ones after, in the workspace.
 struct MoePlan {
-    float *logits;  // [tokens][experts]
+    float *logits;  // [tokens][experts]; null where the choice is given and ids and shares are there already
     int *ids;       // [slots] experts
     float *shares;  // [slots]
     bf16_t *x;      // [terms][tokens][128 kbd]
@@ -294,6 +294,52 @@ __global__ __launch_bounds__(64) void moe_top_kernel(const float *__restrict__ l
     }
 }
 
+// A choice that the caller made, and x as bf16 terms: what the logits kernel and the
+// choice leave for the rest. The first workgroup checks the choice: a token with an
+// expert out of range, or the same one twice, gets experts that are neither and NaN
+// shares, so that the kernels after may trust the ids (an expert's rows are at most
+// the tokens). A launch's time.
+template <class T, int TERMS>
+__global__ __launch_bounds__(256) void moe_take_kernel(const T *__restrict__ x, const int *__restrict__ ids,
+                                                       const float *__restrict__ shares, int tokens, int experts,
+                                                       int top, int d, int kbd, MoePlan plan) {
+    __shared__ int s_ids[DZ_MOE_MAX_TOKENS * kMostTop], s_bad[DZ_MOE_MAX_TOKENS];
+    const int dp = kbd * 128, slots = tokens * top;
+    if (blockIdx.x == 0) {
+        for (int s = threadIdx.x; s < slots; s += 256) s_ids[s] = ids[s];
+        for (int t = threadIdx.x; t < tokens; t += 256) s_bad[t] = 0;
+        __syncthreads();
+        for (int s = threadIdx.x; s < slots; s += 256) {
+            const int t = s / top, e = s_ids[s];
+            bool bad = e < 0 || e >= experts;
+            for (int o = t * top; o < s; o++) bad |= s_ids[o] == e;
+            if (bad) s_bad[t] = 1;
+        }
+        __syncthreads();
+        for (int s = threadIdx.x; s < slots; s += 256) {
+            const bool bad = s_bad[s / top] != 0;
+            plan.ids[s] = bad ? s % top : s_ids[s];
+            plan.shares[s] = bad ? __builtin_nanf("") : shares[s];
+        }
+    }
+    const int units = dp / 8 * tokens;
+    for (int u = blockIdx.x * 256 + threadIdx.x; u < units; u += gridDim.x * 256) {
+        const int t = u / (dp / 8), k0 = u % (dp / 8) * 8;
+        float v[8];
+        fp8_load8(x + (size_t)t * d, k0, d, v);
+        bf16x8_t out[TERMS];
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            bf16_t part[TERMS];
+            moe_split<TERMS>(v[c], part);
+#pragma unroll
+            for (int i = 0; i < TERMS; i++) out[i][c] = part[i];
+        }
+#pragma unroll
+        for (int i = 0; i < TERMS; i++) *(bf16x8_t *)(plan.x + ((size_t)i * tokens + t) * dp + k0) = out[i];
+    }
+}
+
 // Eight codes (two words) as bf16, exactly.
 __device__ __forceinline__ bf16x8_t moe_to_bf16(uint32_t lo, uint32_t hi) {
     const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false);
@@ -352,7 +398,9 @@ __global__ __launch_bounds__(kGateWaves * 64) void moe_gate_up_kernel(
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int g = lane / 16, j = lane % 16, tiles = (ff + 15) / 16, slots = tokens * top;
     const bool writes = blockIdx.x == 0 && blockIdx.y == 0;
-    for (int i = wave; i < tokens; i += kGateWaves) {
+    if (!plan.logits)
+        for (int i = threadIdx.x; i < slots; i += kGateWaves * 64) s_ids[i] = plan.ids[i];
+    for (int i = plan.logits ? wave : tokens; i < tokens; i += kGateWaves) {
         int e;
         float c;
         moe_top_any(plan.logits + (size_t)i * experts, experts, top, renormalize, s_top[wave], e, c);
@@ -823,6 +871,21 @@ void launch_logits(const dz_moe *e, const void *x, int dtype, int tokens, const 
                            c.experts, c.hidden, e->kbd, plan);
 }
 
+void launch_take(const dz_moe *e, const void *x, int dtype, int tokens, const int *ids, const float *shares,
+                 const MoePlan &plan, hipStream_t s) {
+    const dz_moe_config &c = e->cfg;
+    const dim3 grid(std::min(cdiv((size_t)tokens * e->kbd * 16, 256), 1024u));
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL((moe_take_kernel<float, 3>), grid, dim3(256), 0, s, (const float *)x, ids, shares, tokens,
+                           c.experts, c.top_k, c.hidden, e->kbd, plan);
+    else if (dtype == DZ_F16)
+        hipLaunchKernelGGL((moe_take_kernel<half_t, 2>), grid, dim3(256), 0, s, (const half_t *)x, ids, shares, tokens,
+                           c.experts, c.top_k, c.hidden, e->kbd, plan);
+    else
+        hipLaunchKernelGGL((moe_take_kernel<bf16_t, 1>), grid, dim3(256), 0, s, (const bf16_t *)x, ids, shares, tokens,
+                           c.experts, c.top_k, c.hidden, e->kbd, plan);
+}
+
 void launch_top(const dz_moe *e, int tokens, const MoePlan &plan, int *ids, float *shares, hipStream_t s) {
     hipLaunchKernelGGL(moe_top_kernel, dim3(tokens), dim3(64), 0, s, plan.logits, e->cfg.experts, e->cfg.top_k,
                        e->cfg.renormalize, ids, shares);
@@ -871,7 +934,7 @@ void launch_experts(const dz_moe *e, int dtype, int tokens, const MoePlan &plan,
     const unsigned tiles = e->kbf * 8, cus = (unsigned)device_cus();
     const bool many = slots > 12 * c.experts;  // rows an expert, on average
     if (moe_wide_gate(e, tokens, XT)) {
-        launch_top(e, tokens, plan, plan.ids, plan.shares, s);
+        if (plan.logits) launch_top(e, tokens, plan, plan.ids, plan.shares, s);
         if (many) launch_wide_gate<2, XT, HT, XT == 3 ? 2 : 3>(e, tokens, plan, s);
         else launch_wide_gate<1, XT, HT, XT == 1 ? 4 : 3>(e, tokens, plan, s);
     } else {
@@ -1004,20 +1067,52 @@ int32_t moe_route(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, si
     return ctx_launched(ctx, "mixture of experts route");
 }
 
-int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, void *y) {
-    if (int32_t rc = moe_call_ok(ctx, e, x, dtype, tokens, y)) return rc;
+int32_t moe_logits(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, float *logits) {
+    if (int32_t rc = moe_call_ok(ctx, e, x, dtype, tokens, logits)) return rc;
     if (tokens == 0) return DZ_OK;
+    MoePlan plan{};
+    plan.logits = logits;
+    launch_logits(e, x, dtype, (int)tokens, plan, ctx_stream(ctx));
+    return ctx_launched(ctx, "mixture of experts logits");
+}
+
+namespace {
+
+// The layer on its own router's choice, or on the one given.
+int32_t moe_run(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, const int32_t *ids,
+                const float *shares, void *y) {
     void *work = nullptr;
     if (int32_t rc = ctx_workspace(ctx, moe_plan(e, tokens, dtype, true, nullptr, nullptr), &work)) return rc;
     MoePlan plan;
     moe_plan(e, tokens, dtype, true, (uint8_t *)work, &plan);
     hipStream_t s = ctx_stream(ctx);
     const int t = (int)tokens;
-    launch_logits(e, x, dtype, t, plan, s);
+    if (ids) {
+        plan.logits = nullptr;
+        launch_take(e, x, dtype, t, ids, shares, plan, s);
+    } else {
+        launch_logits(e, x, dtype, t, plan, s);
+    }
     if (dtype == DZ_F32) launch_experts<3, 3>(e, dtype, t, plan, y, s);
     else if (dtype == DZ_F16) launch_experts<2, 2>(e, dtype, t, plan, y, s);
     else launch_experts<1, 2>(e, dtype, t, plan, y, s);
     return ctx_launched(ctx, "mixture of experts");
+}
+
+}  // namespace
+
+int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, void *y) {
+    if (int32_t rc = moe_call_ok(ctx, e, x, dtype, tokens, y)) return rc;
+    if (tokens == 0) return DZ_OK;
+    return moe_run(ctx, e, x, dtype, tokens, nullptr, nullptr, y);
+}
+
+int32_t moe_forward_selected(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens,
+                             const int32_t *ids, const float *shares, void *y) {
+    if (int32_t rc = moe_call_ok(ctx, e, x, dtype, tokens, y)) return rc;
+    if (tokens && (!ids || !shares)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (tokens == 0) return DZ_OK;
+    return moe_run(ctx, e, x, dtype, tokens, ids, shares, y);
 }
 
 }  // namespace dz

@@ -1,0 +1,342 @@
+// mx4.hip -- products on microscaled 4-bit floating point (mx4.hpp has the form
+// and the layout).
+//
+//   y[i, j] = sum over 32-blocks b of 2^(ex[i, b] + ew[j, b]) sum over k in b of cx[i, k] cw[j, k]
+//
+// The matrix unit multiplies e2m1 codes, scales them and adds them to f32 sums in
+// one instruction: products of codes and the sum over a block are exact in it, and
+// its additions of blocks f32's (random codes, scales within 2^10 of each other: 2.7e-8
+// off, relative, in the 2-norm), so that f32 outputs need no path of their own.
+#include <algorithm>
+
+#include "../../include/decisive_rocm.h"
+#include "mx4.hpp"
+#include "tiles.hpp"
+
+struct dz_mx4_weight {
+    int rows = 0, cols = 0, kbs = 0;
+    int device = 0;
+    uint8_t *codes = nullptr;   // device
+    uint8_t *scales = nullptr;  // device, behind the codes in the same allocation
+    size_t bytes = 0;
+};
+
+namespace dz {
+
+int32_t ctx_fail(dz_ctx *ctx, int32_t code, const std::string &msg);
+int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what);
+hipStream_t ctx_stream(dz_ctx *ctx);
+int *ctx_flag(dz_ctx *ctx);
+int ctx_device(dz_ctx *ctx);
+int32_t ctx_workspace(dz_ctx *ctx, size_t bytes, void **out);
+int32_t ctx_launched(dz_ctx *ctx, const char *what);
+int32_t ctx_flag_value(dz_ctx *ctx, int *value);
+
+namespace {
+
+// ---- weights -------------------------------------------------------------------
+
+// One thread per block of 32 codes (16 bytes of a row), its scale with it;
+// consecutive threads take consecutive blocks of a row.
+__global__ __launch_bounds__(256) void mx4_retile_kernel(const uint8_t *__restrict__ codes,
+                                                         const uint8_t *__restrict__ scales, size_t pieces, int rows,
+                                                         int cols, int kbs, uint8_t *__restrict__ dst,
+                                                         uint8_t *__restrict__ dst_scales, int *bad) {
+    const int row_bytes = (cols + 1) / 2, blocks = (cols + 31) / 32;
+    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < pieces; id += gridDim.x * (size_t)256) {
+        const int b = (int)(id % (4 * kbs)), kb = b / 4, g = b % 4;
+        const size_t row = id / (4 * kbs);
+        uint4_t w = {0, 0, 0, 0};
+        uint8_t scale = 0;
+        if (row < (size_t)rows && b < blocks) {
+            const uint8_t *src = codes + row * row_bytes + 16 * b;
+            scale = scales[row * blocks + b];
+            if (scale == 255) atomicOr(bad, 1);
+            if (32 * b + 32 <= cols) {
+                w = *(const uint4_bytes_t *)src;
+            } else {
+                for (int e = 0; 32 * b + e < cols; e++)
+                    w[e / 8] |= (uint32_t)(src[e / 2] >> (4 * (e % 2)) & 15) << (4 * (e % 8));
+            }
+        }
+        *(uint4_t *)(dst + mx4_code_at(row, kb, g, 0, kbs)) = w;
+        dst_scales[mx4_scale_at(row, kb, g, kbs)] = scale;
+    }
+}
+
+__global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint8_t *__restrict__ codes,
+                                                          const uint8_t *__restrict__ scales, int rows, int cols,
+                                                          int kbs, float *__restrict__ y) {
+    const size_t count = (size_t)rows * cols;
+    for (size_t id = blockIdx.x * (size_t)256 + threadIdx.x; id < count; id += gridDim.x * (size_t)256) {
+        const size_t row = id / cols;
+        const int k = (int)(id % cols), kb = k / 128, g = k / 32 % 4;
+        const uint32_t c = codes[mx4_code_at(row, kb, g, 0, kbs) + k % 32 / 2] >> (4 * (k % 2));
+        const uint32_t size = c & 7;
+        // 0 and 0.5, then 1, 1.5, 2, 3, 4, 6: one mantissa bit under the exponent field
+        const float v = size < 2 ? 0.5f * (float)size : word_as_float((size + 252) << 22);
+        y[id] = __fmul_rn(c & 8 ? -v : v, mx4_scale_value(scales[mx4_scale_at(row, kb, g, kbs)]));
+    }
+}
+
+// ---- activations ---------------------------------------------------------------
+
+// A workgroup takes 64 rows of one 128-block, whose scale words it writes side by
+// side: 16 lanes a row and eight values a lane, four rows a wave and step. Codes go
+// out as 4-byte pieces; four lanes make the 16 bytes of a block.
+template <class T>
+__global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
+                                                           uint8_t *__restrict__ q, uint8_t *__restrict__ s, int *bad) {
+    const int kb = blockIdx.x, piece = threadIdx.x % 16, k0 = kb * 128 + piece * 8;
+    const int panel = blockIdx.z * gridDim.y + blockIdx.y;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const size_t row = (size_t)panel * 64 + 16 * i + threadIdx.x / 16;
+        if (row >= (size_t)m) return;
+        float v[8];
+        fp8_load8(x + row * k, k0, k, v);
+        uint32_t scale;
+        const uint32_t codes = mx4_quantize8(v, scale);
+        *(uint32_t *)(q + mx4_code_at(row, kb, piece / 4, piece % 4, kbs)) = codes;
+        if (piece % 4 == 0) {
+            s[mx4_scale_at(row, kb, piece / 4, kbs)] = (uint8_t)scale;
+            if (bad && scale == 255) atomicOr(bad, 1);
+        }
+    }
+}
+
+// ---- products: the weight streamed over a few rows -----------------------------
+
+// The dots of 16 x 16 rows over 128 k, scaled and added to c: `a` and `b` are a
+// lane's 32 codes, sa and sb the words whose byte UA or UB is its block's scale.
+template <int UA, int UB>
+__device__ __forceinline__ float4_t mx4_mfma(uint4_t a, uint32_t sa, uint4_t b, uint32_t sb, float4_t c) {
+    const int8v_t va = {(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0};
+    const int8v_t vb = {(int)b[0], (int)b[1], (int)b[2], (int)b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, UA, (int)sa, UB, (int)sb);
+}
+
+// A workgroup owns 16 weight rows and 16 MB activation rows. Its waves take runs of
+// the k-blocks, operands straight from memory, and their f32 partials are added in
+// wave order, from LDS. The matrix unit's operands are swapped (weight first), so a
+// lane holds one activation row and four output columns.
+constexpr int kMx4Waves = 8;
+
+template <int MB>
+__global__ __launch_bounds__(kMx4Waves * 64) void mx4_rows_kernel(const uint8_t *__restrict__ codes,
+                                                                  const uint8_t *__restrict__ scales, int n, int kbs,
+                                                                  const uint8_t *__restrict__ q,
+                                                                  const uint8_t *__restrict__ sx, int m,
+                                                                  void *__restrict__ y, int dtype) {
+    __shared__ __align__(16) float part[kMx4Waves][MB * 256];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int g = lane / 16, j = lane % 16;
+    const int tiles = (n + 15) / 16, t = blockIdx.x % tiles, row0 = blockIdx.x / tiles * 16 * MB;
+    const uint8_t *w = codes + (size_t)t * kbs * 1024 + lane * 16;
+    const uint8_t *ws = scales + (size_t)(t / 4) * kbs * 256 + lane * 4 + t % 4;
+    float4_t acc[MB];
+#pragma unroll
+    for (int b = 0; b < MB; b++) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const int first = (int)((int64_t)kbs * wave / kMx4Waves), last = (int)((int64_t)kbs * (wave + 1) / kMx4Waves);
+    for (int kb = first; kb < last; kb++) {
+        const uint4_t a = __builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 1024));
+        const uint32_t sa = ws[(size_t)kb * 256];
+#pragma unroll
+        for (int b = 0; b < MB; b++) {
+            const int tile = row0 / 16 + b;
+            if (tile * 16 >= m) break;
+            const uint4_t v = *(const uint4_t *)(q + ((size_t)tile * kbs + kb) * 1024 + lane * 16);
+            const uint32_t sb = sx[((size_t)(tile / 4) * kbs + kb) * 256 + lane * 4 + tile % 4];
+            acc[b] = mx4_mfma<0, 0>(a, sa, v, sb, acc[b]);
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < MB; b++) *(float4_t *)&part[wave][(b * 16 + j) * 16 + 4 * g] = acc[b];
+    __syncthreads();
+    for (int i = threadIdx.x; i < MB * 256; i += kMx4Waves * 64) {
+        const int row = row0 + i / 16, col = t * 16 + i % 16;
+        if (row >= m || col >= n) continue;
+        float v = part[0][i];
+#pragma unroll
+        for (int u = 1; u < kMx4Waves; u++) v += part[u][i];
+        fp8_store(y, dtype, (size_t)row * n + col, v);
+    }
+}
+
+template <int MB>
+void mx4_rows_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
+                     hipStream_t s) {
+    hipLaunchKernelGGL(mx4_rows_kernel<MB>, dim3(cdiv(w->rows, 16) * cdiv(m, 16 * MB)), dim3(kMx4Waves * 64), 0, s,
+                       w->codes, w->scales, w->rows, w->kbs, q, sx, m, y, dtype);
+}
+
+void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
+    const int kbs = (int)cdiv(k, 128);
+    const unsigned panels = cdiv(m, 64), most = 32768;  // a grid's y ends at 65535
+    const dim3 grid(kbs, std::min(panels, most), cdiv(panels, most));
+    if (dtype == DZ_F32)
+        hipLaunchKernelGGL(mx4_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, q, sx, bad);
+    else if (dtype == DZ_F16)
+        hipLaunchKernelGGL(mx4_quantize_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)x, m, k, kbs, q, sx, bad);
+    else
+        hipLaunchKernelGGL(mx4_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx, bad);
+}
+
+// The product of m > 0 rows of codes.
+void launch_mx4_product(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
+                        hipStream_t s) {
+    if (m <= 16) mx4_rows_launch<1>(w, q, sx, m, y, dtype, s);
+    else mx4_rows_launch<4>(w, q, sx, m, y, dtype, s);
+}
+
+bool mx4_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }
+size_t whole(size_t n) { return (n + 255) / 256 * 256; }
+
+int32_t mx4_alloc(dz_ctx *ctx, size_t rows, size_t cols, dz_mx4_weight **out) {
+    if (rows == 0 || cols == 0 || rows > kMx4MostRows || cols > kMx4MostCols)
+        return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "invalid weight shape");
+    dz_mx4_weight *w = new (std::nothrow) dz_mx4_weight();
+    if (!w) return ctx_fail(ctx, DZ_RESOURCE_LIMIT, "weight allocation");
+    w->device = ctx_device(ctx);
+    w->rows = (int)rows;
+    w->cols = (int)cols;
+    w->kbs = (int)((cols + 127) / 128);
+    w->bytes = mx4_code_bytes(rows, cols) + mx4_scale_bytes(rows, cols);
+    const hipError_t e = hipMalloc(&w->codes, w->bytes);
+    w->scales = w->codes + mx4_code_bytes(rows, cols);
+    if (e != hipSuccess) {
+        delete w;
+        return ctx_hip_fail(ctx, e, "weight allocation");
+    }
+    *out = w;
+    return DZ_OK;
+}
+
+void mx4_release(dz_mx4_weight *w) {
+    if (!w) return;
+    hipFree(w->codes);
+    delete w;
+}
+
+int32_t mx4_weight_ok(dz_ctx *ctx, const dz_mx4_weight *w) {
+    if (!w) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (w->device != ctx_device(ctx)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "the weight lives on another device");
+    return DZ_OK;
+}
+
+int32_t mx4_codes_ok(dz_ctx *ctx, const uint8_t *q, const uint8_t *s) {
+    if (((uintptr_t)q & 15) != 0 || ((uintptr_t)s & 15) != 0)
+        return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes and scales must be 16-byte aligned");
+    return DZ_OK;
+}
+
+// A handle once its contents are checked (the flag that the kernels just enqueued may set).
+int32_t mx4_finish(dz_ctx *ctx, dz_mx4_weight *w, const char *complaint, dz_mx4_weight **out) {
+    int value = 0;
+    int32_t rc = ctx_flag_value(ctx, &value);
+    if (!rc && value) rc = ctx_fail(ctx, DZ_INVALID_CHECKPOINT, complaint);
+    if (rc) {
+        mx4_release(w);
+        return rc;
+    }
+    *out = w;
+    return DZ_OK;
+}
+
+}  // namespace
+
+int32_t mx4_weight_create(dz_ctx *ctx, const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols,
+                          dz_mx4_weight **out) {
+    if (!out) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    *out = nullptr;
+    if (!codes || !scales) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    dz_mx4_weight *w = nullptr;
+    if (int32_t rc = mx4_alloc(ctx, rows, cols, &w)) return rc;
+    hipStream_t s = ctx_stream(ctx);
+    launch_fill_i32(ctx_flag(ctx), 0, 1, s);
+    const size_t pieces = (rows + 15) / 16 * 16 * w->kbs * 4;
+    hipLaunchKernelGGL(mx4_retile_kernel, dim3((unsigned)std::min((pieces + 255) / 256, (size_t)1 << 20)), dim3(256), 0,
+                       s, codes, scales, pieces, w->rows, w->cols, w->kbs, w->codes, w->scales, ctx_flag(ctx));
+    return mx4_finish(ctx, w, "invalid 4-bit floating point weight", out);
+}
+
+int32_t mx4_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                            dz_mx4_weight **out) {
+    if (!out) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    *out = nullptr;
+    if (!values) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!mx4_dtype(dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    dz_mx4_weight *w = nullptr;
+    if (int32_t rc = mx4_alloc(ctx, rows, cols, &w)) return rc;
+    hipStream_t s = ctx_stream(ctx);
+    launch_fill_i32(ctx_flag(ctx), 0, 1, s);
+    launch_mx4_quantize(values, dtype, w->rows, w->cols, w->codes, w->scales, ctx_flag(ctx), s);
+    return mx4_finish(ctx, w, "non-finite weight", out);
+}
+
+void mx4_weight_free(dz_mx4_weight *w) { mx4_release(w); }
+
+int32_t mx4_weight_info(const dz_mx4_weight *w, size_t *rows, size_t *cols, size_t *device_bytes) {
+    if (!w) return DZ_INVALID_REQUEST;
+    if (rows) *rows = (size_t)w->rows;
+    if (cols) *cols = (size_t)w->cols;
+    if (device_bytes) *device_bytes = w->bytes;
+    return DZ_OK;
+}
+
+int32_t mx4_dequant(dz_ctx *ctx, const dz_mx4_weight *w, float *y) {
+    if (int32_t rc = mx4_weight_ok(ctx, w)) return rc;
+    if (!y) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    const size_t blocks = ((size_t)w->rows * w->cols + 255) / 256;
+    hipLaunchKernelGGL(mx4_dequant_kernel, dim3((unsigned)std::min(blocks, (size_t)1 << 20)), dim3(256), 0,
+                       ctx_stream(ctx), w->codes, w->scales, w->rows, w->cols, w->kbs, y);
+    return ctx_launched(ctx, "mx4 dequant");
+}
+
+int32_t mx4_bytes(size_t m, size_t k, size_t *codes, size_t *scales) {
+    if (k == 0 || k > kMx4MostCols || m > kMx4MostRows) return DZ_INVALID_PARAMETERS;
+    if (codes) *codes = mx4_code_bytes(m, k);
+    if (scales) *scales = mx4_scale_bytes(m, k);
+    return DZ_OK;
+}
+
+int32_t mx4_quantize(dz_ctx *ctx, const void *x, int32_t dtype, size_t m, size_t k, uint8_t *q, uint8_t *s) {
+    if (!mx4_dtype(dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (k == 0 || k > kMx4MostCols) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "invalid activation shape");
+    if (m && (!x || !q || !s)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (m > kMx4MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (int32_t rc = mx4_codes_ok(ctx, q, s)) return rc;
+    if (m == 0) return DZ_OK;
+    launch_mx4_quantize(x, dtype, (int)m, (int)k, q, s, nullptr, ctx_stream(ctx));
+    return ctx_launched(ctx, "mx4 quantize");
+}
+
+int32_t mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q, const uint8_t *s, size_t m, void *y,
+                      int32_t y_dtype) {
+    if (int32_t rc = mx4_weight_ok(ctx, w)) return rc;
+    if (m && (!q || !s || !y)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!mx4_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (m > kMx4MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (int32_t rc = mx4_codes_ok(ctx, q, s)) return rc;
+    if (m == 0) return DZ_OK;
+    launch_mx4_product(w, q, s, (int)m, y, y_dtype, ctx_stream(ctx));
+    return ctx_launched(ctx, "mx4 linear");
+}
+
+int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                   int32_t y_dtype) {
+    if (int32_t rc = mx4_weight_ok(ctx, w)) return rc;
+    if (m && (!x || !y)) return ctx_fail(ctx, DZ_INVALID_REQUEST, "null pointer");
+    if (!mx4_dtype(x_dtype) || !mx4_dtype(y_dtype)) return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "unknown dtype");
+    if (m > kMx4MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
+    if (m == 0) return DZ_OK;
+    const size_t codes = whole(mx4_code_bytes(m, w->cols)), scales = whole(mx4_scale_bytes(m, w->cols));
+    void *work = nullptr;
+    if (int32_t rc = ctx_workspace(ctx, codes + scales, &work)) return rc;
+    uint8_t *q = (uint8_t *)work, *sx = q + codes;
+    launch_mx4_quantize(x, x_dtype, (int)m, w->cols, q, sx, nullptr, ctx_stream(ctx));
+    launch_mx4_product(w, q, sx, (int)m, y, y_dtype, ctx_stream(ctx));
+    return ctx_launched(ctx, "mx4 linear");
+}
+
+}  // namespace dz

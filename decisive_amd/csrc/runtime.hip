@@ -110,6 +110,27 @@ int32_t moe_info(const dz_moe *e, dz_moe_config *cfg, size_t *device_bytes);
 int32_t moe_route(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, int32_t *ids,
                   float *shares);
 int32_t moe_forward(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, void *y);
+int32_t moe_logits(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens, float *logits);
+int32_t moe_select(dz_ctx *ctx, const dz_moe_selection *rule, const void *logits, int32_t dtype, size_t tokens,
+                   const float *bias, int32_t *ids, float *shares);
+int32_t moe_forward_selected(dz_ctx *ctx, const dz_moe *e, const void *x, int32_t dtype, size_t tokens,
+                             const int32_t *ids, const float *shares, void *y);
+int32_t mx4_weight_create(dz_ctx *ctx, const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols,
+                          dz_mx4_weight **out);
+int32_t mx4_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                            dz_mx4_weight **out);
+void mx4_weight_free(dz_mx4_weight *w);
+int32_t mx4_weight_info(const dz_mx4_weight *w, size_t *rows, size_t *cols, size_t *device_bytes);
+int32_t mx4_dequant(dz_ctx *ctx, const dz_mx4_weight *w, float *y);
+int32_t mx4_bytes(size_t m, size_t k, size_t *codes, size_t *scales);
+int32_t mx4_quantize(dz_ctx *ctx, const void *x, int32_t dtype, size_t m, size_t k, uint8_t *q, uint8_t *s);
+int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                   int32_t y_dtype);
+int32_t mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q, const uint8_t *s, size_t m, void *y,
+                      int32_t y_dtype);
+int32_t add_rmsnorm(dz_ctx *ctx, const void *x, const void *residual, int32_t dtype, size_t rows, size_t d,
+                    const float *w, float eps, int32_t zero_centered, void *sum, void *y, uint8_t *q, void *s,
+                    bool mx);
 }  // namespace dz
 
 namespace {
@@ -1136,6 +1157,87 @@ int32_t dz_moe_route(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtyp
 int32_t dz_moe_forward(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtype, size_t tokens, void *y) {
     DZ_BEGIN(ctx);
     return dz::moe_forward(ctx, moe, x, dtype, tokens, y);
+}
+
+int32_t dz_moe_logits(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtype, size_t tokens, float *logits) {
+    DZ_BEGIN(ctx);
+    return dz::moe_logits(ctx, moe, x, dtype, tokens, logits);
+}
+
+int32_t dz_moe_select(dz_ctx *ctx, const dz_moe_selection *rule, const void *logits, int32_t dtype, size_t tokens,
+                      const float *bias, int32_t *ids, float *shares) {
+    DZ_BEGIN(ctx);
+    return dz::moe_select(ctx, rule, logits, dtype, tokens, bias, ids, shares);
+}
+
+int32_t dz_moe_forward_selected(dz_ctx *ctx, const dz_moe *moe, const void *x, int32_t dtype, size_t tokens,
+                                const int32_t *ids, const float *shares, void *y) {
+    DZ_BEGIN(ctx);
+    return dz::moe_forward_selected(ctx, moe, x, dtype, tokens, ids, shares, y);
+}
+
+int32_t dz_mx4_weight_create(dz_ctx *ctx, const uint8_t *codes, const uint8_t *scales, size_t rows, size_t cols,
+                             dz_mx4_weight **out) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    return dz::mx4_weight_create(ctx, codes, scales, rows, cols, out);
+}
+
+int32_t dz_mx4_weight_quantize(dz_ctx *ctx, const void *values, int32_t dtype, size_t rows, size_t cols,
+                               dz_mx4_weight **out) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    return dz::mx4_weight_quantize(ctx, values, dtype, rows, cols, out);
+}
+
+int32_t dz_mx4_weight_free(dz_ctx *ctx, dz_mx4_weight *w) {
+    DZ_BEGIN(ctx);
+    DZ_NOT_CAPTURING(ctx);
+    DZ_HIP(ctx, hipStreamSynchronize(ctx->stream), "stream synchronize");
+    dz::mx4_weight_free(w);
+    return DZ_OK;
+}
+
+int32_t dz_mx4_weight_info(const dz_mx4_weight *w, size_t *rows, size_t *cols, size_t *device_bytes) {
+    return dz::mx4_weight_info(w, rows, cols, device_bytes);
+}
+
+int32_t dz_mx4_dequant(dz_ctx *ctx, const dz_mx4_weight *w, float *y) {
+    DZ_BEGIN(ctx);
+    return dz::mx4_dequant(ctx, w, y);
+}
+
+int32_t dz_mx4_bytes(size_t m, size_t k, size_t *codes, size_t *scales) { return dz::mx4_bytes(m, k, codes, scales); }
+
+int32_t dz_mx4_quantize(dz_ctx *ctx, const void *x, int32_t x_dtype, size_t m, size_t k, uint8_t *q, uint8_t *s) {
+    DZ_BEGIN(ctx);
+    return dz::mx4_quantize(ctx, x, x_dtype, m, k, q, s);
+}
+
+int32_t dz_mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x_dtype, size_t m, void *y,
+                      int32_t y_dtype) {
+    DZ_BEGIN(ctx);
+    return dz::mx4_linear(ctx, w, x, x_dtype, m, y, y_dtype);
+}
+
+int32_t dz_mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q, const uint8_t *s, size_t m, void *y,
+                         int32_t y_dtype) {
+    DZ_BEGIN(ctx);
+    return dz::mx4_linear_q4(ctx, w, q, s, m, y, y_dtype);
+}
+
+int32_t dz_add_rmsnorm_fp8(dz_ctx *ctx, const void *x, const void *residual, int32_t dtype, size_t rows, size_t d,
+                           const float *w, float eps, int32_t zero_centered, void *sum, void *y, uint8_t *q,
+                           float *s) {
+    DZ_BEGIN(ctx);
+    return dz::add_rmsnorm(ctx, x, residual, dtype, rows, d, w, eps, zero_centered, sum, y, q, s, false);
+}
+
+int32_t dz_add_rmsnorm_mx4(dz_ctx *ctx, const void *x, const void *residual, int32_t dtype, size_t rows, size_t d,
+                           const float *w, float eps, int32_t zero_centered, void *sum, void *y, uint8_t *q,
+                           uint8_t *s) {
+    DZ_BEGIN(ctx);
+    return dz::add_rmsnorm(ctx, x, residual, dtype, rows, d, w, eps, zero_centered, sum, y, q, s, true);
 }
 
 // ---- epilogues --------------------------------------------------------------------------

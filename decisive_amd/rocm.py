@@ -84,6 +84,12 @@ class MoeConfig(ctypes.Structure):
                 ("ff", ctypes.c_int32), ("renormalize", ctypes.c_int32)]
 
 
+class MoeSelection(ctypes.Structure):
+    _fields_ = [("experts", ctypes.c_int32), ("top_k", ctypes.c_int32), ("sigmoid", ctypes.c_int32),
+                ("groups", ctypes.c_int32), ("top_groups", ctypes.c_int32), ("group_best", ctypes.c_int32),
+                ("renormalize", ctypes.c_int32), ("scale", ctypes.c_float)]
+
+
 MOE_MAX_TOKENS = 128  # dz_moe_forward's tokens per call
 
 
@@ -176,6 +182,20 @@ _SIGNATURES = {
     "dz_moe_info": (I32, [P, ctypes.POINTER(MoeConfig), ctypes.POINTER(SZ)]),
     "dz_moe_route": (I32, [P, P, P, I32, SZ, P, P]),
     "dz_moe_forward": (I32, [P, P, P, I32, SZ, P]),
+    "dz_moe_logits": (I32, [P, P, P, I32, SZ, P]),
+    "dz_moe_select": (I32, [P, ctypes.POINTER(MoeSelection), P, I32, SZ, P, P, P]),
+    "dz_moe_forward_selected": (I32, [P, P, P, I32, SZ, P, P, P]),
+    "dz_mx4_weight_create": (I32, [P, P, P, SZ, SZ, PP]),
+    "dz_mx4_weight_quantize": (I32, [P, P, I32, SZ, SZ, PP]),
+    "dz_mx4_weight_free": (I32, [P, P]),
+    "dz_mx4_weight_info": (I32, [P, ctypes.POINTER(SZ), ctypes.POINTER(SZ), ctypes.POINTER(SZ)]),
+    "dz_mx4_dequant": (I32, [P, P, P]),
+    "dz_mx4_bytes": (I32, [SZ, SZ, ctypes.POINTER(SZ), ctypes.POINTER(SZ)]),
+    "dz_mx4_quantize": (I32, [P, P, I32, SZ, SZ, P, P]),
+    "dz_mx4_linear": (I32, [P, P, P, I32, SZ, P, I32]),
+    "dz_mx4_linear_q4": (I32, [P, P, P, P, SZ, P, I32]),
+    "dz_add_rmsnorm_fp8": (I32, [P, P, P, I32, SZ, SZ, P, F, I32, P, P, P, P]),
+    "dz_add_rmsnorm_mx4": (I32, [P, P, P, I32, SZ, SZ, P, F, I32, P, P, P, P]),
     "dz_tune": (I32, [P, U32, ctypes.c_char_p, ctypes.c_char_p, SZ]),
     "dz_select_variant": (I32, [P, ctypes.c_char_p, ctypes.c_char_p]),
 }
@@ -272,6 +292,38 @@ class Fp8Weight:
             pass
 
 
+class Mx4Weight:
+    """A device-resident weight in e2m1 with a power of two for each 32 values of a row (dz_mx4_weight)."""
+
+    def __init__(self, ctx: "Context", handle: int):
+        self.ctx, self.handle = ctx, handle
+        rows, cols, dbytes = SZ(), SZ(), SZ()
+        load().dz_mx4_weight_info(handle, ctypes.byref(rows), ctypes.byref(cols), ctypes.byref(dbytes))
+        self.rows, self.cols, self.device_bytes = rows.value, cols.value, dbytes.value
+
+    def free(self):
+        if self.handle:
+            self.ctx._check(load().dz_mx4_weight_free(self.ctx.handle, self.handle))
+        self.handle = 0
+
+    def __del__(self):
+        try:
+            if self.handle and self.ctx.handle:
+                load().dz_mx4_weight_free(self.ctx.handle, self.handle)
+                self.handle = 0
+        except Exception:
+            pass
+
+
+def mx4_bytes(m: int, k: int) -> tuple[int, int]:
+    """dz_mx4_bytes: the bytes of the codes and of the scales of m rows of k activations."""
+    codes, scales = SZ(), SZ()
+    rc = load().dz_mx4_bytes(m, k, ctypes.byref(codes), ctypes.byref(scales))
+    if rc:
+        raise DzError(rc, "invalid activation shape")
+    return codes.value, scales.value
+
+
 class Moe:
     """A mixture-of-experts layer for a few tokens (dz_moe)."""
 
@@ -287,6 +339,13 @@ class Moe:
 
     def forward(self, x, dtype: int, tokens: int, y):
         self.ctx._check(load().dz_moe_forward(self.ctx.handle, self.handle, _addr(x), dtype, tokens, _addr(y)))
+
+    def logits(self, x, dtype: int, tokens: int, logits):
+        self.ctx._check(load().dz_moe_logits(self.ctx.handle, self.handle, _addr(x), dtype, tokens, _addr(logits)))
+
+    def forward_selected(self, x, dtype: int, tokens: int, ids, shares, y):
+        self.ctx._check(load().dz_moe_forward_selected(self.ctx.handle, self.handle, _addr(x), dtype, tokens,
+                                                       _addr(ids), _addr(shares), _addr(y)))
 
     def free(self):
         if self.handle:
@@ -494,6 +553,45 @@ class Context:
 
     def fp8_linear_q8(self, w: "Fp8Weight", q, s, m: int, y, y_dtype: int):
         self._check(load().dz_fp8_linear_q8(self.handle, w.handle, _addr(q), _addr(s), m, _addr(y), y_dtype))
+
+    def mx4_weight(self, codes, scales, rows: int, cols: int) -> "Mx4Weight":
+        """dz_mx4_weight_create: codes [rows x ceil(cols/2)] and scale bytes [rows x ceil(cols/32)], both on the device."""
+        h = P()
+        self._check(load().dz_mx4_weight_create(self.handle, _addr(codes), _addr(scales), rows, cols,
+                                                ctypes.byref(h)))
+        return Mx4Weight(self, h.value)
+
+    def mx4_weight_quantize(self, values, dtype: int, rows: int, cols: int) -> "Mx4Weight":
+        h = P()
+        self._check(load().dz_mx4_weight_quantize(self.handle, _addr(values), dtype, rows, cols, ctypes.byref(h)))
+        return Mx4Weight(self, h.value)
+
+    def mx4_dequant(self, w: "Mx4Weight", y):
+        self._check(load().dz_mx4_dequant(self.handle, w.handle, _addr(y)))
+
+    def mx4_quantize(self, x, x_dtype: int, m: int, k: int, q, s):
+        self._check(load().dz_mx4_quantize(self.handle, _addr(x), x_dtype, m, k, _addr(q), _addr(s)))
+
+    def mx4_linear(self, w: "Mx4Weight", x, x_dtype: int, m: int, y, y_dtype: int):
+        self._check(load().dz_mx4_linear(self.handle, w.handle, _addr(x), x_dtype, m, _addr(y), y_dtype))
+
+    def mx4_linear_q4(self, w: "Mx4Weight", q, s, m: int, y, y_dtype: int):
+        self._check(load().dz_mx4_linear_q4(self.handle, w.handle, _addr(q), _addr(s), m, _addr(y), y_dtype))
+
+    def add_rmsnorm_fp8(self, x, residual, dtype: int, rows: int, d: int, w, eps: float, total, q, s, y=None,
+                        zero_centered: bool = True):
+        """dz_add_rmsnorm_fp8: `total` receives x + residual, q and s the normed rows' codes and scales."""
+        self._check(load().dz_add_rmsnorm_fp8(self.handle, _addr(x), _addr(residual), dtype, rows, d, _addr(w), eps,
+                                              int(zero_centered), _addr(total), _addr(y), _addr(q), _addr(s)))
+
+    def add_rmsnorm_mx4(self, x, residual, dtype: int, rows: int, d: int, w, eps: float, total, q, s, y=None,
+                        zero_centered: bool = True):
+        self._check(load().dz_add_rmsnorm_mx4(self.handle, _addr(x), _addr(residual), dtype, rows, d, _addr(w), eps,
+                                              int(zero_centered), _addr(total), _addr(y), _addr(q), _addr(s)))
+
+    def moe_select(self, rule: MoeSelection, logits, dtype: int, tokens: int, bias, ids, shares):
+        self._check(load().dz_moe_select(self.handle, ctypes.byref(rule), _addr(logits), dtype, tokens, _addr(bias),
+                                         _addr(ids), _addr(shares)))
 
     def moe(self, cfg: MoeConfig, router, router_dtype: int, gate, up, down) -> "Moe":
         """dz_moe_create: gate, up and down are pairs (codes, scales) over all experts."""

@@ -39,7 +39,8 @@
  *    dz_pplx_set_vector, dz_pplx_layer and dz_pplx_layer_part (they may grow
  *    the model's activation buffers), dz_pplx_activation,
  *    dz_pplx_forward_rows, dz_pplx_set_residency, dz_fp8_weight_create,
- *    dz_fp8_weight_quantize, dz_fp8_weight_free, dz_moe_create, dz_moe_free and
+ *    dz_fp8_weight_quantize, dz_fp8_weight_free, dz_mx4_weight_create,
+ *    dz_mx4_weight_quantize, dz_mx4_weight_free, dz_moe_create, dz_moe_free and
  *    dz_tune.
  */
 #ifndef DECISIVE_ROCM_H
@@ -377,6 +378,92 @@ int32_t dz_fp8_linear(dz_ctx *ctx, const dz_fp8_weight *w, const void *x_dev, in
 int32_t dz_fp8_linear_q8(dz_ctx *ctx, const dz_fp8_weight *w, const uint8_t *q_dev, const float *s_dev, size_t m,
                          void *y_dev, int32_t y_dtype);
 
+/* ---- microscaled 4-bit floating point ------------------------------------------- */
+
+/* No counterpart in the reference: weights and activations in e2m1 (0, 0.5, 1,
+ * 1.5, 2, 3, 4, 6 and their negatives; the codes 0..7, and 8..15 for the
+ * negatives) with a scale 2^e for each 32 values along k, kept as the byte
+ * e + 127 (255 is NaN): the MXFP4 form of the OCP Microscaling Formats
+ * specification 1.0. A block's e is floor(log2 max|v|) - 2, at least -127 (what a
+ * block of zeros has), and a code is v / 2^e to nearest even, cut at 6. Sizes need
+ * not be multiples of anything; the last block of a row is short. A handle is
+ * read-only once made: contexts of its device may share it. */
+typedef struct dz_mx4_weight dz_mx4_weight;
+
+/* A weight from a checkpoint's arrays on the device: codes_dev
+ * [rows x ceil(cols/2)] bytes row-major, two codes a byte, the even column in the
+ * low half; scales_dev [rows x ceil(cols/32)] bytes. Both are copied (re-tiled);
+ * what stands past cols is not read as a value. A scale of 255 is
+ * DZ_INVALID_CHECKPOINT. rows <= 2^24, cols <= 2^20 (DZ_INVALID_PARAMETERS).
+ * Synchronous. */
+int32_t dz_mx4_weight_create(dz_ctx *ctx, const uint8_t *codes_dev, const uint8_t *scales_dev, size_t rows,
+                             size_t cols, dz_mx4_weight **out);
+/* A weight from values_dev [rows x cols] of `dtype`, quantized as above. A value
+ * that is not finite is DZ_INVALID_CHECKPOINT. Synchronous. */
+int32_t dz_mx4_weight_quantize(dz_ctx *ctx, const void *values_dev, int32_t dtype, size_t rows, size_t cols,
+                               dz_mx4_weight **out);
+int32_t dz_mx4_weight_free(dz_ctx *ctx, dz_mx4_weight *w);
+/* rows, cols and device bytes; any pointer may be NULL. */
+int32_t dz_mx4_weight_info(const dz_mx4_weight *w, size_t *rows, size_t *cols, size_t *device_bytes);
+/* y_dev f32 [rows x cols] = code * 2^e (infinite where 2^e times a code is past f32's range). */
+int32_t dz_mx4_dequant(dz_ctx *ctx, const dz_mx4_weight *w, float *y_dev);
+
+/* The bytes of the codes and of the scales of m rows of k activations; either
+ * pointer may be NULL. With G = ceil(k/128): codes [ceil(m/16)][G][64][16], where
+ * piece 16 g + j of chunk (t, b) holds row 16 t + j, k = 128 b + 32 g .. + 31, the
+ * even k in the low half of a byte; scales [ceil(m/64)][G][64][4], where byte u of
+ * piece 16 g + j of (R, b) is that of row 64 R + 16 u + j, k as above.
+ * DZ_INVALID_PARAMETERS for k = 0, k > 2^20 or m > 2^24. */
+int32_t dz_mx4_bytes(size_t m, size_t k, size_t *codes, size_t *scales);
+/* Activations in that form: x_dev [m x k] of `x_dtype` (at any address its type
+ * allows), q_dev and s_dev of dz_mx4_bytes' sizes, 16-byte aligned. Codes past k
+ * are written as 0; rows past m are left as they were. A block with a value that
+ * is not finite gets the scale 255 and codes 0, so that its row's products are NaN
+ * and no other row's. k <= 2^20, m <= 2^24. */
+int32_t dz_mx4_quantize(dz_ctx *ctx, const void *x_dev, int32_t x_dtype, size_t m, size_t k, uint8_t *q_dev,
+                        uint8_t *s_dev);
+/* y = q(x) W^T: x_dev [m x cols(w)] of `x_dtype`, quantized as dz_mx4_quantize
+ * does, y_dev [m x rows(w)] of `y_dtype` (each at any address its type allows; y
+ * may not overlap x). Sums are f32 and rounded once; products of codes and their
+ * sum over a block of 32 are exact. Where the products of a block, or a sum, leave
+ * f32's range the output is infinite or NaN. The order of a row's sum may depend on
+ * m. Uses the context workspace (run the call once before capturing it; one replay
+ * at a time). m may be 0, and is at most 2^24. */
+int32_t dz_mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x_dev, int32_t x_dtype, size_t m, void *y_dev,
+                      int32_t y_dtype);
+/* dz_mx4_linear on activations already quantized (dz_mx4_quantize or
+ * dz_add_rmsnorm_mx4 with k = cols(w)): several weights can share one quantization.
+ * The same bits as dz_mx4_linear's, and the context workspace as there. */
+int32_t dz_mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q_dev, const uint8_t *s_dev, size_t m,
+                         void *y_dev, int32_t y_dtype);
+
+/* ---- the norm before a quantized product ------------------------------------------ */
+
+/* The residual's addition, the RMS norm and the codes that the next products take,
+ * in one pass (dz_add, dz_rmsnorm and dz_fp8_quantize are its f32 parts):
+ *   h = T(f32(x + r)),  i = f32(1 / sqrt(sum h^2 / d + eps)),  y = f32(f32(h i) w)
+ * T is `dtype`, that of x_dev, residual_dev, sum_dev and y_dev, all [rows x d] (at
+ * any address it allows); the sum of squares is held in 64 bits, and w is w_dev[d]
+ * or, with zero_centered = 1, f32(1 + w_dev[d]).
+ *  - residual_dev may be NULL: h = x, and sum_dev must be NULL too;
+ *  - sum_dev (may be NULL) receives h: residual_dev itself, x_dev, or another buffer;
+ *  - y_dev (may be NULL) receives y rounded to T: x_dev, residual_dev or another buffer, not sum_dev;
+ *  - q_dev and s_dev receive y (before that rounding) as dz_fp8_quantize's codes and
+ *    scales (f32 [G x rows]) or dz_mx4_quantize's, for dz_fp8_linear_q8 and
+ *    dz_mx4_linear_q4 with k = d.
+ * Nothing else may overlap. A row of h that holds a value that is not finite has NaN
+ * in its codes' scales, and so NaN products; no other row has. Codes and scales do not
+ * depend on the order of a sum but where i lies within 2^-40 of a rounding border.
+ * eps finite and >= 0, d <= 2^20, rows <= 2^24; codes 16-byte aligned (mx4: scales too). */
+int32_t dz_add_rmsnorm_fp8(dz_ctx *ctx, const void *x_dev, const void *residual_dev, int32_t dtype, size_t rows,
+                           size_t d, const float *w_dev, float eps, int32_t zero_centered, void *sum_dev, void *y_dev,
+                           uint8_t *q_dev, float *s_dev);
+int32_t dz_add_rmsnorm_mx4(dz_ctx *ctx, const void *x_dev, const void *residual_dev, int32_t dtype, size_t rows,
+                           size_t d, const float *w_dev, float eps, int32_t zero_centered, void *sum_dev, void *y_dev,
+                           uint8_t *q_dev, uint8_t *s_dev);
+
+/* ---- mixture of experts ------------------------------------------------------------ */
+
 typedef struct dz_moe_config {
     int32_t experts;     /* at most 512 */
     int32_t top_k;       /* experts a token goes to, at most 16 and at most experts */
@@ -420,6 +507,43 @@ int32_t dz_moe_route(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t 
  * outputs are infinite or NaN. Neither touches another token. Uses the context
  * workspace (run the call once before capturing it; one replay at a time). */
 int32_t dz_moe_forward(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t dtype, size_t tokens, void *y_dev);
+
+/* The layer's router alone: logits_dev f32 [tokens x experts] = x router^T, tokens
+ * as dz_moe_forward takes them. */
+int32_t dz_moe_logits(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t dtype, size_t tokens,
+                      float *logits_dev);
+
+typedef struct dz_moe_selection {
+    int32_t experts;     /* at most 512 */
+    int32_t top_k;       /* experts a token goes to, at most 16 */
+    int32_t sigmoid;     /* 0: scores are the softmax of the logits; 1: 1 / (1 + exp(-logit)) */
+    int32_t groups;      /* equal groups of neighbouring experts, at most 64; 1: none */
+    int32_t top_groups;  /* groups a token's experts come from; top_k experts must fit them */
+    int32_t group_best;  /* 1: a group ranks by its largest value; 2: by the sum of its two largest */
+    int32_t renormalize; /* 1: the chosen experts' shares sum to `scale`; 0: they are scores times `scale` */
+    float scale;         /* finite */
+} dz_moe_selection;
+/* A token's experts by the rule of its layer (no counterpart in the reference; a
+ * plain softmax top-k is dz_moe_route's): logits_dev [tokens x experts] of `dtype`,
+ * bias_dev f32 [experts] or NULL,
+ *   s_e = score of logit e,  c_e = s_e + bias_e
+ *   the top_groups groups of largest rank stay; the top_k experts of largest c in them
+ *   share_e = scale s_e, or scale s_e / (sum of the chosen s)
+ * Equal values go to the lower index. Scores and ranks are held in 64 bits. ids_dev
+ * int32 and shares_dev f32 [tokens x top_k], by falling c. An expert of logit (or
+ * bias) -infinity is masked: it ranks below every other, adds nothing to its group's
+ * rank, is chosen only where nothing else is left (by the lowest index) and a masked
+ * logit's score is 0; chosen scores that are all 0 have shares 0. A token with a logit
+ * or a biased score that is NaN or +infinity gets the experts 0 .. top_k - 1 and NaN
+ * shares. No other token is touched. tokens <= 2^24. */
+int32_t dz_moe_select(dz_ctx *ctx, const dz_moe_selection *rule, const void *logits_dev, int32_t dtype, size_t tokens,
+                      const float *bias_dev, int32_t *ids_dev, float *shares_dev);
+/* dz_moe_forward on a choice already made (dz_moe_select's, or any other):
+ * ids_dev int32 and shares_dev f32 [tokens x top_k(moe)], in any order. A token with
+ * an expert that does not exist, or with one twice, gives NaN outputs. On the choice
+ * of dz_moe_route for the same tokens the same bits as dz_moe_forward's. */
+int32_t dz_moe_forward_selected(dz_ctx *ctx, const dz_moe *moe, const void *x_dev, int32_t dtype, size_t tokens,
+                                const int32_t *ids_dev, const float *shares_dev, void *y_dev);
 
 /* ---- layer epilogues --------------------------------------------------------- */
 
