@@ -28,6 +28,7 @@ int32_t ctx_hip_fail(dz_ctx *ctx, hipError_t e, const char *what);
 hipStream_t ctx_stream(dz_ctx *ctx);
 int *ctx_flag(dz_ctx *ctx);
 int ctx_device(dz_ctx *ctx);
+int ctx_variant(dz_ctx *ctx, const char *family);
 int32_t ctx_workspace(dz_ctx *ctx, size_t bytes, void **out);
 int32_t ctx_launched(dz_ctx *ctx, const char *what);
 int32_t ctx_flag_value(dz_ctx *ctx, int *value);
@@ -170,6 +171,215 @@ void mx4_rows_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx
                        w->codes, w->scales, w->rows, w->kbs, q, sx, m, y, dtype);
 }
 
+// ---- products: tiles over many rows ----------------------------------------------
+
+// dma4 with a scalar offset added to every lane's (dma16_at's contract).
+__device__ __forceinline__ void dma4_at(uint32_t lds, uint32_t voff, int32x4_t rsrc, uint32_t soff) {
+    const int32x4_t r = {__builtin_amdgcn_readfirstlane(rsrc[0]), __builtin_amdgcn_readfirstlane(rsrc[1]),
+                         __builtin_amdgcn_readfirstlane(rsrc[2]), 0x00020000};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
+                 :
+                 : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
+                 : "memory", "m0");
+}
+
+// mx4_mfma with the bytes as values that the compiler knows once loops are unrolled.
+template <int UA>
+__device__ __forceinline__ float4_t mx4_mfma_b(int ub, uint4_t a, uint32_t sa, uint4_t b, uint32_t sb, float4_t c) {
+    if (ub == 0) return mx4_mfma<UA, 0>(a, sa, b, sb, c);
+    if (ub == 1) return mx4_mfma<UA, 1>(a, sa, b, sb, c);
+    if (ub == 2) return mx4_mfma<UA, 2>(a, sa, b, sb, c);
+    return mx4_mfma<UA, 3>(a, sa, b, sb, c);
+}
+__device__ __forceinline__ float4_t mx4_mfma_ab(int ua, int ub, uint4_t a, uint32_t sa, uint4_t b, uint32_t sb,
+                                                float4_t c) {
+    if (ua == 0) return mx4_mfma_b<0>(ub, a, sa, b, sb, c);
+    if (ua == 1) return mx4_mfma_b<1>(ub, a, sa, b, sb, c);
+    if (ua == 2) return mx4_mfma_b<2>(ub, a, sa, b, sb, c);
+    return mx4_mfma_b<3>(ub, a, sa, b, sb, c);
+}
+
+// Block tile BM x BN (activation rows x weight rows). KS groups of WGM x WGN
+// waves each take every KS-th 128-block of k; a step is KS blocks, one a group, in
+// one of NS LDS stages that buffer_load ... lds fills, chunks and scale words as they
+// lie in memory, which is operand order: a lane's 16 bytes are its own, and no two
+// lanes' reads meet in a bank. A wave reads the operands of step i + 1 while it
+// multiplies step i's, so that its products wait for no read; a stage is free once its
+// operands are in registers, a step before it is multiplied, and NS - 1 steps' loads
+// are in flight. Scales cost nothing: the matrix unit adds the exponents. The groups'
+// sums are added in group order, through LDS. Where k is cut, workgroup b / tiles takes
+// `per` of its blocks and writes their sums as f32 for fp8_join.
+template <int BM, int BN, int WGM, int WGN, int KS, int NS>
+__global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8_t *__restrict__ codes,
+                                                                     const uint8_t *__restrict__ scales, int n, int kbs,
+                                                                     const uint8_t *__restrict__ q,
+                                                                     const uint8_t *__restrict__ sx, int m,
+                                                                     void *__restrict__ y, int dtype, int tiles,
+                                                                     int per) {
+    constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
+    constexpr int XPW = BM / 16 / WAVES, WPW = BN / 16 / WAVES;            // 1 KiB loads per wave and stage
+    constexpr int XP = BM < 64 ? 1 : BM / 64, WP = BN < 64 ? 1 : BN / 64;  // panels of scale words
+    constexpr int SPW = (XP + WP + WAVES - 1) / WAVES, PB = XPW + WPW + SPW;
+    constexpr int XW = TM < 64 ? 1 : TM / 64, WW = TN < 64 ? 1 : TN / 64;  // scale words of a wave
+    constexpr int XB = BM * 64, SB = XB + BN * 64, PART = SB + (XP + WP) * 256, STAGE = KS * PART;
+    static_assert(XPW * 16 * WAVES == BM && WPW * 16 * WAVES == BN, "whole loads for each wave");
+    static_assert((TM % 64 == 0 || 64 % TM == 0) && (TN % 64 == 0 || 64 % TN == 0), "scale words of whole or one panel");
+    static_assert((NS - 1) * PB <= 63, "vmcnt range");
+    static_assert((KS - 1) * BM * BN * 4 <= NS * STAGE, "the groups' sums fit the stages");
+    __shared__ __align__(16) uint8_t lds[NS * STAGE];
+
+    const int wave_all = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const int group = wave_all / WAVES, wave = wave_all % WAVES;
+    const int wm = wave / WGN, wn = wave % WGN, g = lane / 16, j = lane % 16;
+    const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
+    int tm, tn;
+    const int split = blockIdx.x / tiles, first = split * per, last = min(kbs, first + per);  // its blocks of k
+    xcd_tile(blockIdx.x - split * tiles, tiles, tiles_m, tiles_n, tm, tn);
+    const int row0 = tm * BM, col0 = tn * BN;
+    const int have_x = min(BM / 16, (m + 15) / 16 - row0 / 16), have_w = min(BN / 16, (n + 15) / 16 - col0 / 16);
+    const int panels_x = min(XP, (m + 63) / 64 - row0 / 64), panels_w = min(WP, (n + 63) / 64 - col0 / 64);
+    const int32x4_t rx = buffer_rsrc(q + (size_t)(row0 / 16) * kbs * 1024, (uint32_t)(have_x * kbs) * 1024u);
+    const int32x4_t rw = buffer_rsrc(codes + (size_t)(col0 / 16) * kbs * 1024, (uint32_t)(have_w * kbs) * 1024u);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + group * PART;
+    // this wave's panels of scale words (some load one twice, so that all waits go by count)
+    int panel[SPW];
+    int32x4_t rs[SPW];
+    uint32_t soff[SPW];
+#pragma unroll
+    for (int p = 0; p < SPW; p++) {
+        panel[p] = (wave * SPW + p) % (XP + WP);
+        const bool of_x = panel[p] < XP;
+        rs[p] = of_x ? buffer_rsrc(sx + (size_t)(row0 / 64) * kbs * 256, (uint32_t)(panels_x * kbs) * 256u)
+                     : buffer_rsrc(scales + (size_t)(col0 / 64) * kbs * 256, (uint32_t)(panels_w * kbs) * 256u);
+        soff[p] = (uint32_t)(of_x ? panel[p] : panel[p] - XP) * kbs * 256 + lane * 4;
+    }
+
+    // Blocks past the last one load nothing (every offset out of range, zeros in LDS).
+    auto load_stage = [&](int stage, int step) {
+        const int kb = first + step * KS + group;
+        const bool live = kb < last;
+        const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u, k = live ? (uint32_t)kb : 0u;
+#pragma unroll
+        for (int p = 0; p < XPW; p++)
+            dma16_at(at + (wave * XPW + p) * 1024, ((uint32_t)((wave * XPW + p) * kbs) * 1024u + lane * 16) | past, rx,
+                     k * 1024);
+#pragma unroll
+        for (int p = 0; p < WPW; p++)
+            dma16_at(at + XB + (wave * WPW + p) * 1024,
+                     ((uint32_t)((wave * WPW + p) * kbs) * 1024u + lane * 16) | past, rw, k * 1024);
+#pragma unroll
+        for (int p = 0; p < SPW; p++) dma4_at(at + SB + panel[p] * 256, soff[p] | past, rs[p], k * 256);
+    };
+
+    struct Operands {
+        uint4_t w[NT], x[MT];
+        uint32_t sw[WW], sx[XW];
+    };
+    float4_t acc[NT][MT];
+#pragma unroll
+    for (int a = 0; a < NT; a++)
+#pragma unroll
+        for (int b = 0; b < MT; b++) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    const uint32_t own = group * PART, x0 = own + wm * TM * 64 + lane * 16, w0 = own + XB + wn * TN * 64 + lane * 16;
+    const uint32_t sx0 = own + SB + wm * TM / 64 * 256 + lane * 4, sw0 = own + SB + XP * 256 + wn * TN / 64 * 256 + lane * 4;
+    // where a wave's tiles are part of a panel, its first tile's byte moves to the front
+    const int xshift = TM < 64 ? (row0 + wm * TM) / 16 % 4 * 8 : 0, wshift = TN < 64 ? (col0 + wn * TN) / 16 % 4 * 8 : 0;
+    auto read_w = [&](const uint8_t *st, int a, Operands &o) { o.w[a] = *(const uint4_t *)(st + w0 + a * 1024); };
+    auto read_x = [&](const uint8_t *st, int b, Operands &o) { o.x[b] = *(const uint4_t *)(st + x0 + b * 1024); };
+    auto read_scales = [&](const uint8_t *st, Operands &o) {
+#pragma unroll
+        for (int i = 0; i < WW; i++) o.sw[i] = *(const uint32_t *)(st + sw0 + i * 256) >> wshift;
+#pragma unroll
+        for (int i = 0; i < XW; i++) o.sx[i] = *(const uint32_t *)(st + sx0 + i * 256) >> xshift;
+    };
+    // the products of one step, the next one's operands read among them
+    auto step = [&](const Operands &now, Operands &next, const uint8_t *st) {
+        read_scales(st, next);
+#pragma unroll
+        for (int a = 0; a < NT; a++) read_w(st, a, next);
+#pragma unroll
+        for (int b = 0; b < MT; b++) {
+            read_x(st, b, next);
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+                acc[a][b] = mx4_mfma_ab(a % 4, b % 4, now.w[a], now.sw[a / 4], now.x[b], now.sx[b / 4], acc[a][b]);
+        }
+    };
+
+    const int steps = (last - first + KS - 1) / KS;
+#pragma unroll
+    for (int p = 0; p < NS; p++) load_stage(p, p);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 1) * PB) : "memory");
+    Operands two[2];
+    read_scales(lds, two[0]);
+#pragma unroll
+    for (int a = 0; a < NT; a++) read_w(lds, a, two[0]);
+#pragma unroll
+    for (int b = 0; b < MT; b++) read_x(lds, b, two[0]);
+    int stage = 0;
+    auto advance = [&](int i, const Operands &now, Operands &next) {
+        // This wave's loads of step i + 1 are done once only the later steps' are left, and its reads of step i's
+        // stage at lgkmcnt(0); then the barrier covers every wave, and the stage takes step i + NS.
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
+        load_stage(stage, i + NS);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+        step(now, next, lds + stage * STAGE);
+    };
+    for (int i = 0; i < steps; i += 2) {
+        advance(i, two[0], two[1]);
+        if (i + 1 < steps) advance(i + 1, two[1], two[0]);
+    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight once the block goes on
+
+    if constexpr (KS > 1) {
+        float4_t *sums = (float4_t *)lds;  // [groups - 1][waves][tiles][64 lanes]
+        __syncthreads();
+        if (group > 0) {
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+#pragma unroll
+                for (int b = 0; b < MT; b++)
+                    sums[(((group - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane] = acc[a][b];
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int h = 1; h < KS; h++)
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+#pragma unroll
+                for (int b = 0; b < MT; b++) acc[a][b] += sums[(((h - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane];
+    }
+#pragma unroll
+    for (int b = 0; b < MT; b++) {
+        const int row = row0 + wm * TM + b * 16 + j;
+        if (row >= m) continue;
+#pragma unroll
+        for (int a = 0; a < NT; a++) {
+            const int col = col0 + wn * TN + a * 16 + 4 * g;
+            if (col < n) fp8_store4(y, dtype, ((size_t)split * m + row) * n + col, acc[a][b], n - col);
+        }
+    }
+}
+
+// What a product needs beside its operands: how its tile cuts k (`splits` runs of
+// blocks), and where the runs' sums go.
+struct Mx4Split {
+    int splits = 1;
+    float *part = nullptr;  // [splits][m][n]
+};
+
+template <int BM, int BN, int WGM, int WGN, int KS, int NS>
+void mx4_tile_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
+                     Mx4Split cut, hipStream_t s) {
+    const unsigned tiles = cdiv(m, BM) * cdiv(w->rows, BN);
+    const int per = (int)cdiv(w->kbs, cut.splits), splits = (int)cdiv(w->kbs, per);
+    hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, WGM, WGN, KS, NS>), dim3(tiles * splits), dim3(WGM * WGN * KS * 64), 0,
+                       s, w->codes, w->scales, w->rows, w->kbs, q, sx, m, splits > 1 ? cut.part : y,
+                       splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, per);
+    if (splits > 1) launch_fp8_join(cut.part, splits, (size_t)m * w->rows, y, dtype, s);
+}
+
 void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
     const unsigned panels = cdiv(m, 64), most = 32768;  // a grid's y ends at 65535
@@ -182,11 +392,49 @@ void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uin
         hipLaunchKernelGGL(mx4_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx, bad);
 }
 
+// The tiles, in the order of the "mx4" family's variants from kTile0 on.
+struct Mx4Tile {
+    int bm, bn;
+};
+constexpr Mx4Tile kMx4Tiles[] = {{32, 32}, {64, 32}, {64, 64}, {64, 64}, {128, 128}, {256, 128}, {256, 256}};
+constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 7;
+
+struct Mx4Pick {
+    int variant, splits;
+};
+
+Mx4Pick mx4_pick(int variant, int m, int n, int kbs) {
+    if (variant) return {variant, 1};
+    if (m <= 16) return {1, 1};
+    if (m <= 32) return {2, 1};
+    const size_t cus = (size_t)device_cus();
+    for (int i = kTiles - 1; i > 0; i--)
+        if ((size_t)cdiv(m, kMx4Tiles[i].bm) * cdiv(n, kMx4Tiles[i].bn) >= cus) return {kTile0 + i, 1};
+    return {kTile0, 1};
+}
+
+// f32 values that a product of m rows needs for its runs' sums.
+size_t mx4_parts(const dz_mx4_weight *w, size_t m, int variant) {
+    const int splits = mx4_pick(variant, (int)m, w->rows, w->kbs).splits;
+    return splits > 1 ? splits * m * w->rows : 0;
+}
+
 // The product of m > 0 rows of codes.
 void launch_mx4_product(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
-                        hipStream_t s) {
-    if (m <= 16) mx4_rows_launch<1>(w, q, sx, m, y, dtype, s);
-    else mx4_rows_launch<4>(w, q, sx, m, y, dtype, s);
+                        int variant, float *part, hipStream_t s) {
+    const Mx4Pick pick = mx4_pick(variant, m, w->rows, w->kbs);
+    const Mx4Split cut{pick.splits, part};
+    switch (pick.variant) {
+        case 1: return mx4_rows_launch<1>(w, q, sx, m, y, dtype, s);
+        case 2: return mx4_rows_launch<2>(w, q, sx, m, y, dtype, s);
+        case 3: return mx4_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 4: return mx4_tile_launch<64, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 5: return mx4_tile_launch<64, 64, 2, 2, 4, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 6: return mx4_tile_launch<64, 64, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 7: return mx4_tile_launch<128, 128, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 8: return mx4_tile_launch<256, 128, 4, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
+        default: return mx4_tile_launch<256, 256, 2, 4, 1, 4>(w, q, sx, m, y, dtype, cut, s);
+    }
 }
 
 bool mx4_dtype(int32_t d) { return d == DZ_F32 || d == DZ_F16 || d == DZ_BF16; }
@@ -319,7 +567,12 @@ int32_t mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q, con
     if (m > kMx4MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (int32_t rc = mx4_codes_ok(ctx, q, s)) return rc;
     if (m == 0) return DZ_OK;
-    launch_mx4_product(w, q, s, (int)m, y, y_dtype, ctx_stream(ctx));
+    const int variant = ctx_variant(ctx, "mx4");
+    const size_t parts = mx4_parts(w, m, variant);
+    void *work = nullptr;
+    if (parts)
+        if (int32_t rc = ctx_workspace(ctx, parts * sizeof(float), &work)) return rc;
+    launch_mx4_product(w, q, s, (int)m, y, y_dtype, variant, (float *)work, ctx_stream(ctx));
     return ctx_launched(ctx, "mx4 linear");
 }
 
@@ -332,10 +585,11 @@ int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x
     if (m == 0) return DZ_OK;
     const size_t codes = whole(mx4_code_bytes(m, w->cols)), scales = whole(mx4_scale_bytes(m, w->cols));
     void *work = nullptr;
-    if (int32_t rc = ctx_workspace(ctx, codes + scales, &work)) return rc;
+    const int variant = ctx_variant(ctx, "mx4");
+    if (int32_t rc = ctx_workspace(ctx, codes + scales + mx4_parts(w, m, variant) * sizeof(float), &work)) return rc;
     uint8_t *q = (uint8_t *)work, *sx = q + codes;
     launch_mx4_quantize(x, x_dtype, (int)m, w->cols, q, sx, nullptr, ctx_stream(ctx));
-    launch_mx4_product(w, q, sx, (int)m, y, y_dtype, ctx_stream(ctx));
+    launch_mx4_product(w, q, sx, (int)m, y, y_dtype, variant, (float *)(sx + scales), ctx_stream(ctx));
     return ctx_launched(ctx, "mx4 linear");
 }
 

@@ -2526,6 +2526,8 @@ const char *const kDeltaNames[] = {"chunked64", "chunked64-c32", "recurrent", "r
 const char *const kNormNames[] = {"fused", "separate"};
 const char *const kFp8Names[] = {"auto",  "rows16",  "rows32",  "32x32k4", "64x32k4",
                                  "64x64k4", "64x64", "64x64k2", "128x128", "256x128", "256x256"};
+const char *const kMx4Names[] = {"auto",    "rows16",  "rows32",  "32x32k4", "64x32k4",
+                                 "64x64k4", "64x64k2", "128x128", "256x128", "256x256"};
 
 template <int W, int MPAD, bool G32, int NP>
 void gemv_launch_np(const Weight &w, const half_t *x, int m, float *y, hipStream_t s) {
@@ -2830,6 +2832,7 @@ int variant_count(const char *family) {
     if (f == "delta_scan") return 5;
     if (f == "norm") return 2;
     if (f == "fp8") return (int)(sizeof(kFp8Names) / sizeof(kFp8Names[0]));
+    if (f == "mx4") return (int)(sizeof(kMx4Names) / sizeof(kMx4Names[0]));
     return 0;
 }
 
@@ -2860,6 +2863,7 @@ const char *variant_name(const char *family, int index) {
     if (f == "delta_scan") return kDeltaNames[index];
     if (f == "norm") return kNormNames[index];
     if (f == "fp8") return kFp8Names[index];
+    if (f == "mx4") return kMx4Names[index];
     return nullptr;
 }
 

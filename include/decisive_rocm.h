@@ -801,8 +801,8 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
                 size_t cap);
 /* Forces a variant of a family by name (tests and benchmarks). Families and
  * variants (the first of each is the default; every variant of a family
- * gives the same bits, except the delta scan's two opt-ins and the "fp8" family
- * below):
+ * gives the same bits, except the delta scan's two opt-ins and the "fp8" and "mx4"
+ * families below):
  *   "gemv"        auto, w16, w8, stream8, stream4, persist (w16/w8: 16 or 8 waves
  *                 share one 16-row tile, each wave a fixed chunk of K; stream8/
  *                 stream4: one wave per tile, 8 or 4 tiles per block, for K a
@@ -856,7 +856,10 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *                 (tiles; k2 and k4 share the 128-blocks of k among two or four
  *                 groups of waves; f32 outputs of 256x256 take 256x128). For tests and benchmarks: "auto" picks by the
  *                 grid, dz_tune leaves it alone, and the variants add a row's blocks
- *                 in orders of their own, so their f32 sums agree to rounding */
+ *                 in orders of their own, so their f32 sums agree to rounding)
+ *   "mx4"         auto, rows16, rows32, 32x32k4, 64x32k4, 64x64k4, 64x64k2, 128x128,
+ *                 256x128, 256x256 (products on microscaled 4-bit floating point: as the
+ *                 "fp8" family's, and as little a tuner's matter) */
 int32_t dz_select_variant(dz_ctx *ctx, const char *family, const char *variant);
 
 #ifdef __cplusplus

@@ -213,6 +213,31 @@ def test_linear_against_64_bits(ctx, m, n, k, x_dtype):
     w.free()
 
 
+VARIANTS = ["rows16", "rows32", "32x32k4", "64x32k4", "64x64k4", "64x64k2", "128x128", "256x128", "256x256"]
+
+
+@pytest.mark.parametrize("variant", VARIANTS)
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (70, 131, 2600), (300, 70, 1111), (257, 513, 129), (33, 300, 5000)])
+def test_every_variant_against_64_bits(ctx, variant, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    w, wide = make_weight(ctx, rng, n, k)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    want, mags = product(values(*quantize(x), k), wide)
+    q, s = buffers(m, k)
+    q.fill_(0x77), s.fill_(255)  # what stands past the rows
+    ctx.mx4_quantize(dev(x), rocm.F32, m, k, q, s)
+    ctx.select_variant("mx4", variant)
+    try:
+        for y_dtype in DTYPES:
+            y = empty((m, n), _torch(y_dtype))
+            ctx.mx4_linear_q4(w, q, s, m, y, y_dtype)
+            ctx.sync()
+            check(f64(y), want, mags, k, y_dtype)
+    finally:
+        ctx.select_variant("mx4", "auto")
+    w.free()
+
+
 @pytest.mark.parametrize("x_dtype", DTYPES)
 @pytest.mark.parametrize("m", [1, 3, 20, 70, 300])
 def test_a_row_that_is_not_finite_makes_its_own_outputs_nan(ctx, m, x_dtype):

@@ -58,3 +58,22 @@ def test_the_rule_s_fields_are_the_header_s():
     named = re.findall(r"(int32_t|float) (\w+);", fields)
     kinds = {"int32_t": ctypes.c_int32, "float": ctypes.c_float}
     assert [(name, kinds[kind]) for kind, name in named] == list(rocm.MoeSelection._fields_)
+
+
+def test_the_header_lists_every_variant():
+    header = (ROOT / "include" / "decisive_rocm.h").read_text()
+    source = (ROOT / "decisive_amd" / "csrc" / "products.hip").read_text()
+    names = re.findall(r'"([^"]+)"', re.search(r"kMx4Names\[\] = \{(.*?)\};", source, re.S).group(1))
+    listed = re.search(r'\n \*   "mx4" (.*?)\*/', header, re.S).group(1)
+    assert names and not set(names) - set(re.findall(r"[\w-]+", listed))
+
+
+def test_barriers_between_stages_wait_for_loads_and_reads():
+    """Stages filled by DMA: before a barrier after which one is loaded again, this wave's loads and its reads are waited
+    for in the same statement, since the compiler's own waits see neither."""
+    source = (ROOT / "decisive_amd" / "csrc" / "mx4.hip").read_text()
+    found = [a for a in re.findall(r"asm volatile\(\s*((?:\"[^\"]*\"\s*)+)", source) if "s_barrier" in a]
+    assert len(found) >= 2
+    for text in found:
+        wait = text.split("s_barrier")[0]
+        assert re.search(r"vmcnt\((%0|0)\)", wait) and "lgkmcnt(0)" in wait, text
