@@ -199,6 +199,27 @@ __device__ __forceinline__ float4_t mx4_mfma_ab(int ua, int ub, uint4_t a, uint3
     return mx4_mfma_b<3>(ub, a, sa, b, sb, c);
 }
 
+// Eight consecutive outputs of a 16-bit type at element `at`, `left` of them inside the row.
+__device__ __forceinline__ void mx4_store8(void *__restrict__ y, size_t at, uint4_t w, int left) {
+    if (left >= 8) {
+        *(uint4_any_t *)((uint16_t *)y + at) = w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 7; e++)
+            if (e < left) ((uint16_t *)y)[at + e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
+    }
+}
+
+// Four values rounded once to f16 (dtype 1) or bf16.
+__device__ __forceinline__ uint2_t mx4_round4(float4_t v, int dtype) {
+    if (dtype == 1) {
+        const half2_t a = {(half_t)v[0], (half_t)v[1]}, b = {(half_t)v[2], (half_t)v[3]};
+        return uint2_t{half2_as_word(a), half2_as_word(b)};
+    }
+    const bf16x2_t a = {(bf16_t)v[0], (bf16_t)v[1]}, b = {(bf16_t)v[2], (bf16_t)v[3]};
+    return uint2_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
 // Block tile BM x BN (activation rows x weight rows). KS groups of WGM x WGN
 // waves each take every KS-th 128-block of k; a step is KS blocks, one a group, in
 // one of NS LDS stages that buffer_load ... lds fills, chunks and scale words as they
@@ -206,16 +227,18 @@ __device__ __forceinline__ float4_t mx4_mfma_ab(int ua, int ub, uint4_t a, uint3
 // lanes' reads meet in a bank. A wave reads the operands of step i + 1 while it
 // multiplies step i's, so that its products wait for no read; a stage is free once its
 // operands are in registers, a step before it is multiplied, and NS - 1 steps' loads
-// are in flight. Scales cost nothing: the matrix unit adds the exponents. The groups'
-// sums are added in group order, through LDS. Where k is cut, workgroup b / tiles takes
-// `per` of its blocks and writes their sums as f32 for fp8_join.
+// are in flight. With KS = 1 a workgroup goes through several tiles, and the loads run
+// on into the next one while a tile's outputs are stored. Scales cost nothing: the matrix
+// unit adds the exponents. The groups' sums are added in group order, through LDS.
+// Where k is cut, unit b / tiles takes `per` of its blocks and writes their sums as f32
+// for fp8_join.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const uint8_t *__restrict__ scales, int n, int kbs,
                                                                      const uint8_t *__restrict__ q,
                                                                      const uint8_t *__restrict__ sx, int m,
                                                                      void *__restrict__ y, int dtype, int tiles,
-                                                                     int per) {
+                                                                     int units, int per) {
     constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
     constexpr int XPW = BM / 16 / WAVES, WPW = BN / 16 / WAVES;            // 1 KiB loads per wave and stage
     constexpr int XP = BM < 64 ? 1 : BM / 64, WP = BN < 64 ? 1 : BN / 64;  // panels of scale words
@@ -224,6 +247,8 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
     constexpr int XB = BM * 64, SB = XB + BN * 64, PART = SB + (XP + WP) * 256, STAGE = KS * PART;
     static_assert(XPW * 16 * WAVES == BM && WPW * 16 * WAVES == BN, "whole loads for each wave");
     static_assert((TM % 64 == 0 || 64 % TM == 0) && (TN % 64 == 0 || 64 % TN == 0), "scale words of whole or one panel");
+    static_assert(NS % 2 == 0, "two steps a turn");
+    static_assert(NT % 2 == 0, "pairs of column tiles are stored together");
     static_assert((NS - 1) * PB <= 63, "vmcnt range");
     static_assert((KS - 1) * BM * BN * 4 <= NS * STAGE, "the groups' sums fit the stages");
     __shared__ __align__(16) uint8_t lds[NS * STAGE];
@@ -232,83 +257,94 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
     const int group = wave_all / WAVES, wave = wave_all % WAVES;
     const int wm = wave / WGN, wn = wave % WGN, g = lane / 16, j = lane % 16;
     const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
-    int tm, tn;
-    const int split = blockIdx.x / tiles, first = split * per, last = min(kbs, first + per);  // its blocks of k
-    xcd_tile(blockIdx.x - split * tiles, tiles, tiles_m, tiles_n, tm, tn);
-    const int row0 = tm * BM, col0 = tn * BN;
-    const int have_x = min(BM / 16, (m + 15) / 16 - row0 / 16), have_w = min(BN / 16, (n + 15) / 16 - col0 / 16);
-    const int panels_x = min(XP, (m + 63) / 64 - row0 / 64), panels_w = min(WP, (n + 63) / 64 - col0 / 64);
-    const int32x4_t rx = buffer_rsrc(q + (size_t)(row0 / 16) * kbs * 1024, (uint32_t)(have_x * kbs) * 1024u);
-    const int32x4_t rw = buffer_rsrc(codes + (size_t)(col0 / 16) * kbs * 1024, (uint32_t)(have_w * kbs) * 1024u);
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + group * PART;
-    // this wave's panels of scale words (some load one twice, so that all waits go by count)
-    int panel[SPW];
-    int32x4_t rs[SPW];
+
+    // A unit of work: a tile and a run of its blocks of k.
+    struct Unit {
+        int split, row0, col0, first, last, steps;
+    };
+    auto unit_of = [&](int id) {
+        Unit u;
+        int tm, tn;
+        u.split = __builtin_amdgcn_readfirstlane(id / tiles);  // divisions leave uniform values in vector registers
+        u.first = u.split * per;
+        u.last = min(kbs, u.first + per);
+        // the operands change places every step, and the loads are NS steps ahead; steps past the last add nothing
+        u.steps = max(NS, (u.last - u.first + 2 * KS - 1) / (2 * KS) * 2);
+        xcd_tile(id - u.split * tiles, tiles, tiles_m, tiles_n, tm, tn);
+        u.row0 = __builtin_amdgcn_readfirstlane(tm) * BM;
+        u.col0 = __builtin_amdgcn_readfirstlane(tn) * BN;
+        return u;
+    };
+
+    // The loads run NS steps ahead of the products: their own unit and step, and what they read of it. Units past the
+    // last one, and blocks past a unit's last, load nothing (every offset out of range, zeros in LDS).
+    int load_id = blockIdx.x, load_step = 0;
+    Unit load = unit_of(load_id);
+    int32x4_t rx, rw, rs[SPW];
+    int panel[SPW];  // this wave's panels of scale words (some load one twice, so that all waits go by count)
     uint32_t soff[SPW];
 #pragma unroll
     for (int p = 0; p < SPW; p++) {
         panel[p] = (wave * SPW + p) % (XP + WP);
-        const bool of_x = panel[p] < XP;
-        rs[p] = of_x ? buffer_rsrc(sx + (size_t)(row0 / 64) * kbs * 256, (uint32_t)(panels_x * kbs) * 256u)
-                     : buffer_rsrc(scales + (size_t)(col0 / 64) * kbs * 256, (uint32_t)(panels_w * kbs) * 256u);
-        soff[p] = (uint32_t)(of_x ? panel[p] : panel[p] - XP) * kbs * 256 + lane * 4;
+        soff[p] = (uint32_t)(panel[p] < XP ? panel[p] : panel[p] - XP) * kbs * 256 + lane * 4;
     }
-
-    // Blocks past the last one load nothing (every offset out of range, zeros in LDS).
-    auto load_stage = [&](int stage, int step) {
-        const int kb = first + step * KS + group;
-        const bool live = kb < last;
+    auto open_unit = [&] {
+        const int have_x = min(BM / 16, (m + 15) / 16 - load.row0 / 16), have_w = min(BN / 16, (n + 15) / 16 - load.col0 / 16);
+        const int panels_x = min(XP, (m + 63) / 64 - load.row0 / 64), panels_w = min(WP, (n + 63) / 64 - load.col0 / 64);
+        rx = buffer_rsrc(q + (size_t)(load.row0 / 16) * kbs * 1024, (uint32_t)(have_x * kbs) * 1024u);
+        rw = buffer_rsrc(codes + (size_t)(load.col0 / 16) * kbs * 1024, (uint32_t)(have_w * kbs) * 1024u);
+#pragma unroll
+        for (int p = 0; p < SPW; p++)
+            rs[p] = panel[p] < XP
+                        ? buffer_rsrc(sx + (size_t)(load.row0 / 64) * kbs * 256, (uint32_t)(panels_x * kbs) * 256u)
+                        : buffer_rsrc(scales + (size_t)(load.col0 / 64) * kbs * 256, (uint32_t)(panels_w * kbs) * 256u);
+    };
+    open_unit();
+    // Load p of a stage's PB.
+    auto load_piece = [&](int stage, int p) {
+        const int kb = load.first + load_step * KS + group;
+        const bool live = load_id < units && kb < load.last;
         const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u, k = live ? (uint32_t)kb : 0u;
-#pragma unroll
-        for (int p = 0; p < XPW; p++)
-            dma16_at(at + (wave * XPW + p) * 1024, ((uint32_t)((wave * XPW + p) * kbs) * 1024u + lane * 16) | past, rx,
-                     k * 1024);
-#pragma unroll
-        for (int p = 0; p < WPW; p++)
-            dma16_at(at + XB + (wave * WPW + p) * 1024,
-                     ((uint32_t)((wave * WPW + p) * kbs) * 1024u + lane * 16) | past, rw, k * 1024);
-#pragma unroll
-        for (int p = 0; p < SPW; p++) dma4_at(at + SB + panel[p] * 256, soff[p] | past, rs[p], k * 256);
-    };
-
-    struct Operands {
-        uint4_t w[NT], x[MT];
-        uint32_t sw[WW], sx[XW];
-    };
-    float4_t acc[NT][MT];
-#pragma unroll
-    for (int a = 0; a < NT; a++)
-#pragma unroll
-        for (int b = 0; b < MT; b++) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
-    const uint32_t own = group * PART, x0 = own + wm * TM * 64 + lane * 16, w0 = own + XB + wn * TN * 64 + lane * 16;
-    const uint32_t sx0 = own + SB + wm * TM / 64 * 256 + lane * 4, sw0 = own + SB + XP * 256 + wn * TN / 64 * 256 + lane * 4;
-    // where a wave's tiles are part of a panel, its first tile's byte moves to the front
-    const int xshift = TM < 64 ? (row0 + wm * TM) / 16 % 4 * 8 : 0, wshift = TN < 64 ? (col0 + wn * TN) / 16 % 4 * 8 : 0;
-    auto read_w = [&](const uint8_t *st, int a, Operands &o) { o.w[a] = *(const uint4_t *)(st + w0 + a * 1024); };
-    auto read_x = [&](const uint8_t *st, int b, Operands &o) { o.x[b] = *(const uint4_t *)(st + x0 + b * 1024); };
-    auto read_scales = [&](const uint8_t *st, Operands &o) {
-#pragma unroll
-        for (int i = 0; i < WW; i++) o.sw[i] = *(const uint32_t *)(st + sw0 + i * 256) >> wshift;
-#pragma unroll
-        for (int i = 0; i < XW; i++) o.sx[i] = *(const uint32_t *)(st + sx0 + i * 256) >> xshift;
-    };
-    // the products of one step, the next one's operands read among them
-    auto step = [&](const Operands &now, Operands &next, const uint8_t *st) {
-        read_scales(st, next);
-#pragma unroll
-        for (int a = 0; a < NT; a++) read_w(st, a, next);
-#pragma unroll
-        for (int b = 0; b < MT; b++) {
-            read_x(st, b, next);
-#pragma unroll
-            for (int a = 0; a < NT; a++)
-                acc[a][b] = mx4_mfma_ab(a % 4, b % 4, now.w[a], now.sw[a / 4], now.x[b], now.sx[b / 4], acc[a][b]);
+        if (p < XPW) {
+            const int u = wave * XPW + p;
+            dma16_at(at + u * 1024, ((uint32_t)(u * kbs) * 1024u + lane * 16) | past, rx, k * 1024);
+        } else if (p < XPW + WPW) {
+            const int u = wave * WPW + p - XPW;
+            dma16_at(at + XB + u * 1024, ((uint32_t)(u * kbs) * 1024u + lane * 16) | past, rw, k * 1024);
+        } else {
+            const int u = p - XPW - WPW;
+            dma4_at(at + SB + panel[u] * 256, soff[u] | past, rs[u], k * 256);
         }
     };
-
-    const int steps = (last - first + KS - 1) / KS;
+    // The weight's operands, the scale words and the last XD row tiles of x are held for two steps; a register of the
+    // other row tiles takes the next step's operand once its products are under way.
+    constexpr int XD = MT >= 4 ? MT / 4 : 1, XH = MT - XD;
+    struct Operands {
+        uint4_t w[NT], x[XD];
+        uint32_t sw[WW], sx[XW];
+    };
+    uint4_t head[XH > 0 ? XH : 1];
+    float4_t acc[NT][MT];
+    const uint32_t own = group * PART, x0 = own + wm * TM * 64 + lane * 16, w0 = own + XB + wn * TN * 64 + lane * 16;
+    const uint32_t sx0 = own + SB + wm * TM / 64 * 256 + lane * 4, sw0 = own + SB + XP * 256 + wn * TN / 64 * 256 + lane * 4;
+    auto read_w = [&](const uint8_t *st, int a, Operands &o) { o.w[a] = *(const uint4_t *)(st + w0 + a * 1024); };
+    auto read_x = [&](const uint8_t *st, int b, Operands &o) {
+        (b < XH ? head[b < XH ? b : 0] : o.x[b < XH ? 0 : b - XH]) = *(const uint4_t *)(st + x0 + b * 1024);
+    };
+    auto read_scales = [&](const uint8_t *st, Operands &o) {
 #pragma unroll
-    for (int p = 0; p < NS; p++) load_stage(p, p);
+        for (int i = 0; i < WW; i++) o.sw[i] = *(const uint32_t *)(st + sw0 + i * 256);
+#pragma unroll
+        for (int i = 0; i < XW; i++) o.sx[i] = *(const uint32_t *)(st + sx0 + i * 256);
+    };
+
+#pragma unroll
+    for (int i = 0; i < NS; i++) {
+#pragma unroll
+        for (int p = 0; p < PB; p++) load_piece(i, p);
+        load_step++;
+    }
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 1) * PB) : "memory");
     Operands two[2];
     read_scales(lds, two[0]);
@@ -317,49 +353,119 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
 #pragma unroll
     for (int b = 0; b < MT; b++) read_x(lds, b, two[0]);
     int stage = 0;
-    auto advance = [&](int i, const Operands &now, Operands &next) {
-        // This wave's loads of step i + 1 are done once only the later steps' are left, and its reads of step i's
-        // stage at lgkmcnt(0); then the barrier covers every wave, and the stage takes step i + NS.
+    // where a wave's tiles are part of a panel, its first tile's byte is not the word's first
+    int xshift = 0, wshift = 0;
+    // The products of a step, the next one's operands read and the loads of the step NS further issued among them, in
+    // this order: left to itself the compiler moves the reads to where they are used.
+    auto advance = [&](const Operands &now, Operands &next) {
+        // This wave's loads of the next step are done once only the later steps' are left (stores among them are
+        // waited for too early, never too late), and its reads of this step's stage at lgkmcnt(0); then the barrier
+        // covers every wave, and the stage is free.
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * PB) : "memory");
-        load_stage(stage, i + NS);
+        const int free_stage = stage;
         stage = stage + 1 == NS ? 0 : stage + 1;
-        step(now, next, lds + stage * STAGE);
+        const uint8_t *st = lds + stage * STAGE;
+        uint32_t sw[WW], sxw[XW];
+#pragma unroll
+        for (int i = 0; i < WW; i++) sw[i] = TN < 64 ? now.sw[i] >> wshift : now.sw[i];
+#pragma unroll
+        for (int i = 0; i < XW; i++) sxw[i] = TM < 64 ? now.sx[i] >> xshift : now.sx[i];
+        constexpr int G = MT > 1 ? MT - 1 : 1;  // groups of products with loads and reads after them
+#pragma unroll
+        for (int b = 0; b < MT; b++) {
+#pragma unroll
+            for (int a = 0; a < NT; a++)
+                acc[a][b] = mx4_mfma_ab(a % 4, b % 4, now.w[a], sw[a / 4], b < XH ? head[b < XH ? b : 0] : now.x[b < XH ? 0 : b - XH],
+                                        sxw[b / 4], acc[a][b]);
+            __builtin_amdgcn_sched_barrier(0);
+            // row tile b's next operand; and, spread over the groups before the last, scales, x's last tiles and w
+            if (b < XH) read_x(st, b, next);
+            constexpr int READS = 1 + XD + NT;
+#pragma unroll
+            for (int r = 0; r < READS; r++) {
+                if (r * G / READS != b) continue;
+                if (r == 0) read_scales(st, next);
+                else if (r <= XD) read_x(st, XH + r - 1, next);
+                else read_w(st, r - 1 - XD, next);
+            }
+#pragma unroll
+            for (int p = 0; p < PB; p++)
+                if (p * G / PB == b) load_piece(free_stage, p);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        load_step++;
     };
-    for (int i = 0; i < steps; i += 2) {
-        advance(i, two[0], two[1]);
-        if (i + 1 < steps) advance(i + 1, two[1], two[0]);
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight once the block goes on
 
-    if constexpr (KS > 1) {
-        float4_t *sums = (float4_t *)lds;  // [groups - 1][waves][tiles][64 lanes]
-        __syncthreads();
-        if (group > 0) {
+    for (int id = blockIdx.x; id < units; id += gridDim.x) {
+        const Unit u = unit_of(id);
+        if (TM < 64) xshift = (u.row0 + wm * TM) / 16 % 4 * 8;
+        if (TN < 64) wshift = (u.col0 + wn * TN) / 16 % 4 * 8;
 #pragma unroll
-            for (int a = 0; a < NT; a++)
+        for (int a = 0; a < NT; a++)
 #pragma unroll
-                for (int b = 0; b < MT; b++)
-                    sums[(((group - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane] = acc[a][b];
+            for (int b = 0; b < MT; b++) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int part = 0; part < 2; part++) {  // the last NS steps load the next unit's first
+            for (int i = part == 0 ? NS : 0; i < (part == 0 ? u.steps : NS); i += 2) {
+                advance(two[0], two[1]);
+                advance(two[1], two[0]);
+            }
+            if (part == 1) break;
+            load_step = 0;
+            load_id += gridDim.x;
+            if (load_id < units) {
+                load = unit_of(load_id);
+                open_unit();
+            }
         }
-        __syncthreads();
-        if (group > 0) return;
+
+        if constexpr (KS > 1) {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight
+            float4_t *sums = (float4_t *)lds;                            // [groups - 1][waves][tiles][64 lanes]
+            __syncthreads();
+            if (group > 0) {
 #pragma unroll
-        for (int h = 1; h < KS; h++)
+                for (int a = 0; a < NT; a++)
 #pragma unroll
-            for (int a = 0; a < NT; a++)
+                    for (int b = 0; b < MT; b++)
+                        sums[(((group - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane] = acc[a][b];
+            }
+            __syncthreads();
+            if (group > 0) return;
 #pragma unroll
-                for (int b = 0; b < MT; b++) acc[a][b] += sums[(((h - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane];
-    }
+            for (int h = 1; h < KS; h++)
 #pragma unroll
-    for (int b = 0; b < MT; b++) {
-        const int row = row0 + wm * TM + b * 16 + j;
-        if (row >= m) continue;
+                for (int a = 0; a < NT; a++)
 #pragma unroll
-        for (int a = 0; a < NT; a++) {
-            const int col = col0 + wn * TN + a * 16 + 4 * g;
-            if (col < n) fp8_store4(y, dtype, ((size_t)split * m + row) * n + col, acc[a][b], n - col);
+                    for (int b = 0; b < MT; b++)
+                        acc[a][b] += sums[(((h - 1) * WAVES + wave) * NT * MT + a * MT + b) * 64 + lane];
+        }
+        // A lane holds row j's columns 4 g .. 4 g + 3 of each tile: 16 bytes in f32. Of 16-bit outputs two column
+        // tiles change lanes (odd rows of 16 lanes of the one with even rows of the other), so that a lane stores
+        // eight columns of one tile, 64 bytes of a row together.
+#pragma unroll
+        for (int b = 0; b < MT; b++) {
+            const int row = u.row0 + wm * TM + b * 16 + j;
+            const size_t line = ((size_t)u.split * m + row) * n;
+            if (dtype == 0) {
+                if (row >= m) continue;
+#pragma unroll
+                for (int a = 0; a < NT; a++) {
+                    const int col = u.col0 + wn * TN + a * 16 + 4 * g;
+                    if (col < n) fp8_store4(y, 0, line + col, acc[a][b], n - col);
+                }
+            } else {
+#pragma unroll
+                for (int a = 0; a < NT; a += 2) {
+                    const uint2_t v = mx4_round4(acc[a][b], dtype), w = mx4_round4(acc[a + 1][b], dtype);
+                    const uint2_t lo = __builtin_bit_cast(uint2_t, __builtin_amdgcn_permlane16_swap(v[0], w[0], false, false));
+                    const uint2_t hi = __builtin_bit_cast(uint2_t, __builtin_amdgcn_permlane16_swap(v[1], w[1], false, false));
+                    const int col = u.col0 + wn * TN + (a + g % 2) * 16 + g / 2 * 8;
+                    if (row < m && col < n) mx4_store8(y, line + col, uint4_t{lo[0], hi[0], lo[1], hi[1]}, n - col);
+                }
+            }
         }
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight when the block ends
 }
 
 // What a product needs beside its operands: how its tile cuts k (`splits` runs of
@@ -374,9 +480,10 @@ void mx4_tile_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx
                      Mx4Split cut, hipStream_t s) {
     const unsigned tiles = cdiv(m, BM) * cdiv(w->rows, BN);
     const int per = (int)cdiv(w->kbs, cut.splits), splits = (int)cdiv(w->kbs, per);
-    hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, WGM, WGN, KS, NS>), dim3(tiles * splits), dim3(WGM * WGN * KS * 64), 0,
-                       s, w->codes, w->scales, w->rows, w->kbs, q, sx, m, splits > 1 ? cut.part : y,
-                       splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, per);
+    const unsigned units = tiles * splits, most = (unsigned)device_cus();
+    hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, WGM, WGN, KS, NS>), dim3(KS == 1 ? std::min(units, most) : units),
+                       dim3(WGM * WGN * KS * 64), 0, s, w->codes, w->scales, w->rows, w->kbs, q, sx, m,
+                       splits > 1 ? (void *)cut.part : y, splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, (int)units, per);
     if (splits > 1) launch_fp8_join(cut.part, splits, (size_t)m * w->rows, y, dtype, s);
 }
 
