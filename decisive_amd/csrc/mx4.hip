@@ -117,45 +117,88 @@ __device__ __forceinline__ float4_t mx4_mfma(uint4_t a, uint32_t sa, uint4_t b, 
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(va, vb, c, 4, 4, UA, (int)sa, UB, (int)sb);
 }
 
-// A workgroup owns 16 weight rows and 16 MB activation rows. Its waves take runs of
-// the k-blocks, operands straight from memory, and their f32 partials are added in
-// wave order, from LDS. The matrix unit's operands are swapped (weight first), so a
-// lane holds one activation row and four output columns.
-constexpr int kMx4Waves = 8;
+// A workgroup owns 16 NT weight rows (NT tiles) and up to 16 activation rows. Its
+// waves take runs of the k-blocks, four of them at a time, operands straight from
+// memory, and their f32 partials are added in wave order, from LDS. The matrix unit's
+// operands are swapped (weight first), so a lane holds one activation row and four
+// output columns. x comes as codes (ROWS = 0) or, a few rows, as it is: then a wave
+// quantizes its own blocks while their weights are on the way, four 128-blocks of a row
+// at once, eight values a lane as mx4_quantize_kernel does, and hands the codes to its
+// lanes as operands through LDS, which spares a launch. The same bits either way.
+constexpr int kMx4Waves = 8, kMx4Batch = 4;
 
-template <int MB>
+template <class T, int ROWS, int NT>
 __global__ __launch_bounds__(kMx4Waves * 64) void mx4_rows_kernel(const uint8_t *__restrict__ codes,
                                                                   const uint8_t *__restrict__ scales, int n, int kbs,
-                                                                  const uint8_t *__restrict__ q,
-                                                                  const uint8_t *__restrict__ sx, int m,
+                                                                  const void *__restrict__ x,
+                                                                  const uint8_t *__restrict__ sx, int m, int k,
                                                                   void *__restrict__ y, int dtype) {
-    __shared__ __align__(16) float part[kMx4Waves][MB * 256];
+    constexpr bool RAW = ROWS > 0;
+    __shared__ __align__(16) float part[kMx4Waves][NT * 256];
+    __shared__ __align__(16) uint32_t s_codes[RAW ? kMx4Waves : 1][RAW ? ROWS : 1][kMx4Batch * 16];
+    __shared__ uint32_t s_scale[RAW ? kMx4Waves : 1][RAW ? ROWS : 1][kMx4Batch * 4];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
     const int g = lane / 16, j = lane % 16;
-    const int tiles = (n + 15) / 16, t = blockIdx.x % tiles, row0 = blockIdx.x / tiles * 16 * MB;
-    const uint8_t *w = codes + (size_t)t * kbs * 1024 + lane * 16;
-    const uint8_t *ws = scales + (size_t)(t / 4) * kbs * 256 + lane * 4 + t % 4;
-    float4_t acc[MB];
+    const int tiles = (n + 15) / 16, groups = (tiles + NT - 1) / NT, t0 = blockIdx.x % groups * NT;
+    const int row0 = blockIdx.x / groups * 16;
+    float4_t acc[NT];
 #pragma unroll
-    for (int b = 0; b < MB; b++) acc[b] = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < NT; t++) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
     const int first = (int)((int64_t)kbs * wave / kMx4Waves), last = (int)((int64_t)kbs * (wave + 1) / kMx4Waves);
-    for (int kb = first; kb < last; kb++) {
-        const uint4_t a = __builtin_nontemporal_load((const uint4_t *)(w + (size_t)kb * 1024));
-        const uint32_t sa = ws[(size_t)kb * 256];
+    for (int kb0 = first; kb0 < last; kb0 += kMx4Batch) {
+        uint4_t w[NT][kMx4Batch], v[kMx4Batch];
+        uint32_t sw[NT][kMx4Batch], sv[kMx4Batch];
 #pragma unroll
-        for (int b = 0; b < MB; b++) {
-            const int tile = row0 / 16 + b;
-            if (tile * 16 >= m) break;
-            const uint4_t v = *(const uint4_t *)(q + ((size_t)tile * kbs + kb) * 1024 + lane * 16);
-            const uint32_t sb = sx[((size_t)(tile / 4) * kbs + kb) * 256 + lane * 4 + tile % 4];
-            acc[b] = mx4_mfma<0, 0>(a, sa, v, sb, acc[b]);
+        for (int t = 0; t < NT; t++) {
+            const int tile = min(t0 + t, tiles - 1);
+#pragma unroll
+            for (int i = 0; i < kMx4Batch; i++) {
+                const int kb = min(kb0 + i, last - 1);
+                w[t][i] = __builtin_nontemporal_load((const uint4_t *)(codes + ((size_t)tile * kbs + kb) * 1024 + lane * 16));
+                sw[t][i] = scales[((size_t)(tile / 4) * kbs + kb) * 256 + lane * 4 + tile % 4];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the weight is under way before x is waited for
+        if constexpr (RAW) {
+            float some[ROWS][8];
+#pragma unroll
+            for (int r = 0; r < ROWS; r++)
+                fp8_load8((const T *)x + (size_t)min(r, m - 1) * k, kb0 * 128 + lane * 8, k, some[r]);
+#pragma unroll
+            for (int r = 0; r < ROWS; r++) {
+                uint32_t scale;
+                s_codes[wave][r][lane] = mx4_quantize8(some[r], scale);
+                if (lane % 4 == 0) s_scale[wave][r][lane / 4] = scale;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const int r = min(j, m - 1);  // rows past the last one multiply that row again
+#pragma unroll
+            for (int i = 0; i < kMx4Batch; i++) {
+                v[i] = *(const uint4_t *)&s_codes[wave][r][(i * 4 + g) * 4];
+                sv[i] = s_scale[wave][r][i * 4 + g];
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // read before the next batch is written
+        } else {
+#pragma unroll
+            for (int i = 0; i < kMx4Batch; i++) {
+                const int kb = min(kb0 + i, last - 1);
+                v[i] = *(const uint4_t *)((const uint8_t *)x + ((size_t)(row0 / 16) * kbs + kb) * 1024 + lane * 16);
+                sv[i] = sx[((size_t)(row0 / 64) * kbs + kb) * 256 + lane * 4 + row0 / 16 % 4];
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kMx4Batch; i++) {
+            if (kb0 + i >= last) break;
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[t] = mx4_mfma<0, 0>(w[t][i], sw[t][i], v[i], sv[i], acc[t]);
         }
     }
 #pragma unroll
-    for (int b = 0; b < MB; b++) *(float4_t *)&part[wave][(b * 16 + j) * 16 + 4 * g] = acc[b];
+    for (int t = 0; t < NT; t++) *(float4_t *)&part[wave][(t * 16 + j) * 16 + 4 * g] = acc[t];
     __syncthreads();
-    for (int i = threadIdx.x; i < MB * 256; i += kMx4Waves * 64) {
-        const int row = row0 + i / 16, col = t * 16 + i % 16;
+    for (int i = threadIdx.x; i < NT * 256; i += kMx4Waves * 64) {
+        const int row = row0 + i / 16 % 16, col = (t0 + i / 256) * 16 + i % 16;
         if (row >= m || col >= n) continue;
         float v = part[0][i];
 #pragma unroll
@@ -164,11 +207,27 @@ __global__ __launch_bounds__(kMx4Waves * 64) void mx4_rows_kernel(const uint8_t 
     }
 }
 
-template <int MB>
+template <class T, int ROWS, int NT>
+void mx4_rows_form(const dz_mx4_weight *w, const void *x, const uint8_t *sx, int m, void *y, int dtype, hipStream_t s) {
+    hipLaunchKernelGGL((mx4_rows_kernel<T, ROWS, NT>), dim3(cdiv(cdiv(w->rows, 16), NT) * cdiv(m, 16)),
+                       dim3(kMx4Waves * 64), 0, s, w->codes, w->scales, w->rows, w->kbs, x, sx, m, w->cols, y, dtype);
+}
+
+// Four tiles a workgroup past four a compute unit, where a workgroup with one has too little to read (us, one / four:
+// 16 rows, K=1024, N=32000 in f32 5.7 / 4.4; K=4096, N=14336 7.7 / 8.2; K=N=4096 3.4 / 5.2).
+bool mx4_many_tiles(const dz_mx4_weight *w) { return cdiv(w->rows, 16) > 4u * (unsigned)device_cus(); }
+
 void mx4_rows_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
                      hipStream_t s) {
-    hipLaunchKernelGGL(mx4_rows_kernel<MB>, dim3(cdiv(w->rows, 16) * cdiv(m, 16 * MB)), dim3(kMx4Waves * 64), 0, s,
-                       w->codes, w->scales, w->rows, w->kbs, q, sx, m, y, dtype);
+    if (mx4_many_tiles(w)) mx4_rows_form<void, 0, 4>(w, q, sx, m, y, dtype, s);
+    else mx4_rows_form<void, 0, 1>(w, q, sx, m, y, dtype, s);
+}
+
+template <class T>
+void mx4_raw_launch(const dz_mx4_weight *w, const void *x, int m, void *y, int dtype, hipStream_t s) {
+    if (m == 1) mx4_rows_form<T, 1, 1>(w, x, nullptr, m, y, dtype, s);
+    else if (m == 2) mx4_rows_form<T, 2, 1>(w, x, nullptr, m, y, dtype, s);
+    else mx4_rows_form<T, 4, 1>(w, x, nullptr, m, y, dtype, s);
 }
 
 // ---- products: tiles over many rows ----------------------------------------------
@@ -504,7 +563,7 @@ struct Mx4Tile {
     int bm, bn;
 };
 constexpr Mx4Tile kMx4Tiles[] = {{32, 32}, {64, 32}, {64, 64}, {64, 64}, {128, 128}, {256, 128}, {256, 256}};
-constexpr int kRowsVariants = 2, kTile0 = 1 + kRowsVariants, kTiles = 7;
+constexpr int kRowsVariants = 1, kTile0 = 1 + kRowsVariants, kTiles = 7;
 
 struct Mx4Pick {
     int variant, splits;
@@ -513,7 +572,6 @@ struct Mx4Pick {
 Mx4Pick mx4_pick(int variant, int m, int n, int kbs) {
     if (variant) return {variant, 1};
     if (m <= 16) return {1, 1};
-    if (m <= 32) return {2, 1};
     const size_t cus = (size_t)device_cus();
     for (int i = kTiles - 1; i > 0; i--)
         if ((size_t)cdiv(m, kMx4Tiles[i].bm) * cdiv(n, kMx4Tiles[i].bn) >= cus) return {kTile0 + i, 1};
@@ -532,14 +590,13 @@ void launch_mx4_product(const dz_mx4_weight *w, const uint8_t *q, const uint8_t 
     const Mx4Pick pick = mx4_pick(variant, m, w->rows, w->kbs);
     const Mx4Split cut{pick.splits, part};
     switch (pick.variant) {
-        case 1: return mx4_rows_launch<1>(w, q, sx, m, y, dtype, s);
-        case 2: return mx4_rows_launch<2>(w, q, sx, m, y, dtype, s);
-        case 3: return mx4_tile_launch<32, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 4: return mx4_tile_launch<64, 32, 2, 1, 4, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 5: return mx4_tile_launch<64, 64, 2, 2, 4, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 6: return mx4_tile_launch<64, 64, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 7: return mx4_tile_launch<128, 128, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 8: return mx4_tile_launch<256, 128, 4, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 1: return mx4_rows_launch(w, q, sx, m, y, dtype, s);
+        case 2: return mx4_tile_launch<32, 32, 2, 1, 4, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 3: return mx4_tile_launch<64, 32, 2, 1, 4, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 4: return mx4_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, cut, s);
+        case 5: return mx4_tile_launch<64, 64, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 6: return mx4_tile_launch<128, 128, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
+        case 7: return mx4_tile_launch<256, 128, 4, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
         default: return mx4_tile_launch<256, 256, 2, 4, 1, 4>(w, q, sx, m, y, dtype, cut, s);
     }
 }
@@ -693,6 +750,13 @@ int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x
     const size_t codes = whole(mx4_code_bytes(m, w->cols)), scales = whole(mx4_scale_bytes(m, w->cols));
     void *work = nullptr;
     const int variant = ctx_variant(ctx, "mx4");
+    if (variant == 0 && m <= 4 && !mx4_many_tiles(w)) {
+        hipStream_t s = ctx_stream(ctx);
+        if (x_dtype == DZ_F32) mx4_raw_launch<float>(w, x, (int)m, y, y_dtype, s);
+        else if (x_dtype == DZ_F16) mx4_raw_launch<half_t>(w, x, (int)m, y, y_dtype, s);
+        else mx4_raw_launch<bf16_t>(w, x, (int)m, y, y_dtype, s);
+        return ctx_launched(ctx, "mx4 linear");
+    }
     if (int32_t rc = ctx_workspace(ctx, codes + scales + mx4_parts(w, m, variant) * sizeof(float), &work)) return rc;
     uint8_t *q = (uint8_t *)work, *sx = q + codes;
     launch_mx4_quantize(x, x_dtype, (int)m, w->cols, q, sx, nullptr, ctx_stream(ctx));

@@ -39,6 +39,15 @@ __device__ __forceinline__ float mx4_scale_value(uint32_t byte) {
     return word_as_float(byte == 0 ? 0x00400000u : byte == 255 ? 0x7fc00000u : byte << 23);
 }
 
+// Eight codes of v / s, s a power of two given as the exponent field of a float (0: 2^-127).
+__device__ __forceinline__ uint32_t mx4_codes8(const float v[8], float s) {
+    uint32_t codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0], v[1], s, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2], v[3], s, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4], v[5], s, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], s, 3);
+}
+
 // One block of 32 values over a quad of lanes, eight a lane: the scale 2^e, e =
 // floor(log2 max|v|) - 2 (at least -127), as its byte, and the lane's eight codes,
 // v / 2^e to nearest even and at most 6 (what v_cvt_scalef32_pk_fp4_f32 gives; it
@@ -56,11 +65,7 @@ __device__ __forceinline__ uint32_t mx4_quantize8(const float v[8], uint32_t &sc
     const uint32_t exponent = most >> 23;
     const uint32_t byte = (exponent > 2 ? exponent : 2u) - 2;
     const float s = word_as_float(byte << 23);
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0], v[1], s, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2], v[3], s, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4], v[5], s, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6], v[7], s, 3);
+    const uint32_t codes = mx4_codes8(v, s);
     const bool finite = exponent < 255;
     scale = finite ? byte : 255u;
     return finite ? codes : 0u;

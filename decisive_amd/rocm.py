@@ -230,12 +230,12 @@ def load():
 
 
 def _addr(x) -> int | None:
-    if x is None:
-        return None
-    if isinstance(x, int):
+    if x is None or isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
+    try:
         return x.data_ptr()
+    except AttributeError:
+        pass
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
