@@ -528,14 +528,6 @@ __global__ __launch_bounds__(256) void fp8_join_kernel(const float *__restrict__
     fp8_store4(y, dtype, at, v, left);
 }
 
-}  // namespace
-
-void launch_fp8_join(const float *part, int splits, size_t count, void *y, int dtype, hipStream_t s) {
-    hipLaunchKernelGGL(fp8_join_kernel, dim3(cdiv(count, 1024)), dim3(256), 0, s, part, splits, count, y, dtype);
-}
-
-namespace {
-
 // What a product needs beside its operands: how its tile cuts k (`splits` runs of
 // blocks), and where the runs' sums go.
 struct Fp8Split {
@@ -553,7 +545,7 @@ void fp8_tile_form(const Fp8Weight &w, const uint8_t *q, const float *sx, int m,
                        splits > 1 ? cut.part : y, splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, per);
     if (splits > 1) {
         const size_t count = (size_t)m * w.rows;
-        launch_fp8_join(cut.part, splits, count, y, dtype, s);
+        hipLaunchKernelGGL(fp8_join_kernel, dim3(cdiv(count, 1024)), dim3(256), 0, s, cut.part, splits, count, y, dtype);
     }
 }
 

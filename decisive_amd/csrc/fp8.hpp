@@ -195,8 +195,6 @@ __device__ __forceinline__ void fp8_store4(void *__restrict__ y, int dtype, size
 // k-block kb kb_bytes further; sets *bad on a NaN code.
 void launch_fp8_retile(const uint8_t *codes, int count, int rows, int cols, uint8_t *dst, size_t matrix_bytes,
                        size_t tile_bytes, size_t kb_bytes, int *bad, hipStream_t s);
-// y (of `dtype`, `count` values) from the f32 sums of `splits` runs of blocks, [splits][count], added in their order.
-void launch_fp8_join(const float *part, int splits, size_t count, void *y, int dtype, hipStream_t s);
 // Copies block scales; sets *bad where one is not finite or is negative.
 void launch_fp8_scales(const float *src, float *dst, size_t n, int *bad, hipStream_t s);
 

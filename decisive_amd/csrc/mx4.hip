@@ -8,6 +8,7 @@
 // its additions of blocks f32's (random codes, scales within 2^10 of each other: 2.7e-8
 // off, relative, in the 2-norm), so that f32 outputs need no path of their own.
 #include <algorithm>
+#include <cmath>
 
 #include "../../include/decisive_rocm.h"
 #include "mx4.hpp"
@@ -289,15 +290,12 @@ __device__ __forceinline__ uint2_t mx4_round4(float4_t v, int dtype) {
 // are in flight. With KS = 1 a workgroup goes through several tiles, and the loads run
 // on into the next one while a tile's outputs are stored. Scales cost nothing: the matrix
 // unit adds the exponents. The groups' sums are added in group order, through LDS.
-// Where k is cut, unit b / tiles takes `per` of its blocks and writes their sums as f32
-// for fp8_join.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const uint8_t *__restrict__ scales, int n, int kbs,
                                                                      const uint8_t *__restrict__ q,
                                                                      const uint8_t *__restrict__ sx, int m,
-                                                                     void *__restrict__ y, int dtype, int tiles,
-                                                                     int units, int per) {
+                                                                     void *__restrict__ y, int dtype, int units) {
     constexpr int WAVES = WGM * WGN, TM = BM / WGM, TN = BN / WGN, MT = TM / 16, NT = TN / 16;
     constexpr int XPW = BM / 16 / WAVES, WPW = BN / 16 / WAVES;            // 1 KiB loads per wave and stage
     constexpr int XP = BM < 64 ? 1 : BM / 64, WP = BN < 64 ? 1 : BN / 64;  // panels of scale words
@@ -318,26 +316,22 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
     const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + group * PART;
 
-    // A unit of work: a tile and a run of its blocks of k.
+    // the operands change places every step, and the loads are NS steps ahead; steps past the last add nothing
+    const int steps = max(NS, (kbs + 2 * KS - 1) / (2 * KS) * 2);
+
+    // A unit of work is a tile.
     struct Unit {
-        int split, row0, col0, first, last, steps;
+        int row0, col0;
     };
     auto unit_of = [&](int id) {
-        Unit u;
         int tm, tn;
-        u.split = __builtin_amdgcn_readfirstlane(id / tiles);  // divisions leave uniform values in vector registers
-        u.first = u.split * per;
-        u.last = min(kbs, u.first + per);
-        // the operands change places every step, and the loads are NS steps ahead; steps past the last add nothing
-        u.steps = max(NS, (u.last - u.first + 2 * KS - 1) / (2 * KS) * 2);
-        xcd_tile(id - u.split * tiles, tiles, tiles_m, tiles_n, tm, tn);
-        u.row0 = __builtin_amdgcn_readfirstlane(tm) * BM;
-        u.col0 = __builtin_amdgcn_readfirstlane(tn) * BN;
-        return u;
+        xcd_tile(id, units, tiles_m, tiles_n, tm, tn);
+        // divisions leave uniform values in vector registers
+        return Unit{__builtin_amdgcn_readfirstlane(tm) * BM, __builtin_amdgcn_readfirstlane(tn) * BN};
     };
 
     // The loads run NS steps ahead of the products: their own unit and step, and what they read of it. Units past the
-    // last one, and blocks past a unit's last, load nothing (every offset out of range, zeros in LDS).
+    // last one, and blocks past k, load nothing (every offset out of range, zeros in LDS).
     int load_id = blockIdx.x, load_step = 0;
     Unit load = unit_of(load_id);
     int32x4_t rx, rw, rs[SPW];
@@ -362,8 +356,8 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
     open_unit();
     // Load p of a stage's PB.
     auto load_piece = [&](int stage, int p) {
-        const int kb = load.first + load_step * KS + group;
-        const bool live = load_id < units && kb < load.last;
+        const int kb = load_step * KS + group;
+        const bool live = load_id < units && kb < kbs;
         const uint32_t at = lds0 + stage * STAGE, past = live ? 0u : 0x80000000u, k = live ? (uint32_t)kb : 0u;
         if (p < XPW) {
             const int u = wave * XPW + p;
@@ -464,7 +458,7 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
 #pragma unroll
             for (int b = 0; b < MT; b++) acc[a][b] = float4_t{0.f, 0.f, 0.f, 0.f};
         for (int part = 0; part < 2; part++) {  // the last NS steps load the next unit's first
-            for (int i = part == 0 ? NS : 0; i < (part == 0 ? u.steps : NS); i += 2) {
+            for (int i = part == 0 ? NS : 0; i < (part == 0 ? steps : NS); i += 2) {
                 advance(two[0], two[1]);
                 advance(two[1], two[0]);
             }
@@ -504,7 +498,7 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
 #pragma unroll
         for (int b = 0; b < MT; b++) {
             const int row = u.row0 + wm * TM + b * 16 + j;
-            const size_t line = ((size_t)u.split * m + row) * n;
+            const size_t line = (size_t)row * n;
             if (dtype == 0) {
                 if (row >= m) continue;
 #pragma unroll
@@ -527,23 +521,16 @@ __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // no LDS write in flight when the block ends
 }
 
-// What a product needs beside its operands: how its tile cuts k (`splits` runs of
-// blocks), and where the runs' sums go.
-struct Mx4Split {
-    int splits = 1;
-    float *part = nullptr;  // [splits][m][n]
-};
-
+// With KS = 1 as many workgroups as fit the compute units at once go through the tiles.
 template <int BM, int BN, int WGM, int WGN, int KS, int NS>
 void mx4_tile_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
-                     Mx4Split cut, hipStream_t s) {
-    const unsigned tiles = cdiv(m, BM) * cdiv(w->rows, BN);
-    const int per = (int)cdiv(w->kbs, cut.splits), splits = (int)cdiv(w->kbs, per);
-    const unsigned units = tiles * splits, most = (unsigned)device_cus();
+                     hipStream_t s) {
+    constexpr int LDS = NS * KS * ((BM + BN) * 64 + ((BM < 64 ? 1 : BM / 64) + (BN < 64 ? 1 : BN / 64)) * 256);
+    constexpr int FIT = std::max(1, std::min(160 * 1024 / LDS, 32 / (WGM * WGN * KS)));
+    const unsigned units = cdiv(m, BM) * cdiv(w->rows, BN), most = (unsigned)device_cus() * FIT;
     hipLaunchKernelGGL((mx4_tile_kernel<BM, BN, WGM, WGN, KS, NS>), dim3(KS == 1 ? std::min(units, most) : units),
-                       dim3(WGM * WGN * KS * 64), 0, s, w->codes, w->scales, w->rows, w->kbs, q, sx, m,
-                       splits > 1 ? (void *)cut.part : y, splits > 1 ? (int)DZ_F32 : dtype, (int)tiles, (int)units, per);
-    if (splits > 1) launch_fp8_join(cut.part, splits, (size_t)m * w->rows, y, dtype, s);
+                       dim3(WGM * WGN * KS * 64), 0, s, w->codes, w->scales, w->rows, w->kbs, q, sx, m, y, dtype,
+                       (int)units);
 }
 
 void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
@@ -558,46 +545,61 @@ void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uin
         hipLaunchKernelGGL(mx4_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx, bad);
 }
 
-// The tiles, in the order of the "mx4" family's variants from kTile0 on.
+// The tiles, in the order of the "mx4" family's variants from kRows on, and the time of
+// a grid on each: f + c us a 128-block of k for the first tile of a compute unit, and
+// more_f + more_c a block for each further one, halfway between whole rounds of the
+// units and their mean (a unit's workgroups overlap). Fitted to 150 shapes drawn at
+// random (17 to 4000 rows, K 100 to 9600, N 40 to 14400, every type out), where the
+// choice is 0.9% slower than the best of these in the geometric mean and at most 13%.
+// Many workgroups a unit hide a short k's latencies, four or two groups of waves on a
+// long k spare it, larger tiles load less for each product. Measured (us, rows16 / 32x32
+// / 32x32k4 / 64x64 / 64x64k2 / 64x128 / 128x128 / 256x256):
+//   57 rows, K=679, N=1096     3.5 / 3.9 / 4.4 / 4.4 / 5.2 / 5.0 / 7.6 / 10
+//   95 rows, K=411, N=8289     7.1 / 5.3 / 9.1 / 6.0 / 7.9 / 6.0 / 8.8 / 11
+//   85 rows, K=1980, N=2137    4.9 / 5.3 / 5.3 / 6.3 / 6.6 / 7.8 / 9.8 / 17
+//   343 rows, K=4096, N=1024   - / 8.7 / 8.4 / 8.3 / 8.1 / 10.0 / 12.6 / 26
+//   847 rows, K=1193, N=3394   - / 11.7 / 23.4 / 9.0 / 11.8 / 8.7 / 9.9 / 15
+//   586 rows, K=4096, N=14336  - / 70 / 92 / 43 / 55 / 35 / 43 / 38
+//   8192 rows, K=N=4096        - / - / 335 / - / 178 / - / 130 / 81
 struct Mx4Tile {
     int bm, bn;
+    float f, c, more_f, more_c;
 };
-constexpr Mx4Tile kMx4Tiles[] = {{32, 32}, {64, 32}, {64, 64}, {64, 64}, {128, 128}, {256, 128}, {256, 256}};
-constexpr int kRowsVariants = 1, kTile0 = 1 + kRowsVariants, kTiles = 7;
+constexpr Mx4Tile kMx4Tiles[] = {{16, 16, 3.3f, 0.021f, 0.07f, 0.041f},   {32, 32, 3.6f, 0.101f, 0.35f, 0.041f},
+                                 {32, 32, 4.3f, 0.064f, 1.4f, 0.047f},    {64, 64, 3.9f, 0.141f, 1.1f, 0.103f},
+                                 {64, 64, 4.9f, 0.108f, 2.4f, 0.095f},    {64, 128, 4.4f, 0.190f, 1.6f, 0.180f},
+                                 {128, 128, 7.7f, 0.199f, 7.6f, 0.295f},  {256, 256, 13.2f, 0.62f, 0.0f, 1.6f}};
+constexpr int kRows = 1, kTiles = 8;
+constexpr int kMostRows = 160;  // that the rows kernel, which reads the weight again every 16, is measured for
 
-struct Mx4Pick {
-    int variant, splits;
-};
-
-Mx4Pick mx4_pick(int variant, int m, int n, int kbs) {
-    if (variant) return {variant, 1};
-    if (m <= 16) return {1, 1};
-    const size_t cus = (size_t)device_cus();
-    for (int i = kTiles - 1; i > 0; i--)
-        if ((size_t)cdiv(m, kMx4Tiles[i].bm) * cdiv(n, kMx4Tiles[i].bn) >= cus) return {kTile0 + i, 1};
-    return {kTile0, 1};
-}
-
-// f32 values that a product of m rows needs for its runs' sums.
-size_t mx4_parts(const dz_mx4_weight *w, size_t m, int variant) {
-    const int splits = mx4_pick(variant, (int)m, w->rows, w->kbs).splits;
-    return splits > 1 ? splits * m * w->rows : 0;
+int mx4_pick(int variant, int m, int n, int kbs) {
+    if (variant) return variant;
+    if (m <= 16) return kRows;
+    const float cus = (float)device_cus(), k = (float)kbs;
+    int best = kRows;
+    float least = 1e30f;
+    for (int i = m <= kMostRows ? 0 : 1; i < kTiles; i++) {
+        const Mx4Tile &t = kMx4Tiles[i];
+        const float each = (float)cdiv(m, t.bm) * (float)cdiv(n, t.bn) / cus;
+        const float rounds = std::max(1.0f, 0.5f * (each + std::ceil(each)));
+        const float us = t.f + t.c * k + (rounds - 1.0f) * (t.more_f + t.more_c * k);
+        if (us < least) least = us, best = kRows + i;
+    }
+    return best;
 }
 
 // The product of m > 0 rows of codes.
 void launch_mx4_product(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx, int m, void *y, int dtype,
-                        int variant, float *part, hipStream_t s) {
-    const Mx4Pick pick = mx4_pick(variant, m, w->rows, w->kbs);
-    const Mx4Split cut{pick.splits, part};
-    switch (pick.variant) {
-        case 1: return mx4_rows_launch(w, q, sx, m, y, dtype, s);
-        case 2: return mx4_tile_launch<32, 32, 2, 1, 4, 2>(w, q, sx, m, y, dtype, cut, s);
-        case 3: return mx4_tile_launch<64, 32, 2, 1, 4, 2>(w, q, sx, m, y, dtype, cut, s);
-        case 4: return mx4_tile_launch<64, 64, 2, 2, 4, 2>(w, q, sx, m, y, dtype, cut, s);
-        case 5: return mx4_tile_launch<64, 64, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 6: return mx4_tile_launch<128, 128, 2, 2, 2, 4>(w, q, sx, m, y, dtype, cut, s);
-        case 7: return mx4_tile_launch<256, 128, 4, 2, 1, 4>(w, q, sx, m, y, dtype, cut, s);
-        default: return mx4_tile_launch<256, 256, 2, 4, 1, 4>(w, q, sx, m, y, dtype, cut, s);
+                        int variant, hipStream_t s) {
+    switch (mx4_pick(variant, m, w->rows, w->kbs)) {
+        case kRows: return mx4_rows_launch(w, q, sx, m, y, dtype, s);
+        case 2: return mx4_tile_launch<32, 32, 2, 1, 1, 4>(w, q, sx, m, y, dtype, s);
+        case 3: return mx4_tile_launch<32, 32, 2, 1, 4, 2>(w, q, sx, m, y, dtype, s);
+        case 4: return mx4_tile_launch<64, 64, 2, 2, 1, 4>(w, q, sx, m, y, dtype, s);
+        case 5: return mx4_tile_launch<64, 64, 2, 2, 2, 4>(w, q, sx, m, y, dtype, s);
+        case 6: return mx4_tile_launch<64, 128, 1, 4, 1, 4>(w, q, sx, m, y, dtype, s);
+        case 7: return mx4_tile_launch<128, 128, 2, 2, 2, 4>(w, q, sx, m, y, dtype, s);
+        default: return mx4_tile_launch<256, 256, 2, 4, 1, 4>(w, q, sx, m, y, dtype, s);
     }
 }
 
@@ -731,12 +733,7 @@ int32_t mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q, con
     if (m > kMx4MostRows) return ctx_fail(ctx, DZ_INPUT_TOO_LONG, "input budget exceeded");
     if (int32_t rc = mx4_codes_ok(ctx, q, s)) return rc;
     if (m == 0) return DZ_OK;
-    const int variant = ctx_variant(ctx, "mx4");
-    const size_t parts = mx4_parts(w, m, variant);
-    void *work = nullptr;
-    if (parts)
-        if (int32_t rc = ctx_workspace(ctx, parts * sizeof(float), &work)) return rc;
-    launch_mx4_product(w, q, s, (int)m, y, y_dtype, variant, (float *)work, ctx_stream(ctx));
+    launch_mx4_product(w, q, s, (int)m, y, y_dtype, ctx_variant(ctx, "mx4"), ctx_stream(ctx));
     return ctx_launched(ctx, "mx4 linear");
 }
 
@@ -757,10 +754,10 @@ int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x
         else mx4_raw_launch<bf16_t>(w, x, (int)m, y, y_dtype, s);
         return ctx_launched(ctx, "mx4 linear");
     }
-    if (int32_t rc = ctx_workspace(ctx, codes + scales + mx4_parts(w, m, variant) * sizeof(float), &work)) return rc;
+    if (int32_t rc = ctx_workspace(ctx, codes + scales, &work)) return rc;
     uint8_t *q = (uint8_t *)work, *sx = q + codes;
     launch_mx4_quantize(x, x_dtype, (int)m, w->cols, q, sx, nullptr, ctx_stream(ctx));
-    launch_mx4_product(w, q, sx, (int)m, y, y_dtype, variant, (float *)(sx + scales), ctx_stream(ctx));
+    launch_mx4_product(w, q, sx, (int)m, y, y_dtype, variant, ctx_stream(ctx));
     return ctx_launched(ctx, "mx4 linear");
 }
 

@@ -2526,8 +2526,8 @@ const char *const kDeltaNames[] = {"chunked64", "chunked64-c32", "recurrent", "r
 const char *const kNormNames[] = {"fused", "separate"};
 const char *const kFp8Names[] = {"auto",  "rows16",  "rows32",  "32x32k4", "64x32k4",
                                  "64x64k4", "64x64", "64x64k2", "128x128", "256x128", "256x256"};
-const char *const kMx4Names[] = {"auto",    "rows16",  "32x32k4", "64x32k4", "64x64k4",
-                                 "64x64k2", "128x128", "256x128", "256x256"};
+const char *const kMx4Names[] = {"auto",  "rows16",  "32x32",  "32x32k4", "64x64",
+                                 "64x64k2", "64x128", "128x128", "256x256"};
 
 template <int W, int MPAD, bool G32, int NP>
 void gemv_launch_np(const Weight &w, const half_t *x, int m, float *y, hipStream_t s) {

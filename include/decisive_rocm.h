@@ -857,9 +857,11 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *                 groups of waves; f32 outputs of 256x256 take 256x128). For tests and benchmarks: "auto" picks by the
  *                 grid, dz_tune leaves it alone, and the variants add a row's blocks
  *                 in orders of their own, so their f32 sums agree to rounding)
- *   "mx4"         auto, rows16, 32x32k4, 64x32k4, 64x64k4, 64x64k2, 128x128,
- *                 256x128, 256x256 (products on microscaled 4-bit floating point: as the
- *                 "fp8" family's, and as little a tuner's matter) */
+ *   "mx4"         auto, rows16 (the weight streamed over 16 rows at a time), 32x32,
+ *                 32x32k4, 64x64, 64x64k2, 64x128, 128x128, 256x256 (tiles; k2, k4 and
+ *                 128x128 share the 128-blocks of k among two or four groups of waves:
+ *                 products on microscaled 4-bit floating point, as the "fp8" family's,
+ *                 and as little a tuner's matter) */
 int32_t dz_select_variant(dz_ctx *ctx, const char *family, const char *variant);
 
 #ifdef __cplusplus

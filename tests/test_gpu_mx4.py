@@ -213,7 +213,7 @@ def test_linear_against_64_bits(ctx, m, n, k, x_dtype):
     w.free()
 
 
-VARIANTS = ["rows16", "32x32k4", "64x32k4", "64x64k4", "64x64k2", "128x128", "256x128", "256x256"]
+VARIANTS = ["rows16", "32x32", "32x32k4", "64x64", "64x64k2", "64x128", "128x128", "256x256"]
 
 
 @pytest.mark.parametrize("variant", VARIANTS)
