@@ -29,7 +29,7 @@ struct AddNorm {
     uint8_t *q;
     void *s;
     int m, d, kbs;
-    float eps;
+    double over_d, eps;
     int zero_centered;
 };
 
@@ -71,9 +71,8 @@ __device__ __forceinline__ void norm_sum8(const AddNorm &a, size_t row, int k0, 
 
 // The normed values of eight, y where it is kept, and their codes.
 template <class T, bool MX>
-__device__ __forceinline__ void norm_codes8(const AddNorm &a, size_t row, int k0, float inverse, float v[8]) {
-    float w[8];
-    fp8_load8(a.w, k0, a.d, w);
+__device__ __forceinline__ void norm_codes8(const AddNorm &a, size_t row, int k0, float inverse, float v[8],
+                                            const float w[8]) {
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = (v[e] * inverse) * (a.zero_centered ? 1.0f + w[e] : w[e]);
     if (k0 + 8 > a.d)  // an infinite or NaN norm makes no values past the row
@@ -95,66 +94,138 @@ __device__ __forceinline__ void norm_codes8(const AddNorm &a, size_t row, int k0
     }
 }
 
-__device__ __forceinline__ double norm_block_sum(double v) {
-    __shared__ double part[kNormThreads / 64];
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
-    __syncthreads();
-    double all = 0.0;
-    for (int i = 0; i < kNormThreads / 64; i++) all += part[i];
-    return all;
+template <int CTRL>
+__device__ __forceinline__ double norm_dpp(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 
-// A workgroup takes a row, eight values a thread and piece: PIECES of them stay in
-// registers between the sum and the norm; with PIECES = 0, for longer rows, h is
-// read again (x and r where it is not kept).
-template <class T, bool MX, int PIECES>
+// What the lane WIDTH (16 or 32) away holds: both sides of a swap of rows, or halves, of two copies.
+template <int WIDTH>
+__device__ __forceinline__ double norm_swap(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t word[2] = {(uint32_t)b, (uint32_t)(b >> 32)};
+    uint32_t other[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const uint2_t t = __builtin_bit_cast(uint2_t, WIDTH == 16
+                                                          ? __builtin_amdgcn_permlane16_swap(word[i], word[i], false, false)
+                                                          : __builtin_amdgcn_permlane32_swap(word[i], word[i], false, false));
+        other[i] = (threadIdx.x & WIDTH) ? t[0] : t[1];
+    }
+    return __builtin_bit_cast(double, (uint64_t)other[1] << 32 | other[0]);
+}
+
+// The sum over the LANES lanes of a row, in each of them.
+template <int LANES>
+__device__ __forceinline__ double norm_sum(double v) {
+    v += norm_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+    v += norm_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+    v += norm_dpp<0x124>(v);  // row_ror:4
+    v += norm_dpp<0x128>(v);  // row_ror:8
+    if constexpr (LANES > 16) {
+        v += norm_swap<16>(v);
+        v += norm_swap<32>(v);
+    }
+    if constexpr (LANES > 64) {
+        __shared__ double part[kNormThreads / 64];
+        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = (part[0] + part[1]) + (part[2] + part[3]);
+        static_assert(LANES == kNormThreads && kNormThreads == 256, "four waves a row");
+    }
+    return v;
+}
+
+// 1 / sqrt(v) within some 2^-50: the unit's estimate and two steps of Newton's iteration, a third of what a square root
+// and a division of 64 bits take. 0 and infinity keep the estimate, which is exact there.
+__device__ __forceinline__ double norm_rsqrt(double v) {
+    double y = __builtin_amdgcn_rsq(v);
+    if (v > 0.0 && v < __builtin_huge_val()) {
+        const double half = 0.5 * v;
+        y = __builtin_fma(y, __builtin_fma(-half * y, y, 0.5), y);
+        y = __builtin_fma(y, __builtin_fma(-half * y, y, 0.5), y);
+    }
+    return y;
+}
+
+// LANES lanes take a row, eight values a lane and piece: PIECES of them stay in
+// registers between the sum and the norm, and up to two pieces of w are on the way with
+// them; with PIECES = 0, for longer rows, h is read again (x and r where it is not
+// kept). In the 4-bit form neighbouring rows are neighbours on one XCD, whose L2 joins
+// the 16 bytes that each writes of a chunk (us, 16384 rows of 4096 in bf16 104 against
+// 110 with the rows dealt out; in e4m3, whose rows lie apart, 102 against 96). A row a
+// workgroup: 1 row of 2560 in bf16 4.0 us, 229 4.8, both a launch and two trips to
+// memory; 16384 of 4096 95 us, 5.0 TB/s (f32 158, 5.5), the rate of a copy.
+template <class T, bool MX, int LANES, int PIECES>
 __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a) {
-    const size_t row = blockIdx.x;
-    const int end = a.kbs * 128;
-    constexpr int kStep = kNormThreads * 8;
+    constexpr int ROWS = kNormThreads / LANES, STEP = LANES * 8;
+    const size_t row = (size_t)(MX ? xcd_unit(blockIdx.x, gridDim.x) : (int)blockIdx.x) * ROWS + threadIdx.x / LANES;
+    if (LANES < kNormThreads && row >= (size_t)a.m) return;  // whole rows of lanes, and no barrier
+    const int end = a.kbs * 128, lane = threadIdx.x % LANES;
     double sum = 0.0;
-    float v[PIECES > 0 ? PIECES : 1][8];
+    constexpr int EARLY = PIECES <= 2 ? PIECES : 0;
+    float v[PIECES > 0 ? PIECES : 1][8], w[EARLY > 0 ? EARLY : 1][8];
     if constexpr (PIECES > 0) {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) norm_sum8<T>(a, row, threadIdx.x * 8 + i * kStep, v[i]);
+        for (int i = 0; i < EARLY; i++) fp8_load8(a.w, lane * 8 + i * STEP, a.d, w[i]);
+#pragma unroll
+        for (int i = 0; i < PIECES; i++) norm_sum8<T>(a, row, lane * 8 + i * STEP, v[i]);
 #pragma unroll
         for (int i = 0; i < PIECES; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) sum += (double)v[i][e] * (double)v[i][e];
     } else {
-        for (int k0 = threadIdx.x * 8; k0 < a.d; k0 += kStep) {
+        for (int k0 = lane * 8; k0 < a.d; k0 += STEP) {
             norm_sum8<T>(a, row, k0, v[0]);
 #pragma unroll
             for (int e = 0; e < 8; e++) sum += (double)v[0][e] * (double)v[0][e];
         }
     }
-    sum = norm_block_sum(sum);
-    const float inverse = (float)(1.0 / sqrt(sum / (double)a.d + (double)a.eps));
+    sum = norm_sum<LANES>(sum);
+    const float inverse = (float)norm_rsqrt(__builtin_fma(sum, a.over_d, a.eps));
     if constexpr (PIECES > 0) {
 #pragma unroll
         for (int i = 0; i < PIECES; i++) {
-            const int k0 = threadIdx.x * 8 + i * kStep;
-            if (k0 < end) norm_codes8<T, MX>(a, row, k0, inverse, v[i]);  // whole DPP rows of lanes
+            const int k0 = lane * 8 + i * STEP;
+            if (k0 >= end) break;  // whole DPP rows of lanes
+            if (EARLY == 0) fp8_load8(a.w, k0, a.d, w[0]);
+            norm_codes8<T, MX>(a, row, k0, inverse, v[i], w[EARLY > 0 ? i : 0]);
         }
     } else {
         AddNorm again = a;
-        if (a.r && a.h) again.x = a.h, again.r = nullptr;  // each thread reads back what it wrote
+        if (a.r && a.h) again.x = a.h, again.r = nullptr;  // each lane reads back what it wrote
         else again.h = nullptr;
-        for (int k0 = threadIdx.x * 8; k0 < end; k0 += kStep) {
+        for (int k0 = lane * 8; k0 < end; k0 += STEP) {
             norm_sum8<T>(again, row, k0, v[0]);
-            norm_codes8<T, MX>(a, row, k0, inverse, v[0]);
+            fp8_load8(a.w, k0, a.d, w[0]);
+            norm_codes8<T, MX>(a, row, k0, inverse, v[0], w[0]);
         }
     }
 }
 
+template <class T, bool MX, int LANES, int PIECES>
+void add_norm_form(const AddNorm &a, hipStream_t s) {
+    hipLaunchKernelGGL((add_norm_kernel<T, MX, LANES, PIECES>), dim3(cdiv(a.m, kNormThreads / LANES)),
+                       dim3(kNormThreads), 0, s, a);
+}
+
+// Short rows share a workgroup (16384 rows of 64 in bf16 4.8 us, a workgroup each 22.8);
+// rows up to 2048 have a wave each where there are many (us, wave / workgroup: 16384 rows
+// of 1111 in bf16 39 / 46; 1001 of them 8.0 / 5.7; 16384 of 4096 127 / 102).
 template <class T, bool MX>
 void add_norm_pieces(const AddNorm &a, hipStream_t s) {
-    const dim3 grid(a.m), block(kNormThreads);
-    if (a.d <= kNormThreads * 8) hipLaunchKernelGGL((add_norm_kernel<T, MX, 1>), grid, block, 0, s, a);
-    else if (a.d <= kNormThreads * 16) hipLaunchKernelGGL((add_norm_kernel<T, MX, 2>), grid, block, 0, s, a);
-    else if (a.d <= kNormThreads * 32) hipLaunchKernelGGL((add_norm_kernel<T, MX, 4>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((add_norm_kernel<T, MX, 0>), grid, block, 0, s, a);
+    if (a.d <= 128) return add_norm_form<T, MX, 16, 1>(a, s);
+    if (a.d <= 512) return add_norm_form<T, MX, 64, 1>(a, s);
+    if (a.m >= 4096 && a.d <= 1024) return add_norm_form<T, MX, 64, 2>(a, s);
+    if (a.m >= 4096 && a.d <= 2048) return add_norm_form<T, MX, 64, 4>(a, s);
+    if (a.d <= 2048) add_norm_form<T, MX, 256, 1>(a, s);
+    else if (a.d <= 4096) add_norm_form<T, MX, 256, 2>(a, s);
+    else if (a.d <= 8192) add_norm_form<T, MX, 256, 4>(a, s);
+    else if (a.d <= 12288) add_norm_form<T, MX, 256, 6>(a, s);
+    else add_norm_form<T, MX, 256, 0>(a, s);
 }
 
 template <bool MX>
@@ -180,7 +251,8 @@ int32_t add_rmsnorm(dz_ctx *ctx, const void *x, const void *residual, int32_t dt
     if (((uintptr_t)q & 15) != 0 || (mx && ((uintptr_t)s & 15) != 0))
         return ctx_fail(ctx, DZ_INVALID_PARAMETERS, "codes must be 16-byte aligned");
     if (rows == 0) return DZ_OK;
-    const AddNorm a{x, residual, sum, y, w, q, s, (int)rows, (int)d, (int)cdiv(d, 128), eps, zero_centered};
+    const AddNorm a{x, residual, sum, y, w, q, s, (int)rows, (int)d, (int)cdiv(d, 128), 1.0 / (double)d, (double)eps,
+                    zero_centered};
     if (mx) launch_add_norm<true>(a, dtype, ctx_stream(ctx));
     else launch_add_norm<false>(a, dtype, ctx_stream(ctx));
     return ctx_launched(ctx, "add rmsnorm");

@@ -230,12 +230,14 @@ def load():
 
 
 def _addr(x) -> int | None:
-    if x is None or isinstance(x, int):
-        return x
+    if x is None:
+        return None
     try:
         return x.data_ptr()
     except AttributeError:
         pass
+    if isinstance(x, int):
+        return x
     if hasattr(x, "ctypes"):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
