@@ -103,9 +103,12 @@ __device__ __forceinline__ void fp8_load8(const T *__restrict__ row, int k0, int
                 }
             }
         }
-    } else {
+    } else {  // all eight loads are under way together: past the row its last value again, and not used
+        T some[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = k0 + e < k ? (float)row[k0 + e] : 0.0f;
+        for (int e = 0; e < 8; e++) some[e] = row[k0 + e < k ? k0 + e : k - 1];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[e] = k0 + e < k ? (float)some[e] : 0.0f;
     }
 }
 

@@ -84,21 +84,27 @@ __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint8_t *__restr
 // ---- activations ---------------------------------------------------------------
 
 // A workgroup takes 64 rows of one 128-block, whose scale words it writes side by
-// side: 16 lanes a row and eight values a lane, four rows a wave and step. Codes go
-// out as 4-byte pieces; four lanes make the 16 bytes of a block.
-template <class T>
-__global__ __launch_bounds__(256) void mx4_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
-                                                           uint8_t *__restrict__ q, uint8_t *__restrict__ s, int *bad) {
+// side: 16 lanes a row and eight values a lane, EACH rows a lane. Codes go out as 4-byte
+// pieces; four lanes make the 16 bytes of a block. Bound by memory, sizeof(T) + 17/32
+// bytes a value: 16384 x 4096 bf16 26 us, 6.5 TB/s; a few rows 2.3 us, a launch's time.
+template <class T, int EACH>
+__global__ __launch_bounds__(1024 / EACH) void mx4_quantize_kernel(const T *__restrict__ x, int m, int k, int kbs,
+                                                                   uint8_t *__restrict__ q, uint8_t *__restrict__ s,
+                                                                   int *bad) {
     const int kb = blockIdx.x, piece = threadIdx.x % 16, k0 = kb * 128 + piece * 8;
-    const int panel = blockIdx.z * gridDim.y + blockIdx.y;
+    const size_t row0 = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * 64 + threadIdx.x / 16;
+    float v[EACH][8];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const size_t row = (size_t)panel * 64 + 16 * i + threadIdx.x / 16;
-        if (row >= (size_t)m) return;
-        float v[8];
-        fp8_load8(x + row * k, k0, k, v);
+    for (int i = 0; i < EACH; i++) {
+        const size_t row = row0 + i * (64 / EACH);
+        fp8_load8(x + (row < (size_t)m ? row : (size_t)m - 1) * k, k0, k, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const size_t row = row0 + i * (64 / EACH);
+        if (row >= (size_t)m) return;  // whole DPP rows of lanes
         uint32_t scale;
-        const uint32_t codes = mx4_quantize8(v, scale);
+        const uint32_t codes = mx4_quantize8(v[i], scale);
         *(uint32_t *)(q + mx4_code_at(row, kb, piece / 4, piece % 4, kbs)) = codes;
         if (piece % 4 == 0) {
             s[mx4_scale_at(row, kb, piece / 4, kbs)] = (uint8_t)scale;
@@ -533,16 +539,23 @@ void mx4_tile_launch(const dz_mx4_weight *w, const uint8_t *q, const uint8_t *sx
                        (int)units);
 }
 
-void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
+// Four rows a lane past four workgroups a compute unit (us, one / four: 4096 x 4096 bf16 9.4 / 8.0; 1001 x 4096 3.3 /
+// 3.6; 1001 x 1111 f16 3.0 / 5.0).
+template <class T>
+void mx4_quantize_form(const T *x, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
     const int kbs = (int)cdiv(k, 128);
     const unsigned panels = cdiv(m, 64), most = 32768;  // a grid's y ends at 65535
     const dim3 grid(kbs, std::min(panels, most), cdiv(panels, most));
-    if (dtype == DZ_F32)
-        hipLaunchKernelGGL(mx4_quantize_kernel<float>, grid, dim3(256), 0, s, (const float *)x, m, k, kbs, q, sx, bad);
-    else if (dtype == DZ_F16)
-        hipLaunchKernelGGL(mx4_quantize_kernel<half_t>, grid, dim3(256), 0, s, (const half_t *)x, m, k, kbs, q, sx, bad);
+    if ((size_t)kbs * panels > 4 * (size_t)device_cus())
+        hipLaunchKernelGGL((mx4_quantize_kernel<T, 4>), grid, dim3(256), 0, s, x, m, k, kbs, q, sx, bad);
     else
-        hipLaunchKernelGGL(mx4_quantize_kernel<bf16_t>, grid, dim3(256), 0, s, (const bf16_t *)x, m, k, kbs, q, sx, bad);
+        hipLaunchKernelGGL((mx4_quantize_kernel<T, 1>), grid, dim3(1024), 0, s, x, m, k, kbs, q, sx, bad);
+}
+
+void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uint8_t *sx, int *bad, hipStream_t s) {
+    if (dtype == DZ_F32) mx4_quantize_form((const float *)x, m, k, q, sx, bad, s);
+    else if (dtype == DZ_F16) mx4_quantize_form((const half_t *)x, m, k, q, sx, bad, s);
+    else mx4_quantize_form((const bf16_t *)x, m, k, q, sx, bad, s);
 }
 
 // The tiles, in the order of the "mx4" family's variants from kRows on, and the time of
