@@ -56,18 +56,25 @@ __device__ __forceinline__ void norm_store8(T *row, int k0, int d, const float v
     }
 }
 
-// Eight values of h = T(x + r) in f32, stored where the caller keeps them.
+// Eight values of x and of r, on the way.
 template <class T>
-__device__ __forceinline__ void norm_sum8(const AddNorm &a, size_t row, int k0, float v[8]) {
-    fp8_load8((const T *)a.x + row * a.d, k0, a.d, v);
-    if (a.r) {
-        float r[8];
-        fp8_load8((const T *)a.r + row * a.d, k0, a.d, r);
+struct NormLoad {
+    Fp8Raw<T> x, r;
+    __device__ __forceinline__ void load(const AddNorm &a, size_t row, int k0) {
+        x.load((const T *)a.x + row * a.d, k0, a.d);
+        if (a.r) r.load((const T *)a.r + row * a.d, k0, a.d);
+    }
+    // h = T(x + r) in f32, stored where the caller keeps it
+    __device__ __forceinline__ void add(const AddNorm &a, size_t row, int k0, float v[8]) const {
+        x.values(v);
+        if (!a.r) return;
+        float other[8];
+        r.values(other);
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = (float)(T)f32_rounded(v[e] + r[e]);
+        for (int e = 0; e < 8; e++) v[e] = (float)(T)f32_rounded(v[e] + other[e]);
         if (a.h) norm_store8((T *)a.h + row * a.d, k0, a.d, v);
     }
-}
+};
 
 // The normed values of eight, y where it is kept, and their codes.
 template <class T, bool MX>
@@ -167,19 +174,29 @@ __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a)
     const int end = a.kbs * 128, lane = threadIdx.x % LANES;
     double sum = 0.0;
     constexpr int EARLY = PIECES <= 2 ? PIECES : 0;
-    float v[PIECES > 0 ? PIECES : 1][8], w[EARLY > 0 ? EARLY : 1][8];
+    float v[PIECES > 0 ? PIECES : 1][8], w[8];
+    Fp8Raw<float> early[EARLY > 0 ? EARLY : 1];
     if constexpr (PIECES > 0) {
 #pragma unroll
-        for (int i = 0; i < EARLY; i++) fp8_load8(a.w, lane * 8 + i * STEP, a.d, w[i]);
+        for (int i = 0; i < EARLY; i++) early[i].load(a.w, lane * 8 + i * STEP, a.d);
+        // two pieces' loads are under way together; a store of h, which may lie in x or r, would hold them up
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) norm_sum8<T>(a, row, lane * 8 + i * STEP, v[i]);
+        for (int i0 = 0; i0 < PIECES; i0 += 2) {
+            NormLoad<T> some[2];
+#pragma unroll
+            for (int i = i0; i < i0 + 2 && i < PIECES; i++) some[i - i0].load(a, row, lane * 8 + i * STEP);
+#pragma unroll
+            for (int i = i0; i < i0 + 2 && i < PIECES; i++) some[i - i0].add(a, row, lane * 8 + i * STEP, v[i]);
+        }
 #pragma unroll
         for (int i = 0; i < PIECES; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) sum += (double)v[i][e] * (double)v[i][e];
     } else {
         for (int k0 = lane * 8; k0 < a.d; k0 += STEP) {
-            norm_sum8<T>(a, row, k0, v[0]);
+            NormLoad<T> some;
+            some.load(a, row, k0);
+            some.add(a, row, k0, v[0]);
 #pragma unroll
             for (int e = 0; e < 8; e++) sum += (double)v[0][e] * (double)v[0][e];
         }
@@ -191,17 +208,21 @@ __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a)
         for (int i = 0; i < PIECES; i++) {
             const int k0 = lane * 8 + i * STEP;
             if (k0 >= end) break;  // whole DPP rows of lanes
-            if (EARLY == 0) fp8_load8(a.w, k0, a.d, w[0]);
-            norm_codes8<T, MX>(a, row, k0, inverse, v[i], w[EARLY > 0 ? i : 0]);
+            if (EARLY == 0) early[0].load(a.w, k0, a.d);
+            early[EARLY > 0 ? i : 0].values(w);
+            norm_codes8<T, MX>(a, row, k0, inverse, v[i], w);
         }
     } else {
         AddNorm again = a;
         if (a.r && a.h) again.x = a.h, again.r = nullptr;  // each lane reads back what it wrote
         else again.h = nullptr;
         for (int k0 = lane * 8; k0 < end; k0 += STEP) {
-            norm_sum8<T>(again, row, k0, v[0]);
-            fp8_load8(a.w, k0, a.d, w[0]);
-            norm_codes8<T, MX>(a, row, k0, inverse, v[0], w[0]);
+            NormLoad<T> some;
+            some.load(again, row, k0);
+            early[0].load(a.w, k0, a.d);
+            some.add(again, row, k0, v[0]);
+            early[0].values(w);
+            norm_codes8<T, MX>(a, row, k0, inverse, v[0], w);
         }
     }
 }

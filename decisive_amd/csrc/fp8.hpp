@@ -83,33 +83,57 @@ typedef unsigned int uint4_any_t __attribute__((ext_vector_type(4), aligned(2)))
 typedef unsigned int uint2_any_t __attribute__((ext_vector_type(2), aligned(2)));
 typedef unsigned int uint4_bytes_t __attribute__((ext_vector_type(4), aligned(1)));
 
-// Eight consecutive values of a row from k0 on, as f32; past k zero.
+// Eight consecutive values of a row from k0 on as they lie in memory, past k zero. Nothing here waits for whole
+// vectors, so that several of these are under way together.
 template <class T>
-__device__ __forceinline__ void fp8_load8(const T *__restrict__ row, int k0, int k, float v[8]) {
-    if (k0 + 8 <= k) {
-        if constexpr (sizeof(T) == 4) {
-            const float4_t a = *(const float4_any_t *)(row + k0), b = *(const float4_any_t *)(row + k0 + 4);
-#pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = a[e], v[4 + e] = b[e];
-        } else {
-            const uint4_t w = *(const uint4_any_t *)(row + k0);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if constexpr (__is_same(T, half_t)) {
-                    const half2_t p = word_as_half2(w[e]);
-                    v[2 * e] = (float)p[0], v[2 * e + 1] = (float)p[1];
-                } else {
-                    v[2 * e] = word_as_float(w[e] << 16), v[2 * e + 1] = word_as_float(w[e] & 0xffff0000u);
-                }
+struct Fp8Raw {
+    uint4_t w[sizeof(T) / 2 > 1 ? 2 : 1];
+
+    __device__ __forceinline__ void load(const T *__restrict__ row, int k0, int k) {
+        if (k0 + 8 <= k) {
+            if constexpr (sizeof(T) == 4) {
+                w[0] = __builtin_bit_cast(uint4_t, *(const float4_any_t *)(row + k0));
+                w[1] = __builtin_bit_cast(uint4_t, *(const float4_any_t *)(row + k0 + 4));
+            } else {
+                w[0] = *(const uint4_any_t *)(row + k0);
             }
+            return;
         }
-    } else {  // all eight loads are under way together: past the row its last value again, and not used
-        T some[8];
+        w[0] = uint4_t{0, 0, 0, 0};
+        if constexpr (sizeof(T) == 4) w[1] = w[0];
+        if (k0 >= k) return;
+        T some[8];  // all loads together: past the row its last value again, and not used
 #pragma unroll
         for (int e = 0; e < 8; e++) some[e] = row[k0 + e < k ? k0 + e : k - 1];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = k0 + e < k ? (float)some[e] : 0.0f;
+        for (int e = 0; e < 8; e++) {
+            if constexpr (sizeof(T) == 4)
+                w[e / 4][e % 4] = k0 + e < k ? __builtin_bit_cast(uint32_t, some[e]) : 0u;
+            else
+                w[0][e / 2] |= k0 + e < k ? (uint32_t)__builtin_bit_cast(uint16_t, some[e]) << (16 * (e % 2)) : 0u;
+        }
     }
+    __device__ __forceinline__ void values(float v[8]) const {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if constexpr (sizeof(T) == 4) {
+                v[e] = word_as_float(w[0][e]), v[4 + e] = word_as_float(w[1][e]);
+            } else if constexpr (__is_same(T, half_t)) {
+                const half2_t p = word_as_half2(w[0][e]);
+                v[2 * e] = (float)p[0], v[2 * e + 1] = (float)p[1];
+            } else {
+                v[2 * e] = word_as_float(w[0][e] << 16), v[2 * e + 1] = word_as_float(w[0][e] & 0xffff0000u);
+            }
+        }
+    }
+};
+
+// Eight consecutive values of a row from k0 on, as f32; past k zero.
+template <class T>
+__device__ __forceinline__ void fp8_load8(const T *__restrict__ row, int k0, int k, float v[8]) {
+    Fp8Raw<T> raw;
+    raw.load(row, k0, k);
+    raw.values(v);
 }
 
 template <int CTRL>

@@ -93,18 +93,20 @@ __global__ __launch_bounds__(1024 / EACH) void mx4_quantize_kernel(const T *__re
                                                                    int *bad) {
     const int kb = blockIdx.x, piece = threadIdx.x % 16, k0 = kb * 128 + piece * 8;
     const size_t row0 = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * 64 + threadIdx.x / 16;
-    float v[EACH][8];
+    Fp8Raw<T> raw[EACH];
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
         const size_t row = row0 + i * (64 / EACH);
-        fp8_load8(x + (row < (size_t)m ? row : (size_t)m - 1) * k, k0, k, v[i]);
+        raw[i].load(x + (row < (size_t)m ? row : (size_t)m - 1) * k, k0, k);
     }
 #pragma unroll
     for (int i = 0; i < EACH; i++) {
         const size_t row = row0 + i * (64 / EACH);
         if (row >= (size_t)m) return;  // whole DPP rows of lanes
+        float v[8];
+        raw[i].values(v);
         uint32_t scale;
-        const uint32_t codes = mx4_quantize8(v[i], scale);
+        const uint32_t codes = mx4_quantize8(v, scale);
         *(uint32_t *)(q + mx4_code_at(row, kb, piece / 4, piece % 4, kbs)) = codes;
         if (piece % 4 == 0) {
             s[mx4_scale_at(row, kb, piece / 4, kbs)] = (uint8_t)scale;
@@ -167,14 +169,15 @@ __global__ __launch_bounds__(kMx4Waves * 64) void mx4_rows_kernel(const uint8_t 
         }
         __builtin_amdgcn_sched_barrier(0);  // the weight is under way before x is waited for
         if constexpr (RAW) {
-            float some[ROWS][8];
+            Fp8Raw<T> raw[ROWS];
 #pragma unroll
-            for (int r = 0; r < ROWS; r++)
-                fp8_load8((const T *)x + (size_t)min(r, m - 1) * k, kb0 * 128 + lane * 8, k, some[r]);
+            for (int r = 0; r < ROWS; r++) raw[r].load((const T *)x + (size_t)min(r, m - 1) * k, kb0 * 128 + lane * 8, k);
 #pragma unroll
             for (int r = 0; r < ROWS; r++) {
+                float some[8];
+                raw[r].values(some);
                 uint32_t scale;
-                s_codes[wave][r][lane] = mx4_quantize8(some[r], scale);
+                s_codes[wave][r][lane] = mx4_quantize8(some, scale);
                 if (lane % 4 == 0) s_scale[wave][r][lane / 4] = scale;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
