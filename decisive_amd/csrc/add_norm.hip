@@ -7,6 +7,8 @@
 // (d 2^-53 of it at most) is far below i's own, so that i, and with it every code,
 // does not depend on the order of the sum but for one row in some 10^7. Bound by
 // memory: x, r and h move once each and the codes once.
+#include <algorithm>
+
 #include "../../include/decisive_rocm.h"
 #include "mx4.hpp"
 #include "tiles.hpp"
@@ -169,8 +171,9 @@ __device__ __forceinline__ double norm_rsqrt(double v) {
 template <class T, bool MX, int LANES, int PIECES>
 __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a) {
     constexpr int ROWS = kNormThreads / LANES, STEP = LANES * 8;
-    const size_t row = (size_t)(MX ? xcd_unit(blockIdx.x, gridDim.x) : (int)blockIdx.x) * ROWS + threadIdx.x / LANES;
-    if (LANES < kNormThreads && row >= (size_t)a.m) return;  // whole rows of lanes, and no barrier
+    const size_t block = (size_t)blockIdx.y * gridDim.x + (MX ? xcd_unit(blockIdx.x, gridDim.x) : (int)blockIdx.x);
+    const size_t row = block * ROWS + threadIdx.x / LANES;
+    if (row >= (size_t)a.m) return;  // whole rows of lanes: all of a workgroup that has a barrier
     const int end = a.kbs * 128, lane = threadIdx.x % LANES;
     double sum = 0.0;
     constexpr int EARLY = PIECES <= 2 ? PIECES : 0;
@@ -229,8 +232,9 @@ __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a)
 
 template <class T, bool MX, int LANES, int PIECES>
 void add_norm_form(const AddNorm &a, hipStream_t s) {
-    hipLaunchKernelGGL((add_norm_kernel<T, MX, LANES, PIECES>), dim3(cdiv(a.m, kNormThreads / LANES)),
-                       dim3(kNormThreads), 0, s, a);
+    const unsigned blocks = cdiv(a.m, kNormThreads / LANES), most = 1u << 20;  // a grid has less than 2^32 threads a side
+    const dim3 grid(std::min(blocks, most), cdiv(blocks, most));
+    hipLaunchKernelGGL((add_norm_kernel<T, MX, LANES, PIECES>), grid, dim3(kNormThreads), 0, s, a);
 }
 
 // Short rows share a workgroup (16384 rows of 64 in bf16 4.8 us, a workgroup each 22.8);
