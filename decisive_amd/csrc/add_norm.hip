@@ -132,8 +132,8 @@ template <int LANES>
 __device__ __forceinline__ double norm_sum(double v) {
     v += norm_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
     v += norm_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
-    v += norm_dpp<0x124>(v);  // row_ror:4
-    v += norm_dpp<0x128>(v);  // row_ror:8
+    v += norm_dpp<0x141>(v);  // row_half_mirror, and not a rotation: every lane adds in the same order
+    v += norm_dpp<0x140>(v);  // row_mirror
     if constexpr (LANES > 16) {
         v += norm_swap<16>(v);
         v += norm_swap<32>(v);

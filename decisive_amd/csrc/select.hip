@@ -40,16 +40,17 @@ __device__ __forceinline__ double dpp_move_f64(double v) {
     const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
-// Over the 16 lanes of a row, in every lane: xor 1, xor 2, rotate 4, rotate 8.
+// Over the 16 lanes of a row, in every lane and in one order for all of them (rotations would give each lane a sum of
+// its own, and equal logits unequal scores): quads by xor 1 and xor 2, their halves and the row by mirroring.
 #define DZ_ROW_REDUCE(name, type, move, combine)        \
     __device__ __forceinline__ type name(type v) {      \
         type o = move<0xB1>(v);                         \
         v = combine;                                    \
         o = move<0x4E>(v);                              \
         v = combine;                                    \
-        o = move<0x124>(v);                             \
+        o = move<0x141>(v);                             \
         v = combine;                                    \
-        o = move<0x128>(v);                             \
+        o = move<0x140>(v);                             \
         return combine;                                 \
     }
 template <int CTRL>

@@ -139,6 +139,74 @@ def test_scores_closer_than_f32_can_tell(ctx):
             agree(ctx, rule_of(experts, 8, sigmoid), logits, rocm.F32, bias)
 
 
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("bias", [None, 0.0, 0.25, 1000.0])
+@pytest.mark.parametrize("experts,top,groups,keep", [(64, 8, 1, 1), (256, 8, 8, 4), (256, 16, 4, 2), (512, 16, 1, 1),
+                                                     (40, 5, 10, 3)])
+def test_more_candidates_than_fit(ctx, experts, top, groups, keep, bias, sigmoid):
+    """Rows whose scores are all equal, nearly equal, or equal but for a few: the lowest indices, or the few."""
+    rng = np.random.default_rng(experts + top)
+    logits = np.zeros((12, experts), np.float32)
+    logits[1] = rng.permutation(experts) * np.float32(2.0 ** -26)
+    logits[2, ::3] = 2.0 ** -24
+    logits[3, rng.permutation(experts)[:top + 3]] = 1
+    logits[4, experts // 2:] = -1
+    logits[5] = 3
+    logits[6] = -20 + rng.permutation(experts) * np.float32(2.0 ** -19)
+    logits[7:] = rng.integers(-2, 3, (5, experts)) * np.float32(0.5)
+    b = None if bias is None else np.full(experts, bias, np.float32)
+    for best in (1, 2):
+        agree(ctx, rule_of(experts, top, sigmoid, groups, keep, best), logits, rocm.F32, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("groups,keep,best", [(1, 1, 1), (8, 3, 1), (8, 3, 2)])
+def test_scores_that_64_bits_cannot_tell_apart(ctx, dtype, biased, groups, keep, best):
+    """A sigmoid's logits where it is 1, or 0, to 64 bits or nearly so; a softmax's far below the largest."""
+    rng = np.random.default_rng(11)
+    experts, top = 96, 6
+    logits = rng.standard_normal((12, experts)).astype(np.float32)
+    logits[0] = 40 + rng.permutation(experts)                   # all 1
+    logits[1] = rng.uniform(16, 40, experts)
+    logits[2, 50:] = rng.uniform(15, 38, experts - 50)
+    logits[3] = -rng.uniform(690, 720, experts)                 # the smallest scores, and 0
+    logits[4] = -rng.uniform(700, 760, experts)
+    logits[4, 20] = 0
+    logits[5] = -1000 - rng.permutation(experts)
+    logits[6] = -rng.uniform(600, 800, experts)
+    logits[6, 90] = 0
+    logits[7, 3:] = -2000                                       # a mask by a large number
+    logits[8] = rng.uniform(-60, 60, experts)
+    logits[9] = np.where(np.arange(experts) % 2, -710.0, -709.5)
+    logits[10, ::2] = 16.5
+    logits[11, 1:] = -745.5
+    bias = (0.01 * rng.standard_normal(experts)).astype(np.float32) if biased else None
+    for sigmoid in (0, 1):
+        for renorm in (0, 1):
+            agree(ctx, rule_of(experts, top, sigmoid, groups, keep, best, renorm), logits, dtype, bias)
+
+
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("experts,groups", [(64, 8), (240, 10), (256, 64), (512, 16)])
+def test_groups_closer_than_f32_can_tell(ctx, experts, groups, biased, sigmoid):
+    """The same values in every group but for 2^-26 here and there: the sums' order is decided far below f32."""
+    rng = np.random.default_rng(experts)
+    width = experts // groups
+    logits = np.zeros((30, experts), np.float32)
+    for t in range(30):
+        row = np.tile(np.sort(rng.standard_normal(width)).astype(np.float32) * np.float32(0.25), groups)
+        at = rng.integers(0, experts, groups)
+        row[at] += np.float32(2.0 ** -22) * rng.integers(-2, 3, groups).astype(np.float32)
+        logits[t] = row
+    bias = np.tile((0.1 * rng.standard_normal(width)).astype(np.float32), groups) if biased else None
+    for keep in (1, groups // 2):
+        top = min(4, keep * width)
+        for best in (1, 2):
+            agree(ctx, rule_of(experts, top, sigmoid, groups, keep, best), logits, rocm.F32, bias)
+
+
 def test_many_tokens(ctx):
     rng = np.random.default_rng(3)
     logits = (1.5 * rng.standard_normal((3001, 160))).astype(np.float32)
