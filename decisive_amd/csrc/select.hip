@@ -80,10 +80,13 @@ struct Scores {
         if (sigmoid) return 1.0 / (1.0 + exp(-(double)l));
         return l > kMasked ? exp((double)l - (double)most) / sum : 0.0;
     }
-    // the same in f32, 2^-20 of 1 off at most
+    // The same in f32, 2^-20 of 1 off at most: an exponent x log2 e is rounded by |x| 2^-23 at most, which e^x, or the
+    // sigmoid's distance from 0 or 1, is multiplied with, and |x| e^-|x| is below 0.37; the unit's 2^x and 1 / x are
+    // within 2^-22.
     __device__ __forceinline__ float near(float l, float over_sum) const {
-        if (sigmoid) return __builtin_amdgcn_rcpf(1.0f + expf(-l));
-        return l > kMasked ? expf(l - most) * over_sum : 0.0f;
+        constexpr float kLog2e = 1.44269504f;
+        if (sigmoid) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-l * kLog2e));
+        return __builtin_amdgcn_exp2f((l - most) * kLog2e) * over_sum;  // 0 for a masked logit
     }
 };
 
@@ -275,24 +278,39 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
             }
         }
         const int width = experts / rule.groups;
-        int g = j / width, at = j - g * width;  // of expert 16 i + j
+        if (width % 16 == 0) {  // a group is whole steps of 16 experts, the same for all lanes
+            int g = 0, at = 0;
 #pragma unroll
-        for (int i = 0; i < PER; i++) {
-            if (!(stays >> (g & 63) & 1)) key[i] = kMasked, open &= ~(1u << i);
-            at += 16;
-            while (at >= width) at -= width, g++;
+            for (int i = 0; i < PER; i++) {
+                if (!((uint32_t)stays & 1u << g)) key[i] = kMasked, open &= ~(1u << i);  // 32 groups at most
+                at += 16;
+                if (at == width) at = 0, g++;
+            }
+        } else {
+            int g = j / width, at = j - g * width;  // of expert 16 i + j
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                if (!(stays >> (g & 63) & 1)) key[i] = kMasked, open &= ~(1u << i);
+                at += 16;
+                while (at >= width) at -= width, g++;
+            }
         }
     }
 
     // the lanes' largest keys, and the top-th largest of them
-    float mine = kMasked, next = kMasked;  // and the next largest, where few lanes would let too many pass
+    float mine = kMasked;
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (PER > 1) next = fmaxf(next, fminf(mine, key[i]));
-        mine = fmaxf(mine, key[i]);
-    }
-    float line = row_max_f32(1 + row_not_below<1>(mine, mine) >= top ? mine : kMasked);
-    if (top > 8) {
+    for (int i = 0; i < PER; i++) mine = fmaxf(mine, key[i]);
+    float line;
+    if (top <= 8) {
+        line = row_max_f32(1 + row_not_below<1>(mine, mine) >= top ? mine : kMasked);
+    } else {  // the lanes' two largest: one of each would let too many pass
+        float first = kMasked, next = kMasked;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            next = fmaxf(next, fminf(first, key[i]));
+            first = fmaxf(first, key[i]);
+        }
         const int of_mine = 1 + (next >= mine) + row_not_below<1>(mine, mine) + row_not_below<1>(next, mine);
         const int of_next = 2 + row_not_below<1>(mine, next) + row_not_below<1>(next, next);
         line = row_max_f32(of_mine >= top ? mine : of_next >= top ? next : kMasked);
@@ -300,7 +318,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
     const float least = line - tol * fmaxf(1.0f, fabsf(line));
     int count = 0;
 #pragma unroll
-    for (int i = 0; i < PER; i++) count += key[i] >= least && key[i] > kMasked;
+    for (int i = 0; i < PER; i++) count += key[i] >= least;  // a line of nothing counts all, and is not sure
     const int total = row_sum_i32(count);
     const bool sure = !odd && line > kMasked && total <= kMostCandidates;
     int expert = 0;
@@ -316,7 +334,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
         slot -= count;
 #pragma unroll
         for (int i = 0; i < PER; i++)
-            if (key[i] >= least && key[i] > kMasked) {
+            if (key[i] >= least) {
                 at_row.expert[slot] = 16 * i + j;
                 if (!BIASED) at_row.value[slot] = (double)key[i];
                 slot++;
