@@ -166,8 +166,8 @@ __device__ __forceinline__ double norm_rsqrt(double v) {
 // kept). In the 4-bit form neighbouring rows are neighbours on one XCD, whose L2 joins
 // the 16 bytes that each writes of a chunk (us, 16384 rows of 4096 in bf16 104 against
 // 110 with the rows dealt out; in e4m3, whose rows lie apart, 102 against 96). A row a
-// workgroup: 1 row of 2560 in bf16 4.0 us, 229 4.8, both a launch and two trips to
-// memory; 16384 of 4096 95 us, 5.0 TB/s (f32 158, 5.5), the rate of a copy.
+// workgroup: 1 row of 2560 in bf16 3.6 us, 229 4.2, both a launch and two trips to
+// memory; 16384 of 4096 91-95 us, 5.0-5.2 TB/s (f32 158, 5.5), the rate of a copy.
 template <class T, bool MX, int LANES, int PIECES>
 __global__ __launch_bounds__(kNormThreads) void add_norm_kernel(const AddNorm a) {
     constexpr int ROWS = kNormThreads / LANES, STEP = LANES * 8;

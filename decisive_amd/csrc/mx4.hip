@@ -134,6 +134,9 @@ __device__ __forceinline__ float4_t mx4_mfma(uint4_t a, uint32_t sa, uint4_t b, 
 // quantizes its own blocks while their weights are on the way, four 128-blocks of a row
 // at once, eight values a lane as mx4_quantize_kernel does, and hands the codes to its
 // lanes as operands through LDS, which spares a launch. The same bits either way.
+// Bound by a launch and one trip to memory, then by the weight's bytes (us, from recorded
+// graphs over two weights: K=N=4096, 1 row as it is 3.1, 16 rows of codes 3.4; K=1024,
+// N=32000, 16 rows of codes, f32 out 4.4, 4.5 TB/s).
 constexpr int kMx4Waves = 8, kMx4Batch = 4;
 
 template <class T, int ROWS, int NT>
@@ -299,6 +302,13 @@ __device__ __forceinline__ uint2_t mx4_round4(float4_t v, int dtype) {
 // are in flight. With KS = 1 a workgroup goes through several tiles, and the loads run
 // on into the next one while a tile's outputs are stored. Scales cost nothing: the matrix
 // unit adds the exponents. The groups' sums are added in group order, through LDS.
+// 16384 rows, K=4096, N=14336, bf16 out, 256 x 256: 455-505 us, 3.8-4.2 PFLOP/s, where
+// the unit sustains 7.0 from registers on such operands. Bound by the loads into LDS (34
+// KiB a step and compute unit at 52-60 B/ns; loads alone take 385 us, products with the
+// barriers alone 318) together with the power that holds the clock at some 1.8 GHz; the
+// matrix unit is busy 0.55 of the cycles, LDS has no bank conflicts. Four waves of 128 x
+// 128 took 637, 256 x 128 tiles and 32x32x64 instructions more than 256 x 256. Shorter
+// products are the latency of their k-steps (1001 rows, K=1111, N=1777 7.1 us).
 template <int BM, int BN, int WGM, int WGN, int KS, int NS>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const uint8_t *__restrict__ scales, int n, int kbs,
@@ -580,16 +590,24 @@ void launch_mx4_quantize(const void *x, int dtype, int m, int k, uint8_t *q, uin
 struct Mx4Tile {
     int bm, bn;
     float f, c, more_f, more_c;
+    bool persistent;
 };
-constexpr Mx4Tile kMx4Tiles[] = {{16, 16, 3.3f, 0.021f, 0.07f, 0.041f},   {32, 32, 3.6f, 0.101f, 0.35f, 0.041f},
-                                 {32, 32, 4.3f, 0.064f, 1.4f, 0.047f},    {64, 64, 3.9f, 0.141f, 1.1f, 0.103f},
-                                 {64, 64, 4.9f, 0.108f, 2.4f, 0.095f},    {64, 128, 4.4f, 0.190f, 1.6f, 0.180f},
-                                 {128, 128, 7.7f, 0.199f, 7.6f, 0.295f},  {256, 256, 13.2f, 0.62f, 0.0f, 1.6f}};
+constexpr Mx4Tile kMx4Tiles[] = {
+    {16, 16, 3.3f, 0.021f, 0.07f, 0.041f, false}, {32, 32, 3.6f, 0.101f, 0.35f, 0.041f, true},
+    {32, 32, 4.3f, 0.064f, 1.4f, 0.047f, false},  {64, 64, 3.9f, 0.141f, 1.1f, 0.103f, true},
+    {64, 64, 4.9f, 0.108f, 2.4f, 0.095f, false},  {64, 128, 4.4f, 0.190f, 1.6f, 0.180f, true},
+    {128, 128, 7.7f, 0.199f, 7.6f, 0.295f, false}, {256, 256, 13.2f, 0.62f, 0.0f, 1.6f, true}};
 constexpr int kRows = 1, kTiles = 8;
 constexpr int kMostRows = 160;  // that the rows kernel, which reads the weight again every 16, is measured for
 
+// A grid has less than 2^32 threads: the forms with a workgroup of up to 512 a tile go up to 2^23 tiles.
+bool mx4_fits(int variant, int m, int n) {
+    const Mx4Tile &t = kMx4Tiles[variant - kRows];
+    return t.persistent || (size_t)cdiv(m, t.bm) * cdiv(n, t.bn) < (size_t)1 << 23;
+}
+
 int mx4_pick(int variant, int m, int n, int kbs) {
-    if (variant) return variant;
+    if (variant) return mx4_fits(variant, m, n) ? variant : kTiles;
     if (m <= 16) return kRows;
     const float cus = (float)device_cus(), k = (float)kbs;
     int best = kRows;
@@ -599,7 +617,7 @@ int mx4_pick(int variant, int m, int n, int kbs) {
         const float each = (float)cdiv(m, t.bm) * (float)cdiv(n, t.bn) / cus;
         const float rounds = std::max(1.0f, 0.5f * (each + std::ceil(each)));
         const float us = t.f + t.c * k + (rounds - 1.0f) * (t.more_f + t.more_c * k);
-        if (us < least) least = us, best = kRows + i;
+        if (us < least && mx4_fits(kRows + i, m, n)) least = us, best = kRows + i;
     }
     return best;
 }

@@ -427,13 +427,14 @@ int32_t dz_mx4_quantize(dz_ctx *ctx, const void *x_dev, int32_t x_dtype, size_t 
  * may not overlap x). Sums are f32 and rounded once; products of codes and their
  * sum over a block of 32 are exact. Where the products of a block, or a sum, leave
  * f32's range the output is infinite or NaN. The order of a row's sum may depend on
- * m. Uses the context workspace (run the call once before capturing it; one replay
- * at a time). m may be 0, and is at most 2^24. */
+ * m. From five rows on (from one on for weights of many rows) the quantized rows stand
+ * in the context workspace (run the call once before capturing it; one replay at a
+ * time). m may be 0, and is at most 2^24. */
 int32_t dz_mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x_dev, int32_t x_dtype, size_t m, void *y_dev,
                       int32_t y_dtype);
 /* dz_mx4_linear on activations already quantized (dz_mx4_quantize or
  * dz_add_rmsnorm_mx4 with k = cols(w)): several weights can share one quantization.
- * The same bits as dz_mx4_linear's, and the context workspace as there. */
+ * The same bits as dz_mx4_linear's; y may overlap neither array. No workspace. */
 int32_t dz_mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q_dev, const uint8_t *s_dev, size_t m,
                          void *y_dev, int32_t y_dtype);
 
@@ -535,7 +536,7 @@ typedef struct dz_moe_selection {
  * rank, is chosen only where nothing else is left (by the lowest index) and a masked
  * logit's score is 0; chosen scores that are all 0 have shares 0. A token with a logit
  * or a biased score that is NaN or +infinity gets the experts 0 .. top_k - 1 and NaN
- * shares. No other token is touched. tokens <= 2^24. */
+ * shares. No other token is touched. Results overlap nothing. tokens <= 2^24. */
 int32_t dz_moe_select(dz_ctx *ctx, const dz_moe_selection *rule, const void *logits_dev, int32_t dtype, size_t tokens,
                       const float *bias_dev, int32_t *ids_dev, float *shares_dev);
 /* dz_moe_forward on a choice already made (dz_moe_select's, or any other):
@@ -859,7 +860,8 @@ int32_t dz_tune(dz_ctx *ctx, uint32_t budget_ms, const char *cache_in, char *cac
  *                 in orders of their own, so their f32 sums agree to rounding)
  *   "mx4"         auto, rows16 (the weight streamed over 16 rows at a time), 32x32,
  *                 32x32k4, 64x64, 64x64k2, 64x128, 128x128, 256x256 (tiles; k2, k4 and
- *                 128x128 share the 128-blocks of k among two or four groups of waves:
+ *                 128x128 share the 128-blocks of k among two or four groups of waves;
+ *                 past 2^23 tiles 256x256 takes their place, as it does rows16's:
  *                 products on microscaled 4-bit floating point, as the "fp8" family's,
  *                 and as little a tuner's matter) */
 int32_t dz_select_variant(dz_ctx *ctx, const char *family, const char *variant);

@@ -151,6 +151,29 @@ def test_outputs_past_32_bits(ctx, y_dtype):
     torch.cuda.empty_cache()
 
 
+def test_a_form_whose_grid_would_be_too_large(ctx):
+    """8.4 million tiles of 32 x 32, of 512 threads each: more than a grid's 2^32 threads, so another form takes them."""
+    import torch
+    rng = np.random.default_rng(8)
+    m, n, k = 140001, 61441, 32
+    w, wide = make_weight(ctx, rng, n, k)
+    x = (0.1 * rng.standard_normal((m, k))).astype(np.float32)
+    y = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    xd = dev(x)
+    ctx.select_variant("mx4", "32x32k4")
+    try:
+        ctx.mx4_linear(w, xd, rocm.F32, m, y, rocm.BF16)
+        ctx.sync()
+    finally:
+        ctx.select_variant("mx4", "auto")
+    rows = ends(rng, 20, m, 20)
+    want, mags = product(values(*quantize(x[rows]), k), wide)
+    check(f64(y[torch.from_numpy(rows).cuda()]), want, mags, k, rocm.BF16)
+    w.free()
+    del y
+    torch.cuda.empty_cache()
+
+
 @pytest.mark.parametrize("form", ["fp8", "mx4"])
 @pytest.mark.parametrize("m,d", [(3, WIDEST), (LONGEST, 3), (LONGEST, 600), ((1 << 21) + 5, 2050)])
 def test_norms_of_the_widest_and_the_most_rows(ctx, form, m, d):
