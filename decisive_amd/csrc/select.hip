@@ -19,11 +19,11 @@
 // groups that stay are spread over the lanes. The k-th largest of the lanes' largest
 // scores is below the k-th largest of all: candidates are at or above it.
 //
-// Bound by the vector unit's issue, some 1500 instructions a wave of four tokens (us, 256
-// experts, bf16, eight by biased sigmoids in 4 of 8 groups: 16384 tokens 16.8, of which
-// groups 4.4 and the bias 1.0 (its 64-bit scores); 8 of 64 by softmax 8.4, 16 of 512 with
-// groups and a bias 27.8; reading the logits alone takes 2). A few tokens are a launch
-// and one wave's chain: 8.9, by softmax without groups 5.6, of 64 experts 4.1.
+// Bound by the vector unit's issue, some 1300 instructions a wave of four tokens with
+// their 64-bit ones, and by the chain of one wave (us, 256 experts, f32, eight by biased
+// sigmoids in 4 of 8 groups: 16384 tokens 16.8, of which groups 4.4 and the bias 1.0 (its
+// 64-bit scores); 8 of 64 8.4, 16 of 512 27.8; the logits' bytes alone would take 3.4). A
+// few tokens are a launch and that chain: 8.9, without groups and bias 5.6, of 64 4.1.
 #include "../../include/decisive_rocm.h"
 #include "fp8.hpp"
 #include "tiles.hpp"
