@@ -11,7 +11,7 @@
 //  - with one, f32 scores (2^-20 off at most) leave the experts that may be among the
 //    largest, some 11 of 256 for eight of them, and 64 bits order those;
 //  - groups are ranked in f32, and again in 64 bits only where one that stays lies
-//    within 2^-18 of one that does not.
+//    within 2^-18 (of the largest summand, where that is above 1) of one that does not.
 // What those tests do not cover (masked experts that have to be chosen, more candidates
 // than kMostCandidates) goes through 64 bits expert by expert.
 //
@@ -130,13 +130,14 @@ __device__ __attribute__((noinline)) int select_wide(const float *logits, const 
 }
 
 // Which groups stay, as bits, from the values of their experts (`value`, of type V): a group ranks by its largest one
-// or, with `sums`, by `score` of its two largest added. Also the least rank that stays and the largest that does not.
-// 16 / groups lanes take a group, or a lane several groups.
+// or by `score` of its two largest added. Also the least rank that stays, the largest that does not, and the largest
+// size of a lane's summands, which may cancel. 16 / groups lanes take a group, or a lane several groups.
 template <class V, class F, class G>
 __device__ __forceinline__ uint64_t select_groups(const dz_moe_selection &rule, V *ranks, F value, G score,
-                                                  V &least_kept, V &most_left) {
+                                                  V &least_kept, V &most_left, V &summand) {
     const int j = threadIdx.x % 16, width = rule.experts / rule.groups;
     const V nothing = -(V)__builtin_huge_val();
+    summand = 0;
     int parts = 1;
     while (parts * 2 * rule.groups <= 16) parts *= 2;
     for (int g = j / parts; g < rule.groups; g += 16 / parts) {
@@ -152,7 +153,12 @@ __device__ __forceinline__ uint64_t select_groups(const dz_moe_selection &rule, 
             second = max(max(second, s), min(first, f));
             first = max(first, f);
         }
-        if (rule.group_best == 2 && first > nothing) first = score(first) + (second > nothing ? score(second) : (V)0);
+        if (rule.group_best == 2 && first > nothing) {
+            const V other = second > nothing ? score(second) : (V)0;
+            first = score(first);
+            summand = max(summand, max(first, -other));  // the lower one is the larger if it is below 0
+            first += other;
+        }
         if (j % parts == 0) ranks[g] = first;
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -265,22 +271,23 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
 #pragma unroll
         for (int i = 0; i < PER; i++) keys[select_at(16 * i + j)] = key[i];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        float kept, left;
+        float kept, left, summand;
         uint64_t stays = select_groups<float>(
             rule, at_row.rank, [&](int e) { return keys[select_at(e)]; },
-            [&](float v) { return BIASED ? v : scores.near(v, over_sum); }, kept, left);
+            [&](float v) { return BIASED ? v : scores.near(v, over_sum); }, kept, left, summand);
         if (BIASED || odd || rule.group_best == 2) {
             kept = -row_max_f32(-kept);
             left = row_max_f32(left);
-            if (odd || !(kept - left > 0x1p-18f * fmaxf(1.0f, fabsf(kept)))) {
-                double wide_kept, wide_left;
+            summand = fmaxf(1.0f, BIASED ? row_max_f32(summand) : 1.0f);
+            if (odd || !(kept - left > 0x1p-18f * fmaxf(summand, fabsf(kept)))) {
+                double wide_kept, wide_left, wide_summand;
                 stays = select_groups<double>(
                     rule, at_row.wide_rank,
                     [&](int e) {
                         const float l = own[e];
                         return l > kMasked ? scores.of(l) + (BIASED ? (double)bias[e] : 0.0) : (double)kMasked;
                     },
-                    [&](double v) { return v; }, wide_kept, wide_left);
+                    [&](double v) { return v; }, wide_kept, wide_left, wide_summand);
             }
         }
         const int width = experts / rule.groups;

@@ -207,6 +207,19 @@ def test_groups_closer_than_f32_can_tell(ctx, experts, groups, biased, sigmoid):
             agree(ctx, rule_of(experts, top, sigmoid, groups, keep, best), logits, rocm.F32, bias)
 
 
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("size", [1e3, 1e6])
+@pytest.mark.parametrize("groups", [4, 32])
+def test_groups_whose_biases_cancel(ctx, groups, size, sigmoid):
+    """A group's two largest are some `size` and -`size`: in f32 each is off by the size's rounding, far more than what the
+    sums of scores differ by. In 64 bits the sums are those of two roundings to some 1e-10."""
+    rng = np.random.default_rng(groups)
+    width = 8
+    logits = rng.standard_normal((700, groups * width)).astype(np.float32)
+    bias = np.tile(np.array([size, -size] + [-4 * size] * (width - 2), np.float32), groups)
+    agree(ctx, rule_of(groups * width, 2, sigmoid, groups, groups // 4, 2), logits, rocm.F32, bias)
+
+
 def test_many_tokens(ctx):
     rng = np.random.default_rng(3)
     logits = (1.5 * rng.standard_normal((3001, 160))).astype(np.float32)
