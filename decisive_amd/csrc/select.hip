@@ -7,7 +7,8 @@
 //  - without a bias the scores order as their logits do, which are exact, but where 64
 //    bits cannot tell scores of different logits apart: those that are 0 count as one
 //    logit, and a row with others (a sigmoid's logit above 16, a softmax's 700 to 746
-//    below the largest) is chosen by scores;
+//    below the largest, one so near 0 that its neighbours in f32 lie within 2^-50 of it)
+//    is chosen by scores;
 //  - with one, f32 scores (2^-20 off at most) leave the experts that may be among the
 //    largest, some 11 of 256 for eight of them, and 64 bits order those;
 //  - groups are ranked in f32, and again in 64 bits only where one that stays lies
@@ -248,15 +249,24 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
     if constexpr (!BIASED) {
         const float zero = rule.sigmoid ? -709.79f : scores.most - 746.0f;  // at and below it a score is 0
         const float high = rule.sigmoid ? 16.0f : __builtin_huge_valf(), low = rule.sigmoid ? zero : scores.most - 700.0f;
+        // neighbours lie 2^-24 of their size apart, and exp's argument is rounded by 2^-53 of the largest logit's
+        const float tiny = 0x1p-26f * fmaxf(1.0f, fabsf(scores.most));
         float least = __builtin_huge_valf();
+        uint32_t nearest = ~0u;  // of the keys' sizes as bits, 0 the last of all
 #pragma unroll
-        for (int i = 0; i < PER; i++) least = fminf(least, 16 * i + j < experts ? key[i] : least);
-        if (scores.most > high || -row_max_f32(-least) < low) {  // hardly ever but for masks
+        for (int i = 0; i < PER; i++) {
+            least = fminf(least, 16 * i + j < experts ? key[i] : least);
+            const uint32_t size = (__builtin_bit_cast(uint32_t, key[i]) << 1) - 1;
+            nearest = size < nearest ? size : nearest;
+        }
+        const bool look = least < low || nearest < __builtin_bit_cast(uint32_t, tiny) << 1;
+        if (scores.most > high || row_sum_i32(look)) {  // hardly ever but for masks
             int odds = 0;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 const bool here = key[i] > kMasked;
-                odds |= here && (key[i] > high || (key[i] > zero && key[i] < low));
+                odds |= here && (key[i] > high || (key[i] > zero && key[i] < low) ||
+                                 (fabsf(key[i]) < tiny && key[i] != 0.0f));
                 key[i] = here ? fmaxf(key[i], zero) : kMasked;
             }
             odd = row_sum_i32(odds) != 0;

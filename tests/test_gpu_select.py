@@ -207,6 +207,23 @@ def test_groups_closer_than_f32_can_tell(ctx, experts, groups, biased, sigmoid):
             agree(ctx, rule_of(experts, top, sigmoid, groups, keep, best), logits, rocm.F32, bias)
 
 
+@pytest.mark.parametrize("dtype", [rocm.F32, rocm.BF16])
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("biased", [False, True])
+@pytest.mark.parametrize("groups,keep,best", [(1, 1, 1), (8, 3, 1), (8, 3, 2)])
+@pytest.mark.parametrize("most", [None, 3.0])
+def test_logits_so_near_0_that_their_scores_are_equal(ctx, most, groups, keep, best, biased, sigmoid, dtype):
+    """exp of any of these is 1, or exp(-most): equal scores, so the lower index."""
+    rng = np.random.default_rng(11)
+    tokens, experts = 40, 96
+    logits = rng.choice(np.array([0, -0.0, 1e-20, -1e-20, 3e-30, -2e-25, 1e-36], np.float32), (tokens, experts))
+    logits[::2, ::3] = rng.standard_normal((tokens // 2, experts // 3)) - 2.0
+    if most is not None:
+        logits[:, 70] = most
+    bias = np.zeros(experts, np.float32) if biased else None
+    agree(ctx, rule_of(experts, 6, sigmoid, groups, keep, best), logits, dtype, bias)
+
+
 @pytest.mark.parametrize("sigmoid", [0, 1])
 @pytest.mark.parametrize("size", [1e3, 1e6])
 @pytest.mark.parametrize("groups", [4, 32])
