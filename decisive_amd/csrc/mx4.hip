@@ -303,12 +303,14 @@ __device__ __forceinline__ uint2_t mx4_round4(float4_t v, int dtype) {
 // on into the next one while a tile's outputs are stored. Scales cost nothing: the matrix
 // unit adds the exponents. The groups' sums are added in group order, through LDS.
 // 16384 rows, K=4096, N=14336, bf16 out, 256 x 256: 455-505 us, 3.8-4.2 PFLOP/s, where
-// the unit sustains 7.0 from registers on such operands. Bound by the loads into LDS (34
-// KiB a step and compute unit at 52-60 B/ns; loads alone take 385 us, products with the
-// barriers alone 318) together with the power that holds the clock at some 1.8 GHz; the
-// matrix unit is busy 0.55 of the cycles, LDS has no bank conflicts. Four waves of 128 x
-// 128 took 637, 256 x 128 tiles and 32x32x64 instructions more than 256 x 256. Shorter
-// products are the latency of their k-steps (1001 rows, K=1111, N=1777 7.1 us).
+// the unit sustains 7.0 from registers on such operands. Each further 4096 of k takes 370
+// us (5.2 PFLOP/s), tiles' ends and 470 MB of outputs the other 120. Bound by power, which
+// holds the clock at some 1.8 GHz (zeros instead of random codes take 388), and by the
+// loads into LDS (34 KiB a step and compute unit; alone 385 us, 40 B/ns; the products with
+// the barriers alone 318); the matrix unit is busy 0.55 of the cycles, LDS has no bank
+// conflicts. Four waves of 128 x 128 took 637, 256 x 128 tiles and 32x32x64 instructions
+// more than 256 x 256; leaving a tile's stores under way into the next one's steps, the
+// same. Shorter products are the latency of their k-steps (1001 rows, K=1111, N=1777 7.1).
 template <int BM, int BN, int WGM, int WGN, int KS, int NS>
 __global__ __launch_bounds__(WGM *WGN *KS * 64) void mx4_tile_kernel(const uint8_t *__restrict__ codes,
                                                                      const uint8_t *__restrict__ scales, int n, int kbs,
