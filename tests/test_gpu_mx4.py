@@ -238,6 +238,34 @@ def test_every_variant_against_64_bits(ctx, variant, m, n, k):
     w.free()
 
 
+@pytest.mark.parametrize("y_dtype", [rocm.F32, rocm.BF16])
+@pytest.mark.parametrize("k", [1, 200, 513, 640, 1100])
+@pytest.mark.parametrize("variant,m,n", [("32x32", 1601, 2900), ("64x64", 1700, 4200), ("64x128", 2100, 5001),
+                                         ("256x256", 4100, 4400), ("128x128", 2300, 2200), ("32x32k4", 1001, 1100)])
+def test_tiles_in_turn_on_one_workgroup(ctx, variant, m, n, k, y_dtype):
+    """More tiles than the units hold at once (the last two forms launch a workgroup each), with fewer 128-blocks of k than
+    stages, as many, and an odd number."""
+    import torch
+    rng = np.random.default_rng(m + k)
+    w, wide = make_weight(ctx, rng, n, k)
+    x = rng.standard_normal((m, k)).astype(np.float32)
+    want, mags = product(values(*quantize(x), k), wide)
+    q, s = buffers(m, k)
+    ctx.mx4_quantize(dev(x), rocm.F32, m, k, q, s)
+    y = empty((m, n), _torch(y_dtype))
+    ctx.select_variant("mx4", variant)
+    try:
+        for _ in range(2):
+            y.fill_(float("nan"))
+            torch.cuda.synchronize()
+            ctx.mx4_linear_q4(w, q, s, m, y, y_dtype)
+            ctx.sync()
+            check(f64(y), want, mags, k, y_dtype)
+    finally:
+        ctx.select_variant("mx4", "auto")
+    w.free()
+
+
 @pytest.mark.parametrize("x_dtype", DTYPES)
 @pytest.mark.parametrize("m", [1, 3, 20, 70, 300])
 def test_a_row_that_is_not_finite_makes_its_own_outputs_nan(ctx, m, x_dtype):
