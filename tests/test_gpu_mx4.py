@@ -331,6 +331,30 @@ def test_scales_from_end_to_end_of_their_range(ctx, m):
     w.free()
 
 
+@pytest.mark.parametrize("y_dtype", DTYPES)
+@pytest.mark.parametrize("m", [1, 16, 40, 300])
+def test_results_below_the_smallest_normal_value(ctx, m, y_dtype):
+    """Outputs of some 2^-130 (f16: 2^-18) are rounded to subnormal values, not to 0. A subnormal f32 sum is off by half
+    its last place, 2^-150, for each block that is added."""
+    rng = np.random.default_rng(m)
+    n, k = 90, 260
+    codes = rng.integers(0, 16, (n, 288)).astype(np.uint8)
+    codes[:, k:] = 0
+    scales = np.full((n, 9), 127 - (16 if y_dtype == rocm.F16 else 50), np.uint8)
+    w = ctx.mx4_weight(dev((codes[:, 0::2] | codes[:, 1::2] << 4)[:, :130]), dev(scales), n, k)
+    x = rng.standard_normal((m, k)).astype(np.float32) * np.float32(2.0 ** (-8 if y_dtype == rocm.F16 else -88))
+    y = empty((m, n), _torch(y_dtype))
+    ctx.mx4_linear(w, dev(x), rocm.F32, m, y, y_dtype)
+    ctx.sync()
+    want, mags = product(values(*quantize(x), k), values(codes, scales, k))
+    got = f64(y)
+    tol = (1 + EPS[y_dtype]) * ((k / 32 + 32) * (2.0 ** -23 * mags + 2.0 ** -150)) + EPS[y_dtype] * np.abs(want) + LEAST[y_dtype]
+    assert (np.abs(got - want) <= tol).all()
+    if y_dtype != rocm.BF16:  # whose least value, 2^-133, is as large as these
+        assert np.count_nonzero(got) > 0.9 * got.size
+    w.free()
+
+
 def test_refusals(ctx):
     import torch
     n, k, m = 32, 256, 4
