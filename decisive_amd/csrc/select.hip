@@ -6,9 +6,9 @@
 // therefore the one that 64 bits make, but few experts need them:
 //  - without a bias the scores order as their logits do, which are exact, but where 64
 //    bits cannot tell scores of different logits apart: those that are 0 count as one
-//    logit, and a row with others (a sigmoid's logit above 16, a softmax's 700 to 746
-//    below the largest, one so near 0 that its neighbours in f32 lie within 2^-50 of it)
-//    is chosen by scores;
+//    logit, and a row with others (a sigmoid's logit above 16 or just above those, a
+//    softmax's 700 to 746 below the largest, one so near 0 that its neighbours in f32 lie
+//    within 2^-50 of it) is chosen by scores;
 //  - with one, f32 scores (2^-20 off at most) leave the experts that may be among the
 //    largest, some 11 of 256 for eight of them, and 64 bits order those;
 //  - groups are ranked in f32, and again in 64 bits only where one that stays lies
@@ -248,7 +248,8 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
     bool odd = false;  // scores of different logits may be equal
     if constexpr (!BIASED) {
         const float zero = rule.sigmoid ? -709.79f : scores.most - 746.0f;  // at and below it a score is 0
-        const float high = rule.sigmoid ? 16.0f : __builtin_huge_valf(), low = rule.sigmoid ? zero : scores.most - 700.0f;
+        // up to `low` some are: exp passes 64 bits' range at 709.7827, short of a sigmoid's `zero`
+        const float high = rule.sigmoid ? 16.0f : __builtin_huge_valf(), low = rule.sigmoid ? -709.0f : scores.most - 700.0f;
         // neighbours lie 2^-24 of their size apart, and exp's argument is rounded by 2^-53 of the largest logit's
         const float tiny = 0x1p-26f * fmaxf(1.0f, fabsf(scores.most));
         float least = __builtin_huge_valf();
