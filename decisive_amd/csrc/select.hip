@@ -7,8 +7,8 @@
 //  - without a bias the scores order as their logits do, which are exact, but where 64
 //    bits cannot tell scores of different logits apart: those that are 0 count as one
 //    logit, and a row with others (a sigmoid's logit above 16 or just above those, a
-//    softmax's 700 to 746 below the largest, one so near 0 that its neighbours in f32 lie
-//    within 2^-50 of it) is chosen by scores;
+//    softmax's 700 to 746 below the largest or any where that is past 2^22, one so near 0
+//    that its neighbours in f32 lie within 2^-50 of it) is chosen by scores;
 //  - with one, f32 scores (2^-20 off at most) leave the experts that may be among the
 //    largest, some 11 of 256 for eight of them, and 64 bits order those;
 //  - groups are ranked in f32, and again in 64 bits only where one that stays lies
@@ -247,6 +247,9 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
     wrong = row_sum_i32(wrong);
     bool odd = false;  // scores of different logits may be equal
     if constexpr (!BIASED) {
+        // below 2^22 `zero` is rounded by 2^-2 at most and lies under 745.14, where 64 bits make exp 0; from 2^25 on it does
+        // not always
+        odd = !rule.sigmoid && !(fabsf(scores.most) < 0x1p22f);
         const float zero = rule.sigmoid ? -709.79f : scores.most - 746.0f;  // at and below it a score is 0
         // up to `low` some are: exp passes 64 bits' range at 709.7827, short of a sigmoid's `zero`
         const float high = rule.sigmoid ? 16.0f : __builtin_huge_valf(), low = rule.sigmoid ? -709.0f : scores.most - 700.0f;
@@ -270,7 +273,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
                                  (fabsf(key[i]) < tiny && key[i] != 0.0f));
                 key[i] = here ? fmaxf(key[i], zero) : kMasked;
             }
-            odd = row_sum_i32(odds) != 0;
+            odd |= row_sum_i32(odds) != 0;
         }
     }
     const float tol = BIASED ? 0x1p-18f : 0.0f;  // of values up to 1; of larger ones their share

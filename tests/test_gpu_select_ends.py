@@ -25,3 +25,26 @@ def test_sigmoids_around_the_largest_exponential(ctx, groups, keep, best, expert
         logits[t, at] = border + rng.integers(-140, 0 if t % 2 else 20, experts // 4) * np.float32(2.0 ** -14)
     for renorm in (0, 1):
         agree(ctx, rule_of(experts, 6, 1, groups, keep, best, renorm), logits, rocm.F32, None)
+
+
+@pytest.mark.parametrize("experts", [24, 96])
+@pytest.mark.parametrize("groups,keep,best", GROUPS)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("exponent", [15, 22, 23, 24, 25, 26, 27, 28, 29, 31, 32, 33, 60, 126])
+def test_softmax_of_logits_whose_steps_are_large(ctx, exponent, sign, groups, keep, best, experts):
+    """f32 logits of 2^25 lie 4 apart, of 2^32 512: what 746 less than the largest is has no f32 of its own, and which
+    scores are 0 is for 64 bits to say."""
+    rng = np.random.default_rng(exponent)
+    tokens = 60
+    most = np.float32(sign * 2.0 ** exponent * 1.25)
+    step = float(np.spacing(abs(most)))
+    logits = np.empty((tokens, experts), np.float64)
+    for t in range(tokens):
+        below = np.rint(rng.uniform(746, 2000, experts) / step) + (2 if step > 300 else 0)
+        at = rng.permutation(experts)[:5]
+        below[at] = np.rint(rng.uniform(600, 760, 5) / step)
+        below[at[0]] = 0
+        logits[t] = float(most) - below * step
+    logits = logits.astype(np.float32)
+    for renorm in (0, 1):
+        agree(ctx, rule_of(experts, 6, 0, groups, keep, best, renorm), logits, rocm.F32, None)
