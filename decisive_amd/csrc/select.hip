@@ -240,7 +240,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const float b = 16 * i + j < experts ? bias[16 * i + j] : 0.0f;
-            wrong |= !(b < __builtin_huge_valf());
+            wrong |= key[i] > kMasked && !(b < __builtin_huge_valf());
             key[i] = key[i] > kMasked ? scores.near(key[i], over_sum) + b : kMasked;
         }
     }

@@ -533,10 +533,11 @@ typedef struct dz_moe_selection {
  * Equal values go to the lower index. Scores and ranks are held in 64 bits. ids_dev
  * int32 and shares_dev f32 [tokens x top_k], by falling c. An expert of logit (or
  * bias) -infinity is masked: it ranks below every other, adds nothing to its group's
- * rank, is chosen only where nothing else is left (by the lowest index) and a masked
- * logit's score is 0; chosen scores that are all 0 have shares 0. A token with a logit
- * or a biased score that is NaN or +infinity gets the experts 0 .. top_k - 1 and NaN
- * shares. No other token is touched. Results overlap nothing. tokens <= 2^24. */
+ * rank and is chosen only where nothing else is left (by the lowest index); a masked
+ * logit's score is 0 and its expert's bias counts for nothing. Chosen scores that are all
+ * 0 have shares 0. A token with a logit or a biased score that is NaN or +infinity gets
+ * the experts 0 .. top_k - 1 and NaN shares. No other token is touched. Results overlap
+ * nothing. tokens <= 2^24. */
 int32_t dz_moe_select(dz_ctx *ctx, const dz_moe_selection *rule, const void *logits_dev, int32_t dtype, size_t tokens,
                       const float *bias_dev, int32_t *ids_dev, float *shares_dev);
 /* dz_moe_forward on a choice already made (dz_moe_select's, or any other):

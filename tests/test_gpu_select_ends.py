@@ -1,5 +1,5 @@
-"""The choice of experts where scores of different logits are equal in 64 bits: against the definition of test_gpu_select,
-ids one by one."""
+"""The choice of experts where scores of different logits are equal in 64 bits, and where a bias is no number: against the
+definition of test_gpu_select, ids one by one."""
 import numpy as np
 import pytest
 
@@ -48,3 +48,20 @@ def test_softmax_of_logits_whose_steps_are_large(ctx, exponent, sign, groups, ke
     logits = logits.astype(np.float32)
     for renorm in (0, 1):
         agree(ctx, rule_of(experts, 6, 0, groups, keep, best, renorm), logits, rocm.F32, None)
+
+
+@pytest.mark.parametrize("dtype", [rocm.F32, rocm.F16, rocm.BF16])
+@pytest.mark.parametrize("sigmoid", [0, 1])
+@pytest.mark.parametrize("groups,keep,best", GROUPS)
+def test_a_bias_that_is_no_number_counts_where_its_expert_does(ctx, groups, keep, best, sigmoid, dtype):
+    """A NaN or infinite bias gives a token NaN shares, but not where the expert's logit masks it."""
+    rng = np.random.default_rng(23)
+    experts, tokens = 96, 30
+    logits = rng.standard_normal((tokens, experts)).astype(np.float32)
+    logits[::3, 40] = -np.inf
+    logits[1::3, [40, 7, 95]] = -np.inf
+    logits[4] = -np.inf
+    for special in ((np.nan,), (np.inf,), (np.nan, np.inf, np.nan), (np.inf, -np.inf, np.nan)):
+        bias = (0.1 * rng.standard_normal(experts)).astype(np.float32)
+        bias[[40, 7, 95][:len(special)]] = special
+        agree(ctx, rule_of(experts, 6, sigmoid, groups, keep, best), logits, dtype, bias)
