@@ -453,8 +453,10 @@ int32_t dz_mx4_linear_q4(dz_ctx *ctx, const dz_mx4_weight *w, const uint8_t *q_d
  *    scales (f32 [G x rows]) or dz_mx4_quantize's, for dz_fp8_linear_q8 and
  *    dz_mx4_linear_q4 with k = d.
  * Nothing else may overlap. A row of h that holds a value that is not finite has NaN
- * in its codes' scales, and so NaN products; no other row has. Codes and scales do not
- * depend on the order of a sum but where i lies within 2^-40 of a rounding border.
+ * in its codes' scales, and so NaN products; so has a finite row in the blocks where a y
+ * is not finite (past f32's range, or 0 times infinity: a row of zeros with eps = 0). No
+ * other row has. Codes and scales do not depend on the order of a sum but where i lies
+ * within 2^-40 of a rounding border.
  * eps finite and >= 0, d <= 2^20, rows <= 2^24; codes 16-byte aligned (mx4: scales too). */
 int32_t dz_add_rmsnorm_fp8(dz_ctx *ctx, const void *x_dev, const void *residual_dev, int32_t dtype, size_t rows,
                            size_t d, const float *w_dev, float eps, int32_t zero_centered, void *sum_dev, void *y_dev,

@@ -1,5 +1,5 @@
 """The norm with codes on the forms that a row's length and the number of rows pick: rows that are read twice, rows of a
-wave each. Bit by bit against the definition of test_gpu_add_norm."""
+wave each, and rows whose normed values are not finite. Bit by bit against the definition of test_gpu_add_norm."""
 import numpy as np
 import pytest
 
@@ -87,3 +87,30 @@ def test_many_rows_of_a_wave_each(ctx, form, dtype, m, d):
         assert np.array_equal(codes, wq) and bits_equal(scales, ws)
         assert np.array_equal(host(ctx, total.float()), h)
         assert np.array_equal(host(ctx, out.float()), kept)
+
+
+@pytest.mark.parametrize("form", ["fp8", "mx4"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [100, 300, 1500, 13001])
+def test_normed_values_that_are_not_finite_spoil_their_blocks(ctx, form, dtype, d):
+    """A row of zeros without an epsilon is 0 times infinity; a large weight takes a row's values past f32's range: such
+    blocks have NaN scales though the row itself is finite, and no other row or block has."""
+    rng = np.random.default_rng(d)
+    m = 9
+    x = rng.standard_normal((m, d)).astype(np.float32)
+    x[2] = 0
+    x[5, d // 2] = 0
+    x[6:, 70] = 9
+    w = np.ones(d, np.float32)
+    w[70] = 3e38
+    xd, x = rows_to(x, dtype)
+    for weight in (np.ones(d, np.float32), w):
+        codes, scales = call(ctx, form, xd, None, dtype, m, d, dev(weight), 0.0, False, None, None)
+        _, y = definition(x, None, weight, 0.0, False, dtype)
+        wq, ws = coded(form, y)
+        rows, want = (scales.T, ws.T) if form == "fp8" else (scales, ws)
+        nan = np.isnan(want) if form == "fp8" else want == 255
+        assert nan[2].sum() == -(-d // (128 if form == "fp8" else 32))
+        assert (nan[6:].sum(1) == (weight is w)).all()  # channel 70's block alone
+        assert np.array_equal(rows, want, equal_nan=form == "fp8")
+        assert np.array_equal(codes, wq)
