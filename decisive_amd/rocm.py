@@ -232,7 +232,9 @@ def load():
 def _addr(x) -> int | None:
     if x is None:
         return None
-    try:
+    if type(x) is int:  # 0.1 us; the exception below takes 0.3 of the 0.4 that it would be
+        return x
+    try:  # 0.17 us for a tensor, 0.23 where the attribute is looked for first
         return x.data_ptr()
     except AttributeError:
         pass
