@@ -103,14 +103,6 @@ __device__ __forceinline__ void norm_codes8(const AddNorm &a, size_t row, int k0
     }
 }
 
-template <int CTRL>
-__device__ __forceinline__ double norm_dpp(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-
 // What the lane WIDTH (16 or 32) away holds: both sides of a swap of rows, or halves, of two copies.
 template <int WIDTH>
 __device__ __forceinline__ double norm_swap(double v) {
@@ -130,10 +122,10 @@ __device__ __forceinline__ double norm_swap(double v) {
 // The sum over the LANES lanes of a row, in each of them.
 template <int LANES>
 __device__ __forceinline__ double norm_sum(double v) {
-    v += norm_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
-    v += norm_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
-    v += norm_dpp<0x141>(v);  // row_half_mirror, and not a rotation: every lane adds in the same order
-    v += norm_dpp<0x140>(v);  // row_mirror
+    v += dpp_move_f64<0xB1>(v);   // quad_perm [1,0,3,2]
+    v += dpp_move_f64<0x4E>(v);   // quad_perm [2,3,0,1]
+    v += dpp_move_f64<0x141>(v);  // row_half_mirror, and not a rotation: every lane adds in the same order
+    v += dpp_move_f64<0x140>(v);  // row_mirror
     if constexpr (LANES > 16) {
         v += norm_swap<16>(v);
         v += norm_swap<32>(v);

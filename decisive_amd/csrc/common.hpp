@@ -176,6 +176,15 @@ __device__ __forceinline__ int xcd_unit(int b, int nblocks) {
     return nblocks % kXcds == 0 ? (b % kXcds) * (nblocks / kXcds) + b / kXcds : b;
 }
 
+// What the lane that CTRL names of a row of 16 holds, in its two halves.
+template <int CTRL>
+__device__ __forceinline__ double dpp_move_f64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+
 // Sum over the 64 lanes of a wave, left in every lane: four DPP adds inside
 // each 16-lane row (xor 1, xor 2, rotate 4, rotate 8), then v_permlane16_swap
 // (odd rows of the first operand trade places with even rows of the second)

@@ -40,13 +40,6 @@ namespace {
 constexpr int kMostExperts = 512, kMostTop = 16, kMostGroups = 64, kMostCandidates = 32, kSelectWaves = 4;
 constexpr float kMasked = -__builtin_huge_valf();
 
-template <int CTRL>
-__device__ __forceinline__ double dpp_move_f64(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)b, CTRL, 0xF, 0xF, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
 // Over the 16 lanes of a row, in every lane and in one order for all of them (rotations would give each lane a sum of
 // its own, and equal logits unequal scores): quads by xor 1 and xor 2, their halves and the row by mirroring.
 #define DZ_ROW_REDUCE(name, type, move, combine)        \
