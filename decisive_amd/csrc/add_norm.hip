@@ -230,8 +230,16 @@ void add_norm_form(const AddNorm &a, hipStream_t s) {
 }
 
 // Short rows share a workgroup (16384 rows of 64 in bf16 4.8 us, a workgroup each 22.8);
-// rows up to 2048 have a wave each where there are many (us, wave / workgroup: 16384 rows
-// of 1111 in bf16 39 / 46; 1001 of them 8.0 / 5.7; 16384 of 4096 127 / 102).
+// rows up to 2048 have a wave each where there are many. us, wave / workgroup, e4m3:
+//   rows            1024        2048        4096        8192        16384
+//   1000, bf16      4.4 / 4.4   5.7 / 6.3   8.2 / 9.8   14.2 / 17.4 22.9 / 31.9
+//   1000, f32       5.0 / 4.7   7.3 / 6.5   11.9 / 11.6 20.1 / 20.3 36.1 / 36.4
+//   1111, bf16      6.5 / 5.2   8.1 / 7.3   12.1 / 12.2 21.3 / 22.2 33.9 / 39.5
+//   2000, bf16      6.6 / 5.6   8.9 / 8.1   14.7 / 13.4 25.7 / 25.4 44.4 / 44.3
+//   2000, f32       7.7 / 6.8   13.1 / 10.7 20.9 / 19.5 36.5 / 34.7 87.7 / 84.1
+// The line suits 16-bit rows; f32 ones past 1024 lose up to a tenth by it. 16384 of 4096
+// would be 127 / 102. Lengths that are no multiple of eight end in single values: 1001 rows
+// of 1111 in f16 with y kept 5.5, of 1110 5.4, of 1112 5.0, of 1152 4.9; one row 3.4 and 3.0.
 template <class T, bool MX>
 void add_norm_pieces(const AddNorm &a, hipStream_t s) {
     if (a.d <= 128) return add_norm_form<T, MX, 16, 1>(a, s);

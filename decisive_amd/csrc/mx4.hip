@@ -66,6 +66,7 @@ __global__ __launch_bounds__(256) void mx4_retile_kernel(const uint8_t *__restri
     }
 }
 
+// One value a thread, its code and its scale by loads of a byte: 4096 x 4096 46 us, 14336 x 4096 150-158 (1.7 TB/s).
 __global__ __launch_bounds__(256) void mx4_dequant_kernel(const uint8_t *__restrict__ codes,
                                                           const uint8_t *__restrict__ scales, int rows, int cols,
                                                           int kbs, float *__restrict__ y) {
@@ -305,9 +306,9 @@ __device__ __forceinline__ uint2_t mx4_round4(float4_t v, int dtype) {
 // 16384 rows, K=4096, N=14336, bf16 out, 256 x 256: 455-505 us, 3.8-4.2 PFLOP/s, where
 // the unit sustains 7.0 from registers on such operands. Each further 4096 of k takes 370
 // us (5.2 PFLOP/s), tiles' ends and 470 MB of outputs the other 120. Bound by power, which
-// holds the clock at some 1.8 GHz (zeros instead of random codes take 388), and by the
+// holds the clock at some 1.85 GHz (zeros instead of random codes take 388), and by the
 // loads into LDS (34 KiB a step and compute unit; alone 385 us, 40 B/ns; the products with
-// the barriers alone 318); the matrix unit is busy 0.55 of the cycles, LDS has no bank
+// the barriers alone 318); the matrix unit is busy 0.58 of the cycles, LDS has no bank
 // conflicts. Four waves of 128 x 128 took 637, 256 x 128 tiles and 32x32x64 instructions
 // more than 256 x 256; leaving a tile's stores under way into the next one's steps, the
 // same. Shorter products are the latency of their k-steps (1001 rows, K=1111, N=1777 7.1).
@@ -783,6 +784,17 @@ int32_t mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x, int32_t x
     const size_t codes = whole(mx4_code_bytes(m, w->cols)), scales = whole(mx4_scale_bytes(m, w->cols));
     void *work = nullptr;
     const int variant = ctx_variant(ctx, "mx4");
+    // Up to four rows as they are, one launch less. us, one launch / two, bf16 x (f32 where it differs), two weights in turn:
+    //   K x N          1 row       2           3                     4
+    //   1024 x 1024    2.7 / 4.1   2.9 / 4.2   3.4 / 4.2             3.4 / 4.2
+    //   4096 x 4096    2.8 / 5.4   3.0 / 5.5   3.5 / 5.5             3.5 / 5.5
+    //   2560 x 9216    4.7 / 7.0   5.1 / 7.0   5.9 / 7.1 (8.8)       6.0 / 7.1 (9.0)
+    //   9216 x 2560    5.1 / 8.6   5.9 / 8.7   7.0 / 8.7             7.1 / 8.7
+    //   4096 x 14336   6.8 / 10.9  7.6 / 11.0  8.3 / 10.9 (10.2)     8.4 / 11.0 (10.5)
+    //   1024 x 16384   4.9 / 5.4   5.8 / 5.3   7.3 / 5.4 (8.1)       7.4 / 5.4 (8.0)
+    // Every workgroup quantizes all of x, so it loses where many of them share a short k (the last line from two rows on),
+    // and on wide weights, whose form of four tiles a workgroup is built for codes only: 1024 x 32000 8.1 / 7.0, 4 rows
+    // 14.1 / 6.9; only 4096 x 32000 would gain (12.5 / 18.4, 4 rows of bf16 17.7 / 18.6).
     if (variant == 0 && m <= 4 && !mx4_many_tiles(w)) {
         hipStream_t s = ctx_stream(ctx);
         if (x_dtype == DZ_F32) mx4_raw_launch<float>(w, x, (int)m, y, y_dtype, s);

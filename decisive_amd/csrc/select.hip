@@ -9,7 +9,7 @@
 //    logit, and a row with others (a sigmoid's logit above 16 or just above those, a
 //    softmax's 700 to 746 below the largest or any where that is past 2^22, one so near 0
 //    that its neighbours in f32 lie within 2^-50 of it) is chosen by scores;
-//  - with one, f32 scores (2^-20 off at most) leave the experts that may be among the
+//  - with one, f32 scores (6 2^-24 off at most) leave the experts that may be among the
 //    largest, some 11 of 256 for eight of them, and 64 bits order those;
 //  - groups are ranked in f32, and again in 64 bits only where one that stays lies
 //    within 2^-18 (of the largest summand, where that is above 1) of one that does not.
@@ -24,7 +24,11 @@
 // their 64-bit ones, and by the chain of one wave (us, 256 experts, f32, eight by biased
 // sigmoids in 4 of 8 groups: 16384 tokens 16.8, of which groups 4.4 and the bias 1.0 (its
 // 64-bit scores); 8 of 64 8.4, 16 of 512 27.8; the logits' bytes alone would take 3.4). A
-// few tokens are a launch and that chain: 8.9, without groups and bias 5.6, of 64 4.1.
+// few tokens are a launch and that chain: 8.9, without groups and bias 5.5, of 64 4.1.
+// Where 64 bits choose all of a row the values decide the time (16384 tokens; one): plain
+// softmax 11.7; 5.5, of equal logits, of masks that leave fewer than eight or of logits
+// past 2^22 24-25; 13-14. Unbiased sigmoids in groups 15.5; 7.6, with a logit above 16 in
+// each row 38; 18. Biased sigmoids in groups 18; 9.0, with biases near 1000 26; 15.
 #include "../../include/decisive_rocm.h"
 #include "fp8.hpp"
 #include "tiles.hpp"
@@ -80,9 +84,10 @@ struct Scores {
         if (sigmoid) return 1.0 / (1.0 + exp(-(double)l));
         return l > kMasked ? exp((double)l - (double)most) / sum : 0.0;
     }
-    // The same in f32, 2^-20 of 1 off at most: an exponent x log2 e is rounded by |x| 2^-23 at most, which e^x, or the
-    // sigmoid's distance from 0 or 1, is multiplied with, and |x| e^-|x| is below 0.37; the unit's 2^x and 1 / x are
-    // within 2^-22.
+    // The same in f32, 6 u off at most, u = 2^-24: the exponent x log2 e, off by 2.3 |x| u (l - most, the product, the
+    // constant), costs 2.3 |x| e^-|x| u < 0.9 u (a sigmoid less); the unit's 2^x and 1 / x 2 u each of a value up to 1, the
+    // sum in f32, its quotient and the product with it u each: a softmax 0.9 + 2 + 3, a sigmoid 0.3 + 0.5 + 1 + 2.
+    // Measured over 2^28 logits each: 1.5 u and 1.8 u.
     __device__ __forceinline__ float near(float l, float over_sum) const {
         constexpr float kLog2e = 1.44269504f;
         if (sigmoid) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-l * kLog2e));
@@ -257,7 +262,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
             nearest = size < nearest ? size : nearest;
         }
         const bool look = least < low || nearest < __builtin_bit_cast(uint32_t, tiny) << 1;
-        if (scores.most > high || row_sum_i32(look)) {  // hardly ever but for masks
+        if (scores.most > high || row_sum_i32(look)) {  // masks, logits far apart, above 16 or next to 0
             int odds = 0;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
@@ -269,7 +274,9 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
             odd |= row_sum_i32(odds) != 0;
         }
     }
-    const float tol = BIASED ? 0x1p-18f : 0.0f;  // of values up to 1; of larger ones their share
+    // Of values up to 1; of larger ones, S, their share. A key is 6 u and its sum's rounding, u S, off (u = 2^-24), two
+    // keys 14 u S where 64 u S are allowed.
+    const float tol = BIASED ? 0x1p-18f : 0.0f;
 
     uint32_t open = 0;
 #pragma unroll
@@ -286,6 +293,7 @@ __global__ __launch_bounds__(kSelectWaves * 64) void select_kernel(const T *__re
             kept = -row_max_f32(-kept);
             left = row_max_f32(left);
             summand = fmaxf(1.0f, BIASED ? row_max_f32(summand) : 1.0f);
+            // two keys added are 14 u S and 2 u S for the addition off, two such ranks 32 u S: half of what is allowed
             if (odd || !(kept - left > 0x1p-18f * fmaxf(summand, fabsf(kept)))) {
                 double wide_kept, wide_left, wide_summand;
                 stays = select_groups<double>(

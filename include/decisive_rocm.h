@@ -427,9 +427,9 @@ int32_t dz_mx4_quantize(dz_ctx *ctx, const void *x_dev, int32_t x_dtype, size_t 
  * may not overlap x). Sums are f32 and rounded once; products of codes and their
  * sum over a block of 32 are exact. Where the products of a block, or a sum, leave
  * f32's range the output is infinite or NaN. The order of a row's sum may depend on
- * m. From five rows on (from one on for weights of many rows) the quantized rows stand
- * in the context workspace (run the call once before capturing it; one replay at a
- * time). m may be 0, and is at most 2^24. */
+ * m. From five rows on (from one on for weights of more than 64 rows a compute unit, or
+ * with a variant forced) the quantized rows stand in the context workspace (run the call
+ * once before capturing it; one replay at a time). m may be 0, and is at most 2^24. */
 int32_t dz_mx4_linear(dz_ctx *ctx, const dz_mx4_weight *w, const void *x_dev, int32_t x_dtype, size_t m, void *y_dev,
                       int32_t y_dtype);
 /* dz_mx4_linear on activations already quantized (dz_mx4_quantize or
