@@ -532,7 +532,8 @@ typedef struct dz_moe_selection {
  *   s_e = score of logit e,  c_e = s_e + bias_e
  *   the top_groups groups of largest rank stay; the top_k experts of largest c in them
  *   share_e = scale s_e, or scale s_e / (sum of the chosen s)
- * Equal values go to the lower index. Scores and ranks are held in 64 bits. ids_dev
+ * Equal values go to the lower index; scores and ranks are held in 64 bits, and those that
+ * their roundings there decide (some 2^-52 of them apart) may go either way. ids_dev
  * int32 and shares_dev f32 [tokens x top_k], by falling c. An expert of logit (or
  * bias) -infinity is masked: it ranks below every other, adds nothing to its group's
  * rank and is chosen only where nothing else is left (by the lowest index); a masked
